@@ -55,6 +55,20 @@ enum : uint32_t {
     ERRBIT_PEER_TIMEOUT = 1u << 4,  // a tensor-parallel peer did not arrive in time
 };
 
+// Makes a context's device current for a call and restores the caller's.
+struct DeviceGuard {
+    int prev = 0, dev;
+    explicit DeviceGuard(int device) : dev(device) {
+        FB_CUDA(cudaGetDevice(&prev));
+        if (prev != dev) FB_CUDA(cudaSetDevice(dev));
+    }
+    ~DeviceGuard() {
+        if (prev != dev) cudaSetDevice(prev);
+    }
+    DeviceGuard(const DeviceGuard &) = delete;
+    DeviceGuard &operator=(const DeviceGuard &) = delete;
+};
+
 // A device buffer owned by the library.
 struct DevBuf {
     void *ptr = nullptr;

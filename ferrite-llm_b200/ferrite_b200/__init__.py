@@ -26,6 +26,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "libferrite_b200.so")
 
 F32, F16, Q4_K, Q6_K, Q8_K, BF16 = 0, 1, 12, 14, 15, 30
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BANDS, ROTARY_YARN = 0, 1, 2, 3
 BLOCK_BYTES = {Q4_K: 144, Q6_K: 210, Q8_K: 292}
 
 # Every symbol include/ferrite_b200.h declares (checked by the CPU tests).
@@ -41,7 +42,8 @@ EXPORTED = (
     "fb_qtensor_upload_slice", "fb_comm_create", "fb_comm_handle", "fb_comm_open", "fb_comm_destroy",
     "fb_model_create_tp", "fb_model_tp_info", "fb_comm_set_timeout_ms", "fb_attn_prefill", "fb_gguf_config",
     "fb_model_load_gguf", "fb_model_forward_all", "fb_sample", "fb_top_logits", "fb_model_set_persistent",
-    "fb_model_step_timeline",
+    "fb_model_step_timeline", "fb_rotary_create", "fb_rotary_destroy", "fb_rotary_frequencies", "fb_rotary_apply",
+    "fb_kv_append", "fb_attn_tree_workspace", "fb_attn_tree", "fb_sample_rows",
 )
 COMM_HANDLE_BYTES = 64
 
@@ -57,6 +59,12 @@ class FerriteError(RuntimeError):
 class SamplerConfig(C.Structure):
     _fields_ = [("temperature", C.c_double), ("top_p", C.c_double), ("top_k", C.c_int), ("min_p", C.c_float),
                 ("repetition_penalty", C.c_float)]
+
+
+class RotaryConfig(C.Structure):
+    _fields_ = [("rot_dim", C.c_int), ("mode", C.c_int), ("scaling", C.c_int), ("theta", C.c_double),
+                ("factor", C.c_double), ("orig_ctx", C.c_int64), ("low", C.c_double), ("high", C.c_double),
+                ("amplitude", C.c_double)]
 
 
 class ModelConfig(C.Structure):
@@ -139,6 +147,14 @@ def _declare(L):
         "fb_top_logits": (i32, [vp, vp, i32, i64, i32, vp, vp]),
         "fb_model_set_persistent": (i32, [vp, i32, P(i32)]),
         "fb_model_step_timeline": (i32, [vp, vp, vp, vp, i64, P(i32), P(i32)]),
+        "fb_rotary_create": (i32, [P(RotaryConfig), P(vp)]),
+        "fb_rotary_destroy": (i32, [vp]),
+        "fb_rotary_frequencies": (i32, [vp, vp, i32, P(C.c_double)]),
+        "fb_rotary_apply": (i32, [vp, vp, i32, vp, i64, i64, vp, i64, i64, vp, i64, i32, i32]),
+        "fb_kv_append": (i32, [vp, vp, i32, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp] + [i32] * 8),
+        "fb_attn_tree_workspace": (i32, [vp] + [i32] * 7 + [P(i64)]),
+        "fb_attn_tree": (i32, [vp, i32, vp, i64, vp, vp, vp, vp, vp, vp, i32, vp, i64] + [i32] * 10 + [f32, vp, i64]),
+        "fb_sample_rows": (i32, [vp, i32, vp, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp]),
         "fb_model_create_tp": (i32, [vp, P(ModelConfig), vp, P(vp)]),
         "fb_model_tp_info": (i32, [vp, P(i32), P(i32), P(i32), P(i32)]),
     }
@@ -317,6 +333,92 @@ def attn_decode_noalloc(ctx: Context, q_ptr, k_ptr, v_ptr, bt_ptr, lens_ptr, out
     the library's device image; see include/ferrite_b200.h)."""
     _check(lib().fb_attn_decode_noalloc(ctx.h, q_ptr, k_ptr, v_ptr, bt_ptr, lens_ptr, out_ptr, batch, n_heads, n_kv,
                                         head_dim, page_size, max_pages, num_pages, max_seq_len, scale))
+
+
+class Rotary:
+    """Rotation frequencies of rotary positions (fb_rotary): the first rot_dim
+    dimensions of a head, mode 0 interleaved / 1 rotate-half, scaled for long
+    contexts by ROTARY_LINEAR (factor), ROTARY_BANDS or ROTARY_YARN (factor,
+    orig_ctx, low, high; see include/ferrite_b200.h).  amplitude 0: the
+    scaling's own."""
+
+    def __init__(self, rot_dim: int, theta: float, mode: int = 1, scaling: int = ROTARY_PLAIN, factor: float = 1.0,
+                 orig_ctx: int = 0, low: float = 0.0, high: float = 0.0, amplitude: float = 0.0):
+        self.h = None
+        cfg = RotaryConfig(rot_dim, mode, scaling, theta, factor, orig_ctx, low, high, amplitude)
+        h = C.c_void_p()
+        _check(lib().fb_rotary_create(C.byref(cfg), C.byref(h)))
+        self.h, self.rot_dim, self.mode = h, rot_dim, mode
+
+    def frequencies(self) -> tuple[np.ndarray, float]:
+        """(radians a position of each pair, amplitude)."""
+        f, a = np.zeros(self.rot_dim // 2), C.c_double()
+        _check(lib().fb_rotary_frequencies(self.h, _np(f), f.size, C.byref(a)))
+        return f, a.value
+
+    def close(self):
+        if self.h:
+            lib().fb_rotary_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def rotary_apply(ctx: Context, rotary: Rotary, dtype: int, x_ptr: int, x_token_stride: int, x_head_stride: int,
+                 y_ptr: int, y_token_stride: int, y_head_stride: int, positions_ptr: int, n_tok: int, n_heads: int,
+                 head_dim: int):
+    """y = x [n_tok][n_heads][head_dim] rotated at each token's position
+    (y_ptr == x_ptr with equal strides: in place)."""
+    _check(lib().fb_rotary_apply(ctx.h, rotary.h, dtype, x_ptr, x_token_stride, x_head_stride, y_ptr, y_token_stride,
+                                 y_head_stride, positions_ptr, n_tok, n_heads, head_dim))
+
+
+def kv_append(ctx: Context, rotary: Rotary | None, dtype: int, k_ptr: int, k_token_stride: int, v_ptr: int,
+              v_token_stride: int, row_offsets_ptr: int, seq_lens_ptr: int, positions_ptr: int, bt_ptr: int,
+              k_pages_ptr: int, v_pages_ptr: int, batch: int, n_rows: int, max_new: int, n_kv: int, head_dim: int,
+              page_size: int, max_pages: int, num_pages: int):
+    """The new rows of a ragged batch into the cache pages (k rotated at
+    positions_ptr, 0: at the cache position; rotary None: not rotated)."""
+    _check(lib().fb_kv_append(ctx.h, rotary.h if rotary is not None else None, dtype, k_ptr, k_token_stride, v_ptr,
+                              v_token_stride, row_offsets_ptr, seq_lens_ptr, positions_ptr or None, bt_ptr,
+                              k_pages_ptr, v_pages_ptr, batch, n_rows, max_new, n_kv, head_dim, page_size, max_pages,
+                              num_pages))
+
+
+def attn_tree_workspace(ctx: Context, batch: int, max_new: int, n_heads: int, n_kv: int, head_dim: int,
+                        page_size: int, max_seq_len: int) -> int:
+    """Bytes of the workspace attn_tree needs for these sizes."""
+    n = C.c_int64()
+    _check(lib().fb_attn_tree_workspace(ctx.h, batch, max_new, n_heads, n_kv, head_dim, page_size, max_seq_len,
+                                        C.byref(n)))
+    return n.value
+
+
+def attn_tree(ctx: Context, dtype: int, q_ptr: int, q_token_stride: int, k_ptr: int, v_ptr: int, bt_ptr: int,
+              row_offsets_ptr: int, seq_lens_ptr: int, mask_ptr: int, mask_words: int, out_ptr: int,
+              out_token_stride: int, batch: int, n_rows: int, max_new: int, n_heads: int, n_kv: int, head_dim: int,
+              page_size: int, max_pages: int, num_pages: int, max_seq_len: int, scale: float, workspace_ptr: int = 0,
+              workspace_bytes: int = 0):
+    """Attention of drafted trees over the paged cache: each new row sees its
+    sequence's prefix and the new rows of its mask bits (mask_ptr 0: a chain)."""
+    _check(lib().fb_attn_tree(ctx.h, dtype, q_ptr, q_token_stride, k_ptr, v_ptr, bt_ptr, row_offsets_ptr,
+                              seq_lens_ptr, mask_ptr or None, mask_words, out_ptr, out_token_stride, batch, n_rows,
+                              max_new, n_heads, n_kv, head_dim, page_size, max_pages, num_pages, max_seq_len, scale,
+                              workspace_ptr or None, workspace_bytes))
+
+
+def sample_rows(ctx: Context, dtype: int, logits_ptr: int, row_stride: int, rows: int, vocab: int,
+                temperature_ptr: int, top_k_ptr: int, top_p_ptr: int, min_p_ptr: int, uniform_ptr: int,
+                tokens_ptr: int, probs_ptr: int = 0):
+    """One token (int32) per logits row from the given uniforms, with per-row
+    settings (f32 / int32 arrays on the device, 0: off)."""
+    _check(lib().fb_sample_rows(ctx.h, dtype, logits_ptr, row_stride, rows, vocab, temperature_ptr or None,
+                                top_k_ptr or None, top_p_ptr or None, min_p_ptr or None, uniform_ptr, tokens_ptr,
+                                probs_ptr or None))
 
 
 # GGUF tensor names of one layer / of the whole model.

@@ -213,6 +213,118 @@ int fb_attn_decode_noalloc(fb_ctx *ctx, const float *q_dev,
                            int head_dim, int page_size, int max_pages,
                            int num_pages, int max_seq_len, float scale);
 
+/* ------------------------------------- verifying trees of drafted tokens ---
+ * The operators of one verification step for a ragged batch of sequences
+ * whose new rows are drafted trees (or single tokens, or prompt chunks):
+ * fb_rotary_apply on q, fb_kv_append for k and v, fb_attn_tree, and
+ * fb_sample_rows on the logits rows.  No reference counterpart: the reference
+ * verifies one chain, token by token (crates/ferrite-core/src/generation.rs:
+ * 340-535).  All four are stream ordered, allocate nothing, never
+ * synchronise, keep nothing between calls, and can be captured into CUDA
+ * graphs; they run on the context's device whichever device is current.
+ * dtype is FB_F32, FB_F16 or FB_BF16; strides count elements.
+ *
+ * The ragged batch: the new rows of sequence b are rows row_offsets[b] ..
+ * row_offsets[b + 1] - 1 (row_offsets_dev: batch + 1 int32, ascending); they
+ * stand at cache positions seq_lens[b] - n_b .. seq_lens[b] - 1, in order, so
+ * seq_lens_dev counts the new rows too.  n_b may be 0.  A sequence with
+ * n_b outside 0..max_new, rows outside 0..n_rows or seq_lens[b] outside
+ * n_b..max_pages * page_size (fb_attn_tree: ..max_seq_len) is left out and
+ * sets the error word's bad-position bit; a page id outside [0, num_pages)
+ * is neither read nor written and sets its bad-page bit.  Rows that belong to
+ * no sequence are not touched.  Page layouts as for fb_attn_decode, head_dim
+ * 64 or 128, page_size 32 or 64.  batch and n_rows may be 0 (nothing to do). */
+
+/* Rotation frequencies of rotary positions over the first rot_dim dimensions
+ * of a head: pair i of rot_dim / 2 turns by f_i = theta^(-2 i / rot_dim)
+ * radians a position, before scaling for long contexts:
+ *   FB_ROTARY_LINEAR  f_i / factor
+ *   FB_ROTARY_BANDS   by the turns t = orig_ctx f_i / 2 pi of the original
+ *                     context: f_i where t >= high, f_i / factor where t <=
+ *                     low, between them the mean of the two weighted by
+ *                     (t - low) / (high - low)
+ *   FB_ROTARY_YARN    f_i (1 - g) + f_i / factor g with the ramp g = (i - a) /
+ *                     (b - a) clamped to 0..1; a and b are the pair indices
+ *                     that make high and low turns over orig_ctx, rot_dim
+ *                     ln(orig_ctx / 2 pi turns) / 2 ln(theta), rounded outward
+ *                     and clamped to 0..rot_dim - 1; b at least a + 0.001
+ * amplitude multiplies cos and sin (0: 1, and for YARN 0.1 ln(factor) + 1).
+ * mode 0 pairs dimensions (2i, 2i + 1), mode 1 (i, i + rot_dim / 2).  A
+ * host-side object: no device memory, usable with every context and thread. */
+typedef struct fb_rotary fb_rotary;
+enum fb_rotary_scaling { FB_ROTARY_PLAIN = 0, FB_ROTARY_LINEAR = 1, FB_ROTARY_BANDS = 2, FB_ROTARY_YARN = 3 };
+typedef struct {
+    int rot_dim; /* even, 2..256 */
+    int mode;
+    int scaling;
+    double theta, factor;
+    int64_t orig_ctx;
+    double low, high;
+    double amplitude;
+} fb_rotary_config;
+int fb_rotary_create(const fb_rotary_config *cfg, fb_rotary **out);
+int fb_rotary_destroy(fb_rotary *r);
+/* The rot_dim / 2 scaled frequencies (radians a position) and the amplitude. */
+int fb_rotary_frequencies(const fb_rotary *r, double *freq_host, int capacity, double *amplitude);
+/* y = x rotated at positions_dev[token] (any int32; a negative one turns
+ * back), for x [n_tok][n_heads][head_dim] with the given token and head
+ * strides; dimensions from rot_dim on are copied.  Angles are reduced in
+ * binary64, so far positions keep full precision.  y_dev == x_dev with equal
+ * strides rotates in place; otherwise x and y must not overlap.  head_dim
+ * up to 1024. */
+int fb_rotary_apply(fb_ctx *ctx, const fb_rotary *r, int dtype, const void *x_dev, int64_t x_token_stride,
+                    int64_t x_head_stride, void *y_dev, int64_t y_token_stride, int64_t y_head_stride,
+                    const int32_t *positions_dev, int64_t n_tok, int n_heads, int head_dim);
+/* Writes the new rows k, v [n_rows][n_kv_heads][head_dim] (token strides;
+ * heads contiguous) into the cache pages as fp16, k first rotated at
+ * positions_dev[row] (r may be NULL: no rotation; positions_dev may be NULL:
+ * the cache position).  Drafted siblings share a position but not a place.
+ * Two rows must not name the same place of one page. */
+int fb_kv_append(fb_ctx *ctx, const fb_rotary *r, int dtype, const void *k_dev, int64_t k_token_stride,
+                 const void *v_dev, int64_t v_token_stride, const int32_t *row_offsets_dev,
+                 const int32_t *seq_lens_dev, const int32_t *positions_dev, const int32_t *block_table_dev,
+                 void *k_pages_dev, void *v_pages_dev, int batch, int n_rows, int max_new, int n_kv_heads,
+                 int head_dim, int page_size, int max_pages, int num_pages);
+/* Attention of the new rows over the cache, which already holds them
+ * (fb_kv_append): row i of sequence b sees the whole prefix (positions below
+ * seq_lens[b] - n_b) and those new rows j of its sequence whose bit j % 32 of
+ * word mask_dev[row * mask_words + j / 32] is set -- a drafted tree: its
+ * ancestors and itself.  mask_dev NULL: rows 0..i (a chain).  A row that sees
+ * nothing gets zeros; what a row does not see never reaches it, NaN and
+ * infinities included.  q [n_rows][n_heads][head_dim] and out of the same
+ * shape and dtype have token strides, heads contiguous.  Scores and sums
+ * in f32; q and the probabilities enter the tensor cores as fp16 high and low
+ * parts.  mask_words >= ceil(max_new / 32).  The workspace is the caller's
+ * (fb_attn_tree_workspace bytes for the same sizes, 16-byte aligned, contents
+ * ignored and clobbered): calls that may overlap need one each. */
+int fb_attn_tree_workspace(fb_ctx *ctx, int batch, int max_new, int n_heads, int n_kv_heads, int head_dim,
+                           int page_size, int max_seq_len, int64_t *bytes);
+int fb_attn_tree(fb_ctx *ctx, int dtype, const void *q_dev, int64_t q_token_stride, const void *k_pages_dev,
+                 const void *v_pages_dev, const int32_t *block_table_dev, const int32_t *row_offsets_dev,
+                 const int32_t *seq_lens_dev, const uint32_t *mask_dev, int mask_words, void *out_dev,
+                 int64_t out_token_stride, int batch, int n_rows, int max_new, int n_heads, int n_kv_heads,
+                 int head_dim, int page_size, int max_pages, int num_pages, int max_seq_len, float scale,
+                 void *workspace_dev, int64_t workspace_bytes);
+/* One token per logits row from given random numbers (fb_sample's rules for
+ * many rows with settings of their own, on the device): weights w = exp((x -
+ * max x) / T); of the row sorted by descending logit (equal logits in index
+ * order) min-p keeps w >= min_p, top-p of those the fewest first ones that
+ * hold top_p of their mass, top-k the first top_k; the token is the first in
+ * index order whose kept mass, its own included, exceeds u times the whole
+ * kept mass.  Every per-row array may be NULL (T = 1, filters off).  T <= 0:
+ * the largest logit.  top_k <= 0, top_p >= 1, min_p <= 0: off; top_p <= 0 or
+ * min_p > 1 keep the largest logit's token (the first of equal ones for
+ * top_p, all of them for min_p).  u is taken into [0, 1]; NaN settings count
+ * as off and NaN u as 0.  NaN logits are never selected, -inf ones only by T
+ * <= 0; +inf ones share the whole mass.  A row without any candidate gets token
+ * -1 and probability 0.  Masses are summed in 64-bit integers (weights in
+ * units of 2^-43), so results do not depend on the order of the work.
+ * probs_dev (may be NULL): the token's probability among the kept ones.
+ * row_stride in elements; vocab 1..524288. */
+int fb_sample_rows(fb_ctx *ctx, int dtype, const void *logits_dev, int64_t row_stride, int64_t rows, int vocab,
+                   const float *temperature_dev, const int32_t *top_k_dev, const float *top_p_dev,
+                   const float *min_p_dev, const float *uniform_dev, int32_t *tokens_dev, float *probs_dev);
+
 /* -------------------------------------------------------------- model --- */
 typedef struct {
     int n_layers, hidden, n_heads, n_kv_heads, head_dim, ffn, vocab;
