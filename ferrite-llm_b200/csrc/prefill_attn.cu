@@ -60,34 +60,6 @@ constexpr uint32_t TA_IDESC_S = umma_idesc_f16(TA_Q, TA_KB, false, true);
 constexpr uint32_t TA_IDESC_O = umma_idesc_f16(TA_Q, TA_HD, false, true);
 static_assert(TA_SMEM <= 227 * 1024, "prefill attention stages must fit");
 
-// Byte offset of 16-byte chunk c of row r in a K-major, 128-byte-swizzled
-// [rows][128 B] slab (8-row atoms of 1024 bytes, the TMA SWIZZLE_128B pattern).
-__device__ __forceinline__ uint32_t sw128_off(int r, int c) {
-    return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
-}
-
-// 2^x (the SFU's approximation: relative error about 2^-22).
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Eight f32 as fp16 hi parts and fp16 lo parts (x - hi).
-__device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const __half2 a = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-        const float2 af = __half22float2(a);
-        const __half2 b = __floats2half2_rn(__fsub_rn(x[2 * i], af.x), __fsub_rn(x[2 * i + 1], af.y));
-        h[i] = *reinterpret_cast<const uint32_t *>(&a);
-        l[i] = *reinterpret_cast<const uint32_t *>(&b);
-    }
-    hi = make_uint4(h[0], h[1], h[2], h[3]);
-    lo = make_uint4(l[0], l[1], l[2], l[3]);
-}
-
 // grid (ceil(T / 128), n_heads), TA_THREADS threads, TA_SMEM dynamic shared memory.
 // kmap: the K pool as rows of 64 keys ([num_pages * n_kv * 128] x 64 fp16),
 // vmap: the V pool as rows of 128 dims ([num_pages * n_kv * 64] x 128 fp16).
@@ -384,32 +356,14 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
 
 namespace fb {
 
-// fp16 pool viewed as rows of `inner` values, boxes of 64 values x box_rows
-// rows, 128-byte swizzle (the MN-major B layouts above).
-static CUtensorMap pool_map(const void *pool, int64_t rows, int64_t inner, uint32_t box_rows) {
-    auto encode = tensor_map_encoder();
-    FB_REQUIRE(encode != nullptr, "attn_prefill: cuTensorMapEncodeTiled is unavailable");
-    FB_REQUIRE(((uintptr_t)pool & 15) == 0, "attn_prefill: KV pools must be 16-byte aligned");
-    CUtensorMap map;
-    const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)inner * 2};
-    const cuuint32_t box[2] = {64, box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult cr = encode(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(pool), dims, strides, box,
-                               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    FB_REQUIRE(cr == CUDA_SUCCESS, "attn_prefill: tensor map encoding failed");
-    return map;
-}
-
 void launch_attn_prefill(fb_ctx *ctx, const float *q, const void *kpool, const void *vpool, const int32_t *bt,
                          int max_pages, int num_pages, int pos0, int T, int n_heads, int n_kv, float scale,
                          float *out) {
     FB_REQUIRE(T >= 1 && pos0 >= 0 && n_kv >= 1 && n_heads % n_kv == 0, "attn_prefill: bad shape");
     FB_REQUIRE((pos0 + T + TA_KB - 1) / TA_KB <= max_pages, "attn_prefill: positions exceed the block table");
     FB_REQUIRE((int64_t)num_pages * n_kv * TA_HD < ((int64_t)1 << 31), "attn_prefill: KV pool too large");
-    const CUtensorMap kmap = pool_map(kpool, (int64_t)num_pages * n_kv * TA_HD, TA_KB, TA_HD);
-    const CUtensorMap vmap = pool_map(vpool, (int64_t)num_pages * n_kv * TA_KB, TA_HD, TA_KB);
+    const CUtensorMap kmap = pool_map("attn_prefill", kpool, (int64_t)num_pages * n_kv * TA_HD, TA_KB, 64, TA_HD);
+    const CUtensorMap vmap = pool_map("attn_prefill", vpool, (int64_t)num_pages * n_kv * TA_KB, TA_HD, 64, TA_KB);
     FB_CUDA(cudaFuncSetAttribute(k_attn_prefill_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TA_SMEM));
     dim3 grid((unsigned)((T + TA_Q - 1) / TA_Q), (unsigned)n_heads);
     k_attn_prefill_tc<<<grid, TA_THREADS, TA_SMEM, ctx->stream>>>(kmap, vmap, q, bt, max_pages, num_pages, pos0, T,

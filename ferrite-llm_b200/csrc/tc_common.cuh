@@ -1,6 +1,6 @@
 // 5th-generation tensor-core (tcgen05 / TMEM) and TMA tensor-copy helpers
-// shared by the prefill GEMM (prefill.cu) and the prefill attention
-// (prefill_attn.cu).  Inline PTX only; no multicast anywhere.
+// shared by the prefill GEMM (prefill.cu), the prefill attention
+// (prefill_attn.cu) and the tree attention (attn_tree.cu).  Inline PTX only; no multicast anywhere.
 #pragma once
 
 #include <cuda.h>
@@ -8,6 +8,7 @@
 
 #include <mutex>
 
+#include "fb_internal.h"
 #include "kq_common.cuh"
 
 namespace fb {
@@ -35,6 +36,17 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t saddr, uint32_t 
     d |= (uint64_t)((sbo >> 4) & 0x3FFF) << 32;
     d |= (uint64_t)1 << 46;
     d |= (uint64_t)2 << 61;
+    return d;
+}
+// The same with 64-byte swizzle: 32 fp16 of M/N a K row (64 bytes), 8 K rows
+// a 512-byte atom.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw64(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+    d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
+    d |= (uint64_t)((sbo >> 4) & 0x3FFF) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)4 << 61;
     return d;
 }
 // kind::f16 instruction descriptor: fp16 A and B, f32 D; a_mn / b_mn select
@@ -92,6 +104,34 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// Byte offset of 16-byte chunk c of row r in a K-major, 128-byte-swizzled
+// [rows][128 B] slab (8-row atoms of 1024 bytes, the TMA SWIZZLE_128B pattern).
+__device__ __forceinline__ uint32_t sw128_off(int r, int c) {
+    return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
+}
+
+// 2^x (the SFU's approximation: relative error about 2^-22).
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Eight f32 as fp16 hi parts and fp16 lo parts (x - hi).
+__device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const __half2 a = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        const float2 af = __half22float2(a);
+        const __half2 b = __floats2half2_rn(__fsub_rn(x[2 * i], af.x), __fsub_rn(x[2 * i + 1], af.y));
+        h[i] = *reinterpret_cast<const uint32_t *>(&a);
+        l[i] = *reinterpret_cast<const uint32_t *>(&b);
+    }
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+    lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
 // cuTensorMapEncodeTiled from the driver (null where unavailable).
 inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     static std::once_flag once;
@@ -104,6 +144,27 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
             fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
     });
     return fn;
+}
+
+// fp16 pool viewed as rows of `inner` values, boxes of box_cols values x
+// box_rows rows; the swizzle is the box's row length, 128 bytes (64 values) or
+// 64 bytes (32 values): the MN-major operand layouts above.
+inline CUtensorMap pool_map(const char *who, const void *pool, int64_t rows, int64_t inner, uint32_t box_cols,
+                            uint32_t box_rows) {
+    auto encode = tensor_map_encoder();
+    FB_REQUIRE(encode != nullptr, std::string(who) + ": cuTensorMapEncodeTiled is unavailable");
+    FB_REQUIRE(((uintptr_t)pool & 15) == 0, std::string(who) + ": KV pools must be 16-byte aligned");
+    CUtensorMap map;
+    const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)inner * 2};
+    const cuuint32_t box[2] = {box_cols, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult cr = encode(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(pool), dims, strides, box,
+                               estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    FB_REQUIRE(cr == CUDA_SUCCESS, std::string(who) + ": tensor map encoding failed");
+    return map;
 }
 
 }  // namespace fb
