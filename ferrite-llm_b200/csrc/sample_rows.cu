@@ -20,10 +20,12 @@
 //  * otherwise: counts and approximate masses of 256 bins of the distance to
 //    the maximum narrow the cut down to a range of at most SR_LIST logits, all
 //    above it are kept.
-// The candidates are sorted in one CTA with exact weights.  Decisions that lean
-// on approximate masses are taken with their error on both sides; where that
-// leaves them open, the exact masses are summed.  Rows whose cut falls among
-// more than SR_LIST logits that no bin tells apart are bisected by key.
+// One CTA ranks the candidates against each other with exact weights (no sort:
+// 512 at most, a few lanes each).  In the first two cases it draws from them
+// alone and the cluster's other CTAs are gone by then.  A decision that leans on
+// approximate masses is taken with their error on both sides; where that leaves
+// it open, the exact mass of the row is summed.  Rows whose cut falls among more
+// than SR_LIST logits that no bin tells apart are bisected by key.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -35,10 +37,12 @@
 namespace fb {
 namespace cg = cooperative_groups;
 
-constexpr int SR_THREADS = 512;
+constexpr int SR_THREADS = 256;
+constexpr int SR_WARPS = SR_THREADS / 32;
 constexpr int SR_MAX_VOCAB = 1 << 19;
-constexpr int SR_LIST = 2048;   // candidates one CTA sorts
-constexpr int SR_TOPK = 512;    // top_k up to here goes by the threads' maxima
+constexpr int SR_LIST = 512;    // candidates one CTA ranks
+constexpr int SR_EACH = SR_LIST / SR_THREADS;
+constexpr int SR_TOPK = 256;    // top_k up to here goes by the threads' maxima
 constexpr int SR_BINS = 256;
 constexpr int SR_CLUSTER = 16;
 constexpr int SR_ROUNDS = 4;    // narrowings before the bisection
@@ -117,24 +121,20 @@ struct RowRule {
     // a step is a Taylor polynomial of e^(f ln2 / 32) (argument below 0.011: degree 5 is below 2^-53).
     // The maximum itself (infinite too) weighs 1, NaN 0.
     __device__ __forceinline__ double weight(float x, float mx, const double *table) const {
-        if (x == mx) return 1.0;
         const double z = __dmul_rn((double)x - (double)mx, scale);
-        if (!(z > -34400.0)) return 0.0;  // below 2^-1075, -inf, NaN
-        const double q = __dadd_rn(z, 6755399441055744.0);  // 1.5 * 2^52: the nearest integer in the low bits
+        const double y = fmax(z, -34400.0);  // 2^-1075 (NaN too)
+        const double q = __dadd_rn(y, 6755399441055744.0);  // 1.5 * 2^52: the nearest integer in the low bits
         const int n = __double2loint(q);
-        const double f = __dmul_rn(__dsub_rn(z, __dsub_rn(q, 6755399441055744.0)), 0.021660849392498290);  // ln2 / 32
+        const double f = __dmul_rn(__dsub_rn(y, __dsub_rn(q, 6755399441055744.0)), 0.021660849392498290);  // ln2 / 32
         double p = __fma_rn(f, 1.0 / 120.0, 1.0 / 24.0);
         p = __fma_rn(p, f, 1.0 / 6.0);
         p = __fma_rn(p, f, 0.5);
         p = __fma_rn(p, f, 1.0);
         p = __fma_rn(p, f, 1.0);
         p = __dmul_rn(p, table[n & 31]);
-        int e = n >> 5;
-        if (e < -1000) {
-            p = __dmul_rn(p, exp64_pow2(-200));
-            e += 200;
-        }
-        return __dmul_rn(p, exp64_pow2(e));
+        const int e = n >> 5, e0 = e / 2;  // (two factors: e reaches -1075; the second product rounds once)
+        p = __dmul_rn(__dmul_rn(p, exp64_pow2(e0)), exp64_pow2(e - e0));
+        return x == mx ? 1.0 : z > -34400.0 ? p : 0.0;
     }
     static __device__ __forceinline__ u64 units(double w) {
         if (!(w > 0.0)) return 0ull;
@@ -150,9 +150,9 @@ template <typename V, typename Op> __device__ __forceinline__ V sr_reduce(V v, V
     __syncthreads();
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
     __syncthreads();
-    V r = sh[threadIdx.x & 15];
+    V r = sh[threadIdx.x & (SR_WARPS - 1)];
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) r = op(r, __shfl_xor_sync(0xffffffffu, r, o));
+    for (int o = SR_WARPS / 2; o > 0; o >>= 1) r = op(r, __shfl_xor_sync(0xffffffffu, r, o));
     return r;
 }
 // Exclusive sum over the block in thread order; *all gets the total.
@@ -169,7 +169,7 @@ template <typename V> __device__ __forceinline__ V sr_scan(V v, V *sh, V *all) {
     __syncthreads();
     V before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < SR_THREADS / 32; w++) {
+    for (int w = 0; w < SR_WARPS; w++) {
         if (w < warp) before += sh[w];
         total += sh[w];
     }
@@ -178,7 +178,7 @@ template <typename V> __device__ __forceinline__ V sr_scan(V v, V *sh, V *all) {
 }
 
 struct SrShared {
-    u64 list[SR_LIST];                 // rank 0: the candidates
+    u64 list[SR_LIST], wt[SR_LIST];    // rank 0: the candidates and their weights
     u64 slot[2][SR_CLUSTER];           // pushed by every rank
     u64 red[32];
     double table[32];
@@ -186,14 +186,20 @@ struct SrShared {
     float unit_of[SR_CLUSTER];         // weight of one step of a rank's mass bins
     uint32_t cnt[2][SR_BINS], mass[2][SR_BINS];
     u64 cut;                           // pushed by rank 0
+    u64 kept_mass;
     unsigned n_list;                   // rank 0: candidates pushed
-    int state;                         // pushed by rank 0
-    int first_bin, last_bin, pick;
+    int first_bin, last_bin;
+    unsigned range_low;
     uint32_t kmin;
     unsigned range_count;
 };
 
-template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_rows(const SampleRowsArgs A) {
+__device__ __forceinline__ float sr_load(const float *p, int i) { return p[i]; }
+__device__ __forceinline__ float sr_load(const __half *p, int i) { return __half2float(p[i]); }
+__device__ __forceinline__ float sr_load(const __nv_bfloat16 *p, int i) { return __bfloat162float(p[i]); }
+
+static_assert(SR_BINS == SR_THREADS, "a thread a bin");
+template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_rows(const SampleRowsArgs A) {
     using W = SrWord<T>;
     constexpr int N = W::N;
     extern __shared__ __align__(16) uint32_t xs[];
@@ -214,7 +220,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_
     for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[0][i] = S.mass[0][i] = 0;
     if (A.vec) {
         constexpr int E = 4 * N;
-#pragma unroll 4
+#pragma unroll 5
         for (int v = tid; v < nwords / 4; v += SR_THREADS) {
             const int i = base + v * E;
             uint4 q = make_uint4(W::PAD, W::PAD, W::PAD, W::PAD);
@@ -249,17 +255,24 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_
             for (int k = 0; k < N; k++) tmax = fmaxf(tmax, f[k]);
         }
     }
-    // f(word index) over the words this thread loaded
-    auto loaded = [&](auto f) {
-        if (A.vec) {
-            for (int v = tid; v < nwords / 4; v += SR_THREADS)
-                for (int k = 0; k < 4; k++) f(4 * v + k);
-        } else {
-            for (int v = tid; v < nwords; v += SR_THREADS) f(v);
+    // f(logit, index) over the logits that a lane's threads of this warp loaded, for the lanes whose flag is set: the
+    // whole warp looks through one lane's logits at a time
+    auto loaded = [&](bool flag, auto f) {
+        for (uint32_t todo = __ballot_sync(0xffffffffu, flag); todo; todo &= todo - 1) {
+            const int src = (tid & ~31) + __ffs(todo) - 1;
+            for (int q = lane; q < ((A.words + 3) & ~3); q += 32) {
+                const int v = A.vec ? 4 * (src + SR_THREADS * (q >> 2)) + (q & 3) : src + SR_THREADS * q;
+                if (v >= nwords) continue;
+                float g[N];
+                W::get(xs[v], g);
+#pragma unroll
+                for (int k = 0; k < N; k++) f(g[k], base + v * N + k);
+            }
         }
     };
     // f(logit, index) over this thread's run of consecutive logits
     auto own = [&](auto f) {
+#pragma unroll 4
         for (int j = 0; j < A.words; j++) {
             const int v = tid * A.words + j;
             float q[N];
@@ -288,12 +301,8 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_
         // the first of the largest logits (a row of -inf has one, a row of NaN none)
         u64 first = ~0ull;
         if (rule.greedy)
-            loaded([&](int v) {
-                float q[N];
-                W::get(xs[v], q);
-#pragma unroll
-                for (int k = 0; k < N; k++)
-                    if (q[k] == mx) first = min(first, (u64)(base + v * N + k));
+            loaded(tmax == mx, [&](float v, int i) {
+                if (v == mx) first = min(first, (u64)i);
             });
         first = sr_reduce(first, S.red, [](u64 a, u64 b) { return a < b ? a : b; });
         if (tid == 0) cl.map_shared_rank(&S, 0)->slot[0][rank] = first;
@@ -341,12 +350,15 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_
     };
     auto rough_mass = [&]() {  // of this CTA's survivors
         float m = 0.f;
+#pragma unroll 4
         for (int v = tid; v < nwords; v += SR_THREADS) {
             float q[N];
             W::get(xs[v], q);
 #pragma unroll
-            for (int k = 0; k < N; k++)
-                if (q[k] >= xmin) m += rough(q[k]);
+            for (int k = 0; k < N; k++) {
+                const float e = rough(q[k]);
+                m += q[k] >= xmin ? e : 0.f;
+            }
         }
         return sr_reduce(m, reinterpret_cast<float *>(S.red), [](float a, float b) { return a + b; });
     };
@@ -358,17 +370,12 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_
         if (at < SR_LIST) lead->list[at] = sr_pair(v, i);
     };
     bool few = false;
-    float m1 = 0.f;  // approximate mass of the survivors (top_k with top-p only)
+    float m1 = 0.f;  // approximate mass of the survivors
     if (rule.min_p > 0.0) {
         few = true;
-        if (tmax >= xmin)
-            loaded([&](int v) {
-                float q[N];
-                W::get(xs[v], q);
-#pragma unroll
-                for (int k = 0; k < N; k++)
-                    if (q[k] >= xmin) to_list(q[k], base + v * N + k);
-            });
+        loaded(tmax >= xmin, [&](float v, int i) {
+            if (v >= xmin) to_list(v, i);
+        });
     } else if (by_topk) {
         few = true;
         const float span = __fsub_rn(mx, low);
@@ -382,149 +389,123 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_
         cl.sync();
         if (tid == 0) S.last_bin = SR_BINS;
         unsigned n = 0, all;
-        if (tid < SR_BINS)
-            for (int i = 0; i < cs; i++) n += cl.map_shared_rank(&S, i)->cnt[0][tid];
+        for (int i = 0; i < cs; i++) n += cl.map_shared_rank(&S, i)->cnt[0][tid];
         const unsigned before = sr_scan(n, reinterpret_cast<unsigned *>(S.red), &all);
         if (before < (unsigned)rule.top_k && before + n >= (unsigned)rule.top_k) S.last_bin = tid;
         __syncthreads();
         const int last = S.last_bin;
         for (int i = 0; i < cs; i++) m1 += has_p ? S.mass_of[i] : 0.f;
         if (last < SR_BINS && inv > 0.f) {
-            if (tmax > -INFINITY && bin(tmax) <= last)
-                loaded([&](int v) {
-                    float q[N];
-                    W::get(xs[v], q);
-#pragma unroll
-                    for (int k = 0; k < N; k++)
-                        if (q[k] > -INFINITY && bin(q[k]) <= last) to_list(q[k], base + v * N + k);
-                });
+            loaded(tmax > -INFINITY && bin(tmax) <= last, [&](float v, int i) {
+                if (v > -INFINITY && bin(v) <= last) to_list(v, i);
+            });
         } else {
             few = false;  // fewer maxima than top_k, or equal ones
         }
     }
 
-    // rank 0: the list in sorted order, its exact masses, and how many of it stay; above = what precedes the list
-    auto sort_list = [&](int n, auto greater) {
-        int p = 2;
-        while (p < n) p <<= 1;
-        for (int i = n + tid; i < p; i += SR_THREADS) S.list[i] = 0;
-        __syncthreads();
-        for (int k = 2; k <= p; k <<= 1)
-            for (int j = k >> 1; j > 0; j >>= 1) {
-                for (int t = tid; t < p / 2; t += SR_THREADS) {
-                    const int i = 2 * t - (t & (j - 1)), o = i + j;
-                    const u64 a = S.list[i], b = S.list[o];
-                    if (greater(b, a) == ((i & k) == 0)) {
-                        S.list[i] = b;
-                        S.list[o] = a;
-                    }
-                }
-                __syncthreads();
-            }
-    };
-    auto by_value = [](u64 a, u64 b) { return a > b; };
-    auto by_index = [](u64 a, u64 b) { return (uint32_t)a > (uint32_t)b; };
     auto value_of = [](u64 pr) { return sr_unkey((uint32_t)(pr >> 32)); };
-    // each thread's 4 consecutive list entries: exclusive masses before them
-    auto list_scan = [&](int n, u64 (&w)[SR_LIST / SR_THREADS], u64 *all) {
-        u64 sum = 0;
-#pragma unroll
-        for (int k = 0; k < SR_LIST / SR_THREADS; k++) {
-            const int i = tid * (SR_LIST / SR_THREADS) + k;
-            w[k] = i < n ? unit_of(value_of(S.list[i])) : 0;
-            sum += w[k];
-        }
-        return sr_scan(sum, S.red, all);
-    };
-    // first list position at which the cut falls, given the mass and count before the list and the needed mass
-    // (lo and hi: its bounds).  SR_LIST: none; -1: lo and hi do not agree.
-    auto find_cut = [&](int n, u64 m_above, unsigned c_above, u64 need_lo, u64 need_hi) {
-        u64 w[SR_LIST / SR_THREADS], all;
-        u64 run = m_above + list_scan(n, w, &all);
-        __syncthreads();
-        if (tid == 0) {
-            S.first_bin = SR_LIST;
-            S.last_bin = SR_LIST;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < SR_LIST / SR_THREADS; k++) {
-            const int i = tid * (SR_LIST / SR_THREADS) + k;
-            run += w[k];
-            if (i >= n) continue;
-            const bool full = rule.top_k && c_above + i + 1 >= (unsigned)rule.top_k;
-            if (full || (has_p && run >= need_lo)) atomicMin(&S.first_bin, i);
-            if (full || (has_p && run >= need_hi)) atomicMin(&S.last_bin, i);
-        }
-        __syncthreads();
-        const int a = S.first_bin, b = S.last_bin;
-        return a == b ? a : -1;
-    };
-    // rank 0: draws from the first `kept` entries of the sorted list
-    auto draw_list = [&](int kept) {
-        __syncthreads();
-        sort_list(kept, by_index);  // (~index descending: index ascending)
-        u64 w[SR_LIST / SR_THREADS], all;
-        u64 run = list_scan(kept, w, &all);
-        u64 target = (u64)(rule.u * (double)all);
-        if (target >= all) target = all - 1;
-#pragma unroll
-        for (int k = 0; k < SR_LIST / SR_THREADS; k++) {
-            const int i = tid * (SR_LIST / SR_THREADS) + k;
-            if (run <= target && target < run + w[k]) {
-                const u64 pr = S.list[i];
-                A.tokens[row] = (int)~(uint32_t)pr;
-                if (A.probs) A.probs[row] = (float)(rule.weight(value_of(pr), mx, S.table) * SR_UNIT / (double)all);
-            }
-            run += w[k];
-        }
-    };
     auto need_of = [&](double mass) { return (u64)ceil(rule.top_p * mass); };
-    auto exact_mass = [&]() {  // of this CTA's survivors
-        u64 m = 0;
-        own([&](float v, int) {
-            if (v >= xmin) m += unit_of(v);
+    // The block ranks the n list entries: a group of lanes adds up, for one entry, what pred lets count.
+    auto ranked = [&](int n, auto counts, auto use) {
+        int g = 1;  // lanes an entry
+        while (g < 32 && g * 2 * n <= SR_THREADS) g *= 2;
+        for (int c = tid / g; c < (n + SR_THREADS / g - 1) / (SR_THREADS / g) * (SR_THREADS / g); c += SR_THREADS / g) {
+            const u64 mine = c < n ? S.list[c] : 0;
+            u64 mass = 0;
+            int number = 0;
+            for (int j = tid & (g - 1); j < n; j += g)
+                if (counts(S.list[j], mine)) {
+                    number++;
+                    mass += S.wt[j];
+                }
+            for (int o = 1; o < g; o <<= 1) {
+                number += __shfl_xor_sync(0xffffffffu, number, o);
+                mass += __shfl_xor_sync(0xffffffffu, mass, o);
+            }
+            if (c < n && (tid & (g - 1)) == 0) use(c, mine, number, mass);
+        }
+    };
+    // Where the cut falls in the list, with the mass and count above the list and the needed mass (its bounds lo, hi):
+    // S.cut and, of the list down to it, S.kept_mass.  False where lo and hi do not agree.
+    auto find_cut = [&](int n, u64 m_above, unsigned c_above, u64 lo, u64 hi) {
+        if (tid == 0) S.first_bin = S.last_bin = n - 1;
+        __syncthreads();
+        int number_of[SR_EACH], k = 0;  // this thread's entries
+        u64 mass_of[SR_EACH], pair_of[SR_EACH];
+#pragma unroll
+        for (int e = 0; e < SR_EACH; e++) number_of[e] = -1;
+        ranked(n, [](u64 a, u64 b) { return a > b; }, [&](int c, u64 mine, int number, u64 mass) {
+            const u64 run = m_above + mass + S.wt[c];
+            const bool full = rule.top_k && c_above + number + 1 >= (unsigned)rule.top_k;
+            if (full || (has_p && run >= lo)) atomicMin(&S.first_bin, number);
+            if (full || (has_p && run >= hi)) atomicMin(&S.last_bin, number);
+#pragma unroll
+            for (int e = 0; e < SR_EACH; e++)
+                if (e == k) {
+                    number_of[e] = number;
+                    mass_of[e] = mass + S.wt[c];
+                    pair_of[e] = mine;
+                }
+            k++;
         });
-        return sr_reduce(m, S.red, addu);
+        __syncthreads();
+        const int at = S.first_bin;
+        if (at != S.last_bin) return false;
+#pragma unroll
+        for (int e = 0; e < SR_EACH; e++)
+            if (number_of[e] == at) {
+                S.cut = pair_of[e];
+                S.kept_mass = mass_of[e];
+            }
+        __syncthreads();
+        return true;
     };
 
     if (few) {
         cl.sync();
-        const unsigned n = lead->n_list;
+        const int n = (int)min(lead->n_list, (unsigned)SR_LIST + 1);
         if (n <= SR_LIST) {
-            const bool open = has_p && rule.min_p == 0.0;  // the decision leans on m1
-            int kept = (int)n;
-            if (rank == 0) {
-                sort_list((int)n, by_value);
-                if (cuts) {
-                    u64 lo = ~0ull, hi = ~0ull;
-                    if (open) {
-                        lo = need_of((double)m1 * (1.0 - 1e-4) * SR_UNIT);
-                        hi = need_of((double)m1 * (1.0 + 1e-4) * SR_UNIT);
-                    } else if (has_p) {
-                        u64 w[SR_LIST / SR_THREADS], all;
-                        list_scan((int)n, w, &all);
-                        lo = hi = need_of((double)all);
-                    }
-                    const int at = find_cut((int)n, 0, 0, lo, hi);
-                    kept = at < 0 ? -1 : at == SR_LIST ? (int)n : at + 1;
+            // rank 0 goes on alone: nothing of the others is read after the barrier above, and a barrier that some
+            // threads have left waits for the others only
+            if (rank != 0) return;
+            for (int i = tid; i < n; i += SR_THREADS) S.wt[i] = unit_of(value_of(S.list[i]));
+            __syncthreads();
+            u64 lo = ~0ull, hi = ~0ull;
+            const bool open = has_p && rule.min_p == 0.0;  // the list does not hold all survivors
+            if (open) {
+                lo = need_of((double)m1 * (1.0 - 1e-4) * SR_UNIT);
+                hi = need_of((double)m1 * (1.0 + 1e-4) * SR_UNIT);
+            } else if (has_p) {
+                u64 m = 0;
+                for (int i = tid; i < n; i += SR_THREADS) m += S.wt[i];
+                lo = hi = need_of((double)sr_reduce(m, S.red, addu));
+            }
+            if (!find_cut(n, 0, 0, lo, hi)) {
+                u64 m = 0;  // the exact mass of the whole row
+#pragma unroll 4
+                for (int i = tid; i < A.vocab; i += SR_THREADS) {
+                    const float v = sr_load(x, i);
+                    const u64 w = unit_of(v);
+                    if (v >= xmin) m += w;
                 }
-                if (tid < cs) cl.map_shared_rank(&S, tid)->state = kept < 0;
-                if (kept >= 0) draw_list(kept);
+                lo = need_of((double)sr_reduce(m, S.red, addu));
+                find_cut(n, 0, 0, lo, lo);
             }
+            const u64 cut = S.cut, total = S.kept_mass;
+            u64 target = (u64)(rule.u * (double)total);
+            if (target >= total) target = total - 1;
+            // mass before each kept entry in index order (the low halves hold ~index)
+            ranked(n, [&](u64 a, u64 b) { return a >= cut && (uint32_t)a > (uint32_t)b; },
+                   [&](int c, u64 mine, int, u64 mass) {
+                       if (mine >= cut && mass <= target && target < mass + S.wt[c]) {
+                           A.tokens[row] = (int)~(uint32_t)mine;
+                           if (A.probs)
+                               A.probs[row] = (float)(rule.weight(value_of(mine), mx, S.table) * SR_UNIT / (double)total);
+                       }
+                   });
+            // the other ranks have read n_list before they left
             cl.sync();
-            if (S.state == 0) return;
-            // the approximate mass left it open: sum the exact one
-            const u64 m = exact_mass();
-            if (tid == 0) lead->slot[0][rank] = m;
-            cl.sync();
-            if (rank == 0) {
-                u64 all = 0;
-                for (int i = 0; i < cs; i++) all += S.slot[0][i];
-                const u64 need = need_of((double)all);
-                const int at = find_cut((int)n, 0, 0, need, need);
-                draw_list(at < 0 || at == SR_LIST ? (int)n : at + 1);
-            }
             return;
         }
     }
@@ -553,12 +534,21 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_
     };
     if (cuts) {
         // lowest survivor, and the approximate mass
-        float lw = INFINITY;
-        own([&](float v, int) {
-            if (v >= xmin) lw = fminf(lw, v);
-        });
+        float lw = INFINITY, mass = 0.f;
+#pragma unroll 4
+        for (int v = tid; v < nwords; v += SR_THREADS) {
+            float q[N];
+            W::get(xs[v], q);
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const bool in = q[k] >= xmin;
+                lw = in ? fminf(lw, q[k]) : lw;
+                const float e = rough(q[k]);
+                mass += in ? e : 0.f;
+            }
+        }
         lw = sr_reduce(lw, reinterpret_cast<float *>(S.red), minf);
-        const float mass = has_p ? rough_mass() : 0.f;
+        mass = sr_reduce(mass, reinterpret_cast<float *>(S.red), [](float a, float b) { return a + b; });
         const float step = mass > 0.f ? __fmul_rn(mass, 0x1p-30f) : 0.f;
         cl.sync();  // the earlier slots have been read
         push(&SrShared::low_of, lw);
@@ -596,14 +586,14 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_
                 if (has_p) atomicAdd(&S.mass[buf][b], __float2uint_rn(__fmul_rn(rough(v), per)));
             });
             cl.sync();
-            unsigned n = 0, n_all;
+            unsigned n = 0, n_low = 0, n_all;  // n_low: of the ranks before this one
             float m = 0.f, m_all;
-            if (tid < SR_BINS)
-                for (int i = 0; i < cs; i++) {
-                    const SrShared *o = cl.map_shared_rank(&S, i);
-                    n += o->cnt[buf][tid];
-                    if (has_p) m += __fmul_rn((float)o->mass[buf][tid], S.unit_of[i]);
-                }
+            for (int i = 0; i < cs; i++) {
+                const SrShared *o = cl.map_shared_rank(&S, i);
+                if (i == rank) n_low = n;
+                n += o->cnt[buf][tid];
+                if (has_p) m += __fmul_rn((float)o->mass[buf][tid], S.unit_of[i]);
+            }
             const unsigned nb = c_above + sr_scan(n, reinterpret_cast<unsigned *>(S.red), &n_all);
             __syncthreads();
             const float mb = m_above + sr_scan(m, reinterpret_cast<float *>(S.red), &m_all);
@@ -613,16 +603,19 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_
             const bool may = n && (full || (has_p && mb + m + slack >= need)), must = n && (full || (has_p && mb + m - slack >= need));
             if (tid == 0) {
                 S.first_bin = S.last_bin = SR_BINS;
-                S.range_count = 0;
+                S.range_count = S.range_low = 0;
             }
             // (the buffer of the next round was read before this round's barrier)
             for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[buf ^ 1][i] = S.mass[buf ^ 1][i] = 0;
             __syncthreads();
-            if (tid < SR_BINS && may) atomicMin(&S.first_bin, tid);
-            if (tid < SR_BINS && must) atomicMin(&S.last_bin, tid);
+            if (may) atomicMin(&S.first_bin, tid);
+            if (must) atomicMin(&S.last_bin, tid);
             __syncthreads();
             const int fb = S.first_bin, lb = min(S.last_bin, SR_BINS - 1);
-            if (tid >= fb && tid <= lb) atomicAdd(&S.range_count, n);
+            if (tid >= fb && tid <= lb) {
+                atomicAdd(&S.range_count, n);
+                atomicAdd(&S.range_low, n_low);
+            }
             if (tid == fb) {
                 S.max_of[0] = mb;  // (the maxima have been read)
                 S.red[31] = nb;
@@ -652,19 +645,20 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_
             lo = nlo;
             hi = nhi;
         }
-        // ---- exact masses: above the range (kept), and of all survivors where top-p needs it
-        u64 m_all = 0;
-        if (rank == 0 && tid == 0) S.n_list = 0;
-        cl.sync();
+        // ---- exact masses: above the range (kept), and of all survivors where top-p needs it; the range to rank 0
         const bool listed = in_range > 0 && in_range <= SR_LIST;
+        const unsigned at0 = S.range_low;  // the entries of the ranks before this one come first
+        __syncthreads();
+        if (tid == 0) S.n_list = 0;
+        __syncthreads();
+        u64 m_all = 0;
         own([&](float v, int i) {
-            if (!(v >= xmin)) return;
-            const int s = side(v);
+            const int s = v >= xmin ? side(v) : -1;
             u64 w = 0;
-            if (s > 0 || has_p) w = unit_of(v);
-            m_all += w;
-            if (s > 0) kept_sum += w;
-            if (s == 0 && listed) to_list(v, i);
+            if (has_p || s > 0) w = unit_of(v);
+            m_all += v >= xmin ? w : 0;
+            kept_sum += s > 0 ? w : 0;
+            if (s == 0 && listed) lead->list[at0 + atomicAdd(&S.n_list, 1u)] = sr_pair(v, i);
         });
         const u64 above = sr_reduce(kept_sum, S.red, addu), all = sr_reduce(m_all, S.red, addu);
         if (tid < cs) {
@@ -683,11 +677,11 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 2) k_sample_
             cut = 0;  // every survivor down to the range's end
         } else if (listed) {
             if (rank == 0) {
-                const int n = (int)S.n_list;
-                sort_list(n, by_value);
-                const int at = find_cut(n, above_all, c_above, need, need);
-                const u64 last = S.list[at < 0 || at == SR_LIST ? n - 1 : at];
-                if (tid < cs) cl.map_shared_rank(&S, tid)->cut = last;
+                const int n = (int)in_range;
+                for (int i = tid; i < n; i += SR_THREADS) S.wt[i] = unit_of(value_of(S.list[i]));
+                __syncthreads();
+                find_cut(n, above_all, c_above, need, need);
+                if (tid < cs) cl.map_shared_rank(&S, tid)->cut = S.cut;
             }
             cl.sync();
             cut = S.cut;
