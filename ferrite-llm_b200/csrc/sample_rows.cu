@@ -10,26 +10,29 @@
 // that is not zero counts for one unit at least, so no kept token is
 // unreachable.
 //
-// Bound: HBM (a row is read once, into the shared memory of a thread-block
-// cluster); a few rows are bound by the cluster's steps.  No sort of the row:
+// Bound: HBM for many rows (a row streams through registers once; what comes
+// later reads a few of its vectors, or passes that find it in L2); a few rows
+// are bound by the steps of the cluster that shares a row.  The first pass keeps
+// the maximum of every group of 16-byte vectors in shared memory.  No sort of
+// the row:
 //  * min-p: the threshold logit is found exactly (the f32 whose binary64 weight
 //    is the first to reach min_p); the survivors are the candidates;
-//  * top_k <= SR_TOPK: at least top_k of the threads' maxima lie above the
+//  * top_k <= SR_TOPK: at least top_k of the groups' maxima lie above the
 //    threshold that a 256-bin count of these maxima gives, so the cut does too:
 //    the logits above it are the candidates (a little over top_k of them);
 //  * otherwise: counts and approximate masses of 256 bins of the distance to
 //    the maximum narrow the cut down to a range of at most SR_LIST logits, all
 //    above it are kept.
 // One CTA ranks the candidates against each other with exact weights (no sort:
-// 512 at most, a few lanes each).  In the first two cases it draws from them
-// alone and the cluster's other CTAs are gone by then.  A decision that leans on
-// approximate masses is taken with their error on both sides; where that leaves
-// it open, the exact mass of the row is summed.  Rows whose cut falls among more
-// than SR_LIST logits that no bin tells apart are bisected by key.
+// 512 at most, a few lanes each) and draws; the cluster's other CTAs are gone by
+// then.  A decision that leans on approximate masses is taken with their error
+// on both sides; where that leaves it open, the exact mass of the row is summed.
+// Rows whose cut falls among more than SR_LIST logits that no bin tells apart are
+// bisected by key.
 #include <cooperative_groups.h>
 #include <math.h>
 
-#include <mutex>
+#include <type_traits>
 
 #include "fb_internal.h"
 #include "kq_common.cuh"
@@ -42,18 +45,24 @@ constexpr int SR_WARPS = SR_THREADS / 32;
 constexpr int SR_MAX_VOCAB = 1 << 19;
 constexpr int SR_LIST = 512;    // candidates one CTA ranks
 constexpr int SR_EACH = SR_LIST / SR_THREADS;
-constexpr int SR_TOPK = 256;    // top_k up to here goes by the threads' maxima
+constexpr int SR_TOPK = 256;    // top_k up to here goes by the groups' maxima
 constexpr int SR_BINS = 256;
 constexpr int SR_CLUSTER = 16;
 constexpr int SR_ROUNDS = 4;    // narrowings before the bisection
+constexpr int SR_GROUPS = 48;   // groups a thread, at most
+constexpr int SR_AHEAD = 4;     // vectors a thread has in flight
+constexpr int SR_FLAGGED = 1024;
 constexpr double SR_UNIT = 8796093022208.0;  // 2^43
 
 using u64 = unsigned long long;
 
+// A row's logits: rank r of the cluster has the run of `chunk` logits from r
+// chunk on, its warp w the run of chunk / 8 from w chunk / 8 on, in `steps`
+// steps of one 16-byte vector a lane; a group is `gsteps` of them.
 struct SampleRowsArgs {
     const void *logits;
     int64_t stride;
-    int vocab, words;  // shared-memory words a thread (odd: its own run is free of bank conflicts)
+    int vocab, chunk, steps, gsteps;
     bool vec;          // rows start on 16 bytes
     const float *temperature, *top_p, *min_p, *uniform;
     const int32_t *top_k;
@@ -61,29 +70,33 @@ struct SampleRowsArgs {
     float *probs;
 };
 
-// A 32-bit word holds one f32 or two 16-bit logits.
-template <typename T> struct SrWord;
-template <> struct SrWord<float> {
-    static constexpr int N = 1;
-    static __device__ __forceinline__ void get(uint32_t w, float (&v)[1]) { v[0] = __uint_as_float(w); }
-    static constexpr uint32_t PAD = 0x7fffffffu;  // NaN: never selected
-};
-template <> struct SrWord<__half> {
-    static constexpr int N = 2;
-    static __device__ __forceinline__ void get(uint32_t w, float (&v)[2]) {
-        v[0] = __half2float(__ushort_as_half((unsigned short)w));
-        v[1] = __half2float(__ushort_as_half((unsigned short)(w >> 16)));
+template <typename T> constexpr int SR_E = 16 / (int)sizeof(T);  // logits a vector
+__device__ __forceinline__ void sr_get(const uint4 &q, float (&v)[4]) {
+    v[0] = __uint_as_float(q.x);
+    v[1] = __uint_as_float(q.y);
+    v[2] = __uint_as_float(q.z);
+    v[3] = __uint_as_float(q.w);
+}
+template <typename T> __device__ __forceinline__ void sr_get16(const uint4 &q, float (&v)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if constexpr (std::is_same<T, __half>::value) {
+            v[2 * k] = __half2float(__ushort_as_half((unsigned short)w[k]));
+            v[2 * k + 1] = __half2float(__ushort_as_half((unsigned short)(w[k] >> 16)));
+        } else {
+            v[2 * k] = __uint_as_float(w[k] << 16);
+            v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        }
     }
-    static constexpr uint32_t PAD = 0x7fff7fffu;
-};
-template <> struct SrWord<__nv_bfloat16> {
-    static constexpr int N = 2;
-    static __device__ __forceinline__ void get(uint32_t w, float (&v)[2]) {
-        v[0] = __uint_as_float(w << 16);
-        v[1] = __uint_as_float(w & 0xffff0000u);
-    }
-    static constexpr uint32_t PAD = 0x7fff7fffu;
-};
+}
+template <typename T> __device__ __forceinline__ void sr_unpack(const uint4 &q, float (&v)[SR_E<T>]) {
+    if constexpr (sizeof(T) == 4) sr_get(q, v);
+    else sr_get16<T>(q, v);
+}
+__device__ __forceinline__ float sr_load(const float *p, int i) { return p[i]; }
+__device__ __forceinline__ float sr_load(const __half *p, int i) { return __half2float(p[i]); }
+__device__ __forceinline__ float sr_load(const __nv_bfloat16 *p, int i) { return __bfloat162float(p[i]); }
 
 // Order-preserving key of a logit (-0 as +0); 0 for NaN, which sorts below all.
 __device__ __forceinline__ uint32_t sr_key(float x) {
@@ -111,7 +124,7 @@ struct RowRule {
         greedy = tt <= 0.f;
         t = (tt != tt || greedy) ? 1.0 : (double)tt;
         scale = 46.16624130844683 / t;  // 32 log2(e) / T
-        c = (float)(scale * 0.03125);
+        c = (float)fmin(scale * 0.03125, 1e30);  // (finite: 0 c stays 0)
         min_p = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
         top_p = tp < 1.f ? fmax((double)tp, 0.0) : 2.0;
         top_k = k > 0 && k < A.vocab ? k : 0;
@@ -178,117 +191,164 @@ template <typename V> __device__ __forceinline__ V sr_scan(V v, V *sh, V *all) {
 }
 
 struct SrShared {
-    u64 list[SR_LIST], wt[SR_LIST];    // rank 0: the candidates and their weights
-    u64 slot[2][SR_CLUSTER];           // pushed by every rank
+    u64 list[SR_LIST], wt[SR_LIST];            // rank 0: the candidates and their weights
+    u64 seg[SR_CLUSTER * SR_WARPS];            // rank 0: kept mass of every warp's run
+    u64 slot[2][SR_CLUSTER];                   // pushed by every rank
     u64 red[32];
+    u64 cut, kept_mass, target;
     double table[32];
     float max_of[SR_CLUSTER], low_of[SR_CLUSTER], mass_of[SR_CLUSTER];
-    float unit_of[SR_CLUSTER];         // weight of one step of a rank's mass bins
+    float unit_of[SR_CLUSTER];                 // weight of one step of a rank's mass bins
     uint32_t cnt[2][SR_BINS], mass[2][SR_BINS];
-    u64 cut;                           // pushed by rank 0
-    u64 kept_mass;
-    unsigned n_list;                   // rank 0: candidates pushed
-    int first_bin, last_bin;
-    unsigned range_low;
+    uint32_t flagged[SR_FLAGGED];              // groups to look into
+    unsigned n_flagged, n_list;                // n_list, rank 0: candidates pushed
+    int first_bin, last_bin, where;
+    unsigned range_count, range_low;
+    float m_at;
     uint32_t kmin;
-    unsigned range_count;
 };
 
-__device__ __forceinline__ float sr_load(const float *p, int i) { return p[i]; }
-__device__ __forceinline__ float sr_load(const __half *p, int i) { return __half2float(p[i]); }
-__device__ __forceinline__ float sr_load(const __nv_bfloat16 *p, int i) { return __bfloat162float(p[i]); }
+static_assert(SR_BINS == SR_THREADS && SR_CLUSTER * SR_WARPS <= SR_THREADS, "a thread a bin, a thread a run");
 
-static_assert(SR_BINS == SR_THREADS, "a thread a bin");
 template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_rows(const SampleRowsArgs A) {
-    using W = SrWord<T>;
-    constexpr int N = W::N;
-    extern __shared__ __align__(16) uint32_t xs[];
+    constexpr int E = SR_E<T>;
+    extern __shared__ float gmax[];  // [group][thread] largest logit
     __shared__ SrShared S;
     cg::cluster_group cl = cg::this_cluster();
-    const int tid = threadIdx.x, lane = tid & 31, rank = cl.block_rank(), cs = cl.num_blocks();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cl.block_rank(), cs = cl.num_blocks();
     const int64_t row = blockIdx.x / cs;
-    const int nwords = SR_THREADS * A.words, base = rank * nwords * N;  // this CTA's logits: base .. base + nwords * N - 1
     const T *x = static_cast<const T *>(A.logits) + row * A.stride;
+    const int run = A.steps * 32 * E;                   // logits of a warp
+    const int base = rank * A.chunk + warp * run;       // the warp's first
+    const int ngroups = (A.steps + A.gsteps - 1) / A.gsteps;
     RowRule rule;
     rule.load(A, row);
     auto addu = [](u64 a, u64 b) { return a + b; };
+    auto addf = [](float a, float b) { return a + b; };
+    auto maxf = [](float a, float b) { return fmaxf(a, b); };
+    auto minf = [](float a, float b) { return fminf(a, b); };
 
-    // ---- the row into shared memory; every thread's maximum of what it loads
-    float tmax = -INFINITY;
-    if (tid < 32) S.table[tid] = exp2((double)tid * 0.03125);
-    if (tid == 0) S.n_list = 0;
-    for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[0][i] = S.mass[0][i] = 0;
-    if (A.vec) {
-        constexpr int E = 4 * N;
-#pragma unroll 5
-        for (int v = tid; v < nwords / 4; v += SR_THREADS) {
-            const int i = base + v * E;
-            uint4 q = make_uint4(W::PAD, W::PAD, W::PAD, W::PAD);
-            if (i + E <= A.vocab) {
-                q = __ldg(reinterpret_cast<const uint4 *>(x + i));
-            } else if (i < A.vocab) {
-                T *e = reinterpret_cast<T *>(&q);
-                for (int k = 0; i + k < A.vocab; k++) e[k] = x[i + k];
+    // E logits from index i on as they are stored, NaN (never selected) behind the row
+    auto fetch = [&](int i) {
+        if (A.vec && i + E <= A.vocab) return __ldg(reinterpret_cast<const uint4 *>(x + i));
+        uint32_t w[4] = {~0u, ~0u, ~0u, ~0u};
+#pragma unroll
+        for (int k = 0; k < E; k++)
+            if (i + k < A.vocab) {
+                if constexpr (E == 4) {
+                    w[k] = __float_as_uint(x[i + k]);
+                } else {
+                    const uint32_t h = *reinterpret_cast<const unsigned short *>(x + i + k);
+                    w[k / 2] = k & 1 ? (w[k / 2] & 0xffffu) | h << 16 : (w[k / 2] & 0xffff0000u) | h;
+                }
             }
-            reinterpret_cast<uint4 *>(xs)[v] = q;
-            const uint32_t w4[4] = {q.x, q.y, q.z, q.w};
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    // f(E logits, first index) over this thread's vectors
+    auto stream = [&](auto f) {
+        for (int s = 0; s < A.steps; s += SR_AHEAD) {
+            uint4 q[SR_AHEAD];
+            const int i0 = base + (s * 32 + lane) * E;
+            if (i0 - lane * E >= A.vocab) break;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                float f[N];
-                W::get(w4[k], f);
+            for (int k = 0; k < SR_AHEAD; k++)
+                if (s + k < A.steps) q[k] = fetch(i0 + k * 32 * E);
 #pragma unroll
-                for (int e = 0; e < N; e++) tmax = fmaxf(tmax, f[e]);
-            }
-        }
-    } else {
-#pragma unroll 4
-        for (int v = tid; v < nwords; v += SR_THREADS) {
-            uint32_t q = W::PAD;
-            T *e = reinterpret_cast<T *>(&q);
-#pragma unroll
-            for (int k = 0; k < N; k++)
-                if (base + v * N + k < A.vocab) e[k] = x[base + v * N + k];
-            xs[v] = q;
-            float f[N];
-            W::get(q, f);
-#pragma unroll
-            for (int k = 0; k < N; k++) tmax = fmaxf(tmax, f[k]);
-        }
-    }
-    // f(logit, index) over the logits that a lane's threads of this warp loaded, for the lanes whose flag is set: the
-    // whole warp looks through one lane's logits at a time
-    auto loaded = [&](bool flag, auto f) {
-        for (uint32_t todo = __ballot_sync(0xffffffffu, flag); todo; todo &= todo - 1) {
-            const int src = (tid & ~31) + __ffs(todo) - 1;
-            for (int q = lane; q < ((A.words + 3) & ~3); q += 32) {
-                const int v = A.vec ? 4 * (src + SR_THREADS * (q >> 2)) + (q & 3) : src + SR_THREADS * q;
-                if (v >= nwords) continue;
-                float g[N];
-                W::get(xs[v], g);
-#pragma unroll
-                for (int k = 0; k < N; k++) f(g[k], base + v * N + k);
-            }
+            for (int k = 0; k < SR_AHEAD; k++)
+                if (s + k < A.steps) {
+                    float v[E];
+                    sr_unpack<T>(q[k], v);
+                    f(v, i0 + k * 32 * E);
+                }
         }
     };
-    // f(logit, index) over this thread's run of consecutive logits
-    auto own = [&](auto f) {
-#pragma unroll 4
-        for (int j = 0; j < A.words; j++) {
-            const int v = tid * A.words + j;
-            float q[N];
-            W::get(xs[v], q);
+
+    // ---- the first pass: the groups' maxima, and for top_k with top-p the approximate mass (each thread's relative to
+    // its own running maximum)
+    const bool by_topk = rule.top_k > 0 && rule.top_k <= SR_TOPK && rule.min_p == 0.0 && !rule.greedy;
+    const bool has_p = rule.top_p < 1.0, cuts = rule.top_k > 0 || has_p;
+    if (tid < 32) S.table[tid] = exp2((double)tid * 0.03125);
+    if (tid == 0) S.n_list = S.n_flagged = 0;
+    S.cnt[0][tid] = S.mass[0][tid] = 0;
+    auto ex2 = [](float y) {
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
+        return e;
+    };
+    float tmax = -INFINITY, tsum = 0.f;
+    {
+        const bool online = by_topk && has_p;
+        for (int g = 0; g < ngroups; g++) {
+            float gm = -INFINITY;
+            const int s1 = min(A.steps, (g + 1) * A.gsteps);
+            for (int s = g * A.gsteps; s < s1; s += SR_AHEAD) {
+                const int i0 = base + (s * 32 + lane) * E;
+                if (i0 - lane * E >= A.vocab) break;
+                uint4 q[SR_AHEAD];
+                float m = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < N; k++) f(q[k], base + v * N + k);
+                for (int k = 0; k < SR_AHEAD; k++)
+                    q[k] = s + k < s1 ? fetch(i0 + k * 32 * E) : make_uint4(~0u, ~0u, ~0u, ~0u);
+#pragma unroll
+                for (int k = 0; k < SR_AHEAD; k++) {
+                    float v[E];
+                    sr_unpack<T>(q[k], v);
+#pragma unroll
+                    for (int e = 0; e < E; e++) m = fmaxf(m, v[e]);
+                }
+                gm = fmaxf(gm, m);
+                if (online && m > -INFINITY) {
+                    const float top = fmaxf(tmax, m);
+                    float sum = tsum > 0.f ? __fmul_rn(tsum, ex2(__fmul_rn(__fsub_rn(tmax, top), rule.c))) : 0.f;
+#pragma unroll
+                    for (int k = 0; k < SR_AHEAD; k++) {
+                        float v[E];
+                        sr_unpack<T>(q[k], v);
+#pragma unroll
+                        for (int e = 0; e < E; e++) {
+                            const float p = ex2(__fmul_rn(__fsub_rn(v[e], top), rule.c));
+                            sum += v[e] > -INFINITY ? p : 0.f;
+                        }
+                    }
+                    tsum = sum;
+                    tmax = top;
+                }
+            }
+            gmax[g * SR_THREADS + tid] = gm;
+            tmax = fmaxf(tmax, gm);
         }
+    }
+    // f(logit, index) over the logits of the groups whose maximum satisfies pred; false: too many such groups
+    auto look_into = [&](auto pred, auto f) {
+        __syncthreads();
+        if (tid == 0) S.n_flagged = 0;
+        __syncthreads();
+        for (int g = 0; g < ngroups; g++)
+            if (pred(gmax[g * SR_THREADS + tid])) {
+                const unsigned at = atomicAdd(&S.n_flagged, 1u);
+                if (at < SR_FLAGGED) S.flagged[at] = (uint32_t)(g * SR_THREADS + tid);
+            }
+        __syncthreads();
+        const unsigned n = S.n_flagged;
+        if (n > SR_FLAGGED) return false;
+        for (unsigned it = tid; it < n * A.gsteps; it += SR_THREADS) {
+            const uint32_t id = S.flagged[it / A.gsteps];
+            const int g = id / SR_THREADS, t = id % SR_THREADS, s = g * A.gsteps + it % A.gsteps;
+            if (s >= A.steps) continue;
+            const int i = rank * A.chunk + (t >> 5) * run + (s * 32 + (t & 31)) * E;
+            float v[E];
+            sr_unpack<T>(fetch(i), v);
+#pragma unroll
+            for (int k = 0; k < E; k++) f(v[k], i + k);
+        }
+        return true;
     };
     auto push = [&](float (SrShared::*field)[SR_CLUSTER], float v) {  // own value into every rank's [rank]
         if (tid < cs) (cl.map_shared_rank(&S, tid)->*field)[rank] = v;
     };
-    auto maxf = [](float a, float b) { return fmaxf(a, b); };
-    auto minf = [](float a, float b) { return fminf(a, b); };
     const float bmax = sr_reduce(tmax, reinterpret_cast<float *>(S.red), maxf);
     const float blow = sr_reduce(tmax > -INFINITY ? tmax : INFINITY, reinterpret_cast<float *>(S.red), minf);
-    cl.sync();  // every rank has started
+    if (cs > 1) cl.sync();  // every rank has started
     push(&SrShared::max_of, bmax);
     push(&SrShared::low_of, blow);
     cl.sync();
@@ -297,12 +357,16 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         mx = fmaxf(mx, S.max_of[i]);
         low = fminf(low, S.low_of[i]);
     }
-    if (rule.greedy || mx == -INFINITY) {
-        // the first of the largest logits (a row of -inf has one, a row of NaN none)
+    const bool none = mx == -INFINITY;  // nothing finite: -inf is taken by greedy rows only, NaN by none
+    if (rule.greedy || none) {
         u64 first = ~0ull;
-        if (rule.greedy)
-            loaded(tmax == mx, [&](float v, int i) {
-                if (v == mx) first = min(first, (u64)i);
+        auto take = [&](float v, int i) {
+            if (v == mx) first = min(first, (u64)i);
+        };
+        if (rule.greedy && !look_into([&](float m) { return m == mx; }, take))
+            stream([&](float (&v)[E], int i) {
+#pragma unroll
+                for (int e = 0; e < E; e++) take(v[e], i + e);
             });
         first = sr_reduce(first, S.red, [](u64 a, u64 b) { return a < b ? a : b; });
         if (tid == 0) cl.map_shared_rank(&S, 0)->slot[0][rank] = first;
@@ -339,51 +403,47 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         __syncthreads();
     }
     const float xmin = rule.min_p > 0.0 ? sr_unkey(S.kmin) : -3.4028235e38f;  // survivors: x >= xmin
-    const bool by_topk = rule.top_k > 0 && rule.top_k <= SR_TOPK;
-    const bool has_p = rule.top_p < 1.0, cuts = rule.top_k > 0 || has_p;
     auto unit_of = [&](float v) { return RowRule::units(rule.weight(v, mx, S.table)); };
     // binary32 weight, relative error below 1e-5 wherever it is not negligible
     auto rough = [&](float v) {
-        float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(__fsub_rn(v, mx), rule.c)));
+        const float e = ex2(__fmul_rn(__fsub_rn(v, mx), rule.c));
         return v == mx ? 1.f : mx == INFINITY ? 0.f : e;
     };
-    auto rough_mass = [&]() {  // of this CTA's survivors
-        float m = 0.f;
-#pragma unroll 4
-        for (int v = tid; v < nwords; v += SR_THREADS) {
-            float q[N];
-            W::get(xs[v], q);
-#pragma unroll
-            for (int k = 0; k < N; k++) {
-                const float e = rough(q[k]);
-                m += q[k] >= xmin ? e : 0.f;
-            }
-        }
-        return sr_reduce(m, reinterpret_cast<float *>(S.red), [](float a, float b) { return a + b; });
-    };
 
-    // ---- few candidates: min-p's survivors, or what lies above the threads' top_k-th largest maximum
+    // ---- few candidates: min-p's survivors, or what lies above the groups' top_k-th largest maximum
     SrShared *lead = cl.map_shared_rank(&S, 0);
     auto to_list = [&](float v, int i) {
         const unsigned at = atomicAdd(&lead->n_list, 1u);
         if (at < SR_LIST) lead->list[at] = sr_pair(v, i);
     };
+    auto too_many = [&]() {
+        if (tid == 0) atomicAdd(&lead->n_list, (unsigned)SR_LIST + 1);
+    };
     bool few = false;
     float m1 = 0.f;  // approximate mass of the survivors
     if (rule.min_p > 0.0) {
         few = true;
-        loaded(tmax >= xmin, [&](float v, int i) {
-            if (v >= xmin) to_list(v, i);
-        });
+        if (!look_into([&](float m) { return m >= xmin; },
+                       [&](float v, int i) {
+                           if (v >= xmin) to_list(v, i);
+                       }))
+            too_many();
     } else if (by_topk) {
         few = true;
         const float span = __fsub_rn(mx, low);
         const float inv = span > 0.f && span < INFINITY ? __fdiv_rn((float)(SR_BINS - 1), span) : 0.f;
-        auto bin = [&](float v) { return v == mx ? 0 : (int)fminf(__fmul_rn(__fsub_rn(mx, v), inv), (float)SR_BINS); };
-        if (tmax > -INFINITY) atomicAdd(&S.cnt[0][min(bin(tmax), SR_BINS - 1)], 1u);
+        // (distances beyond the threads' lowest maximum share bin 255, which cannot be the threshold)
+        auto bin = [&](float v) {
+            return v == mx ? 0 : (int)fminf(__fmul_rn(__fsub_rn(mx, v), inv), (float)(SR_BINS - 1));
+        };
+        for (int g = 0; g < ngroups; g++) {
+            const float m = gmax[g * SR_THREADS + tid];
+            const int b = m > -INFINITY ? bin(m) : SR_BINS - 1;
+            if (b < SR_BINS - 1) atomicAdd(&S.cnt[0][b], 1u);
+        }
         if (has_p) {
-            const float m = rough_mass();
+            const float m = sr_reduce(tsum > 0.f ? __fmul_rn(tsum, rough(tmax)) : 0.f,
+                                      reinterpret_cast<float *>(S.red), addf);
             push(&SrShared::mass_of, m);
         }
         cl.sync();
@@ -396,9 +456,11 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         const int last = S.last_bin;
         for (int i = 0; i < cs; i++) m1 += has_p ? S.mass_of[i] : 0.f;
         if (last < SR_BINS && inv > 0.f) {
-            loaded(tmax > -INFINITY && bin(tmax) <= last, [&](float v, int i) {
-                if (v > -INFINITY && bin(v) <= last) to_list(v, i);
-            });
+            auto in = [&](float v) { return v > -INFINITY && bin(v) <= last; };
+            if (!look_into(in, [&](float v, int i) {
+                    if (in(v)) to_list(v, i);
+                }))
+                too_many();
         } else {
             few = false;  // fewer maxima than top_k, or equal ones
         }
@@ -504,15 +566,13 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
                                A.probs[row] = (float)(rule.weight(value_of(mine), mx, S.table) * SR_UNIT / (double)total);
                        }
                    });
-            // the other ranks have read n_list before they left
-            cl.sync();
+            cl.sync();  // the other ranks have read n_list before they left
             return;
         }
     }
 
     // ---- many candidates: the cut's range by bins of the distance to the maximum
     u64 cut = 0;  // the last kept (logit, index) pair
-    u64 kept_sum = 0;  // this thread's mass that is certainly kept
     float d0[SR_ROUNDS] = {}, inv[SR_ROUNDS] = {};
     int b0[SR_ROUNDS] = {}, b1[SR_ROUNDS] = {};
     int rounds = 0;
@@ -532,29 +592,33 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         }
         return 0;
     };
+    // kept mass of every warp's run, to rank 0
+    auto push_run = [&](u64 m) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+        if (lane == 0) lead->seg[rank * SR_WARPS + warp] = m;
+    };
+    unsigned c_above = 0, in_range = 0;
     if (cuts) {
         // lowest survivor, and the approximate mass
         float lw = INFINITY, mass = 0.f;
-#pragma unroll 4
-        for (int v = tid; v < nwords; v += SR_THREADS) {
-            float q[N];
-            W::get(xs[v], q);
+        stream([&](float (&v)[E], int) {
 #pragma unroll
-            for (int k = 0; k < N; k++) {
-                const bool in = q[k] >= xmin;
-                lw = in ? fminf(lw, q[k]) : lw;
-                const float e = rough(q[k]);
-                mass += in ? e : 0.f;
+            for (int e = 0; e < E; e++) {
+                const bool in = v[e] >= xmin;
+                lw = in ? fminf(lw, v[e]) : lw;
+                const float p = rough(v[e]);
+                mass += in ? p : 0.f;
             }
-        }
+        });
         lw = sr_reduce(lw, reinterpret_cast<float *>(S.red), minf);
-        mass = sr_reduce(mass, reinterpret_cast<float *>(S.red), [](float a, float b) { return a + b; });
+        mass = sr_reduce(mass, reinterpret_cast<float *>(S.red), addf);
         const float step = mass > 0.f ? __fmul_rn(mass, 0x1p-30f) : 0.f;
         cl.sync();  // the earlier slots have been read
         push(&SrShared::low_of, lw);
         push(&SrShared::mass_of, mass);
         push(&SrShared::unit_of, step);
-        for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[0][i] = S.mass[0][i] = 0;
+        S.cnt[0][tid] = S.mass[0][tid] = 0;
         cl.sync();
         low = INFINITY;
         m1 = 0.f;
@@ -565,25 +629,25 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         const float per = step > 0.f ? __fdiv_rn(1.f, step) : 0.f;
         // weights below 2^-43 share the last bin of the first round
         float lo = 0.f, hi = fminf(dist(low), __fdiv_rn(30.f, rule.c * 0.6931472f));
-        unsigned c_above = 0, in_range = 0;
         float m_above = 0.f;
         for (; rounds < SR_ROUNDS; rounds++) {
             const int buf = rounds & 1;
             const float width = hi - lo;
+            const float nd0 = lo, ninv = width > 0.f && width < INFINITY ? __fdiv_rn((float)(SR_BINS - 1), width) : 0.f;
 #pragma unroll
             for (int r = 0; r < SR_ROUNDS; r++)  // (fixed indexes: the rounds stay in registers)
                 if (r == rounds) {
-                    d0[r] = lo;
-                    inv[r] = width > 0.f && width < INFINITY ? __fdiv_rn((float)(SR_BINS - 1), width) : 0.f;
+                    d0[r] = nd0;
+                    inv[r] = ninv;
                 }
-            own([&](float v, int) {
-                if (!(v >= xmin) || side(v) != 0) return;
-                int b = 0;
+            stream([&](float (&v)[E], int) {
 #pragma unroll
-                for (int r = 0; r < SR_ROUNDS; r++)
-                    if (r == rounds) b = bin_in(dist(v), r);
-                atomicAdd(&S.cnt[buf][b], 1u);
-                if (has_p) atomicAdd(&S.mass[buf][b], __float2uint_rn(__fmul_rn(rough(v), per)));
+                for (int e = 0; e < E; e++) {
+                    if (!(v[e] >= xmin) || side(v[e]) != 0) continue;
+                    const int b = (int)fminf(fmaxf(__fmul_rn(__fsub_rn(dist(v[e]), nd0), ninv), 0.f), (float)(SR_BINS - 1));
+                    atomicAdd(&S.cnt[buf][b], 1u);
+                    if (has_p) atomicAdd(&S.mass[buf][b], __float2uint_rn(__fmul_rn(rough(v[e]), per)));
+                }
             });
             cl.sync();
             unsigned n = 0, n_low = 0, n_all;  // n_low: of the ranks before this one
@@ -600,13 +664,14 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
             // the cut is in the first bin that may complete top_k or top_p, or behind it up to the first that must
             const float need = (float)rule.top_p * m1, slack = 2e-4f * m1;
             const bool full = rule.top_k && nb + n >= (unsigned)rule.top_k;
-            const bool may = n && (full || (has_p && mb + m + slack >= need)), must = n && (full || (has_p && mb + m - slack >= need));
+            const bool may = n && (full || (has_p && mb + m + slack >= need));
+            const bool must = n && (full || (has_p && mb + m - slack >= need));
             if (tid == 0) {
                 S.first_bin = S.last_bin = SR_BINS;
                 S.range_count = S.range_low = 0;
             }
             // (the buffer of the next round was read before this round's barrier)
-            for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[buf ^ 1][i] = S.mass[buf ^ 1][i] = 0;
+            S.cnt[buf ^ 1][tid] = S.mass[buf ^ 1][tid] = 0;
             __syncthreads();
             if (may) atomicMin(&S.first_bin, tid);
             if (must) atomicMin(&S.last_bin, tid);
@@ -617,159 +682,174 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
                 atomicAdd(&S.range_low, n_low);
             }
             if (tid == fb) {
-                S.max_of[0] = mb;  // (the maxima have been read)
+                S.m_at = mb;
                 S.red[31] = nb;
             }
             __syncthreads();
-            in_range = fb < SR_BINS ? S.range_count : 0;
 #pragma unroll
             for (int r = 0; r < SR_ROUNDS; r++)
                 if (r == rounds) {
                     b0[r] = fb;
                     b1[r] = lb;
                 }
+            in_range = fb < SR_BINS ? S.range_count : 0;
             if (fb >= SR_BINS) {  // nothing completes them: all survivors of this range stay
-                in_range = 0;
                 rounds++;
                 break;
             }
             c_above = (unsigned)S.red[31];
-            m_above = S.max_of[0];
+            m_above = S.m_at;
             if (in_range <= SR_LIST) {
                 rounds++;
                 break;
             }
             // the next round divides these bins
             const float w1 = width * (1.f / (SR_BINS - 1));
-            const float nlo = lo + w1 * fb, nhi = lb >= SR_BINS - 1 ? fmaxf(dist(low), hi) : lo + w1 * (lb + 1);
-            lo = nlo;
-            hi = nhi;
+            hi = lb >= SR_BINS - 1 ? fmaxf(dist(low), hi) : lo + w1 * (lb + 1);
+            lo = lo + w1 * fb;
         }
-        // ---- exact masses: above the range (kept), and of all survivors where top-p needs it; the range to rank 0
-        const bool listed = in_range > 0 && in_range <= SR_LIST;
-        const unsigned at0 = S.range_low;  // the entries of the ranks before this one come first
+    }
+    // ---- exact masses: above the range (kept), and of all survivors where top-p needs it; the range to rank 0
+    const bool listed = in_range > 0 && in_range <= SR_LIST;
+    const unsigned at0 = listed ? S.range_low : 0;  // the entries of the ranks before this one come first
+    if (listed) {  // (in other cases a rank may still be reading rank 0's count)
         __syncthreads();
         if (tid == 0) S.n_list = 0;
         __syncthreads();
-        u64 m_all = 0;
-        own([&](float v, int i) {
-            const int s = v >= xmin ? side(v) : -1;
+    }
+    u64 kept = 0, m_all = 0;
+    stream([&](float (&v)[E], int i) {
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int s = v[e] >= xmin ? (cuts ? side(v[e]) : 1) : -1;
             u64 w = 0;
-            if (has_p || s > 0) w = unit_of(v);
-            m_all += v >= xmin ? w : 0;
-            kept_sum += s > 0 ? w : 0;
-            if (s == 0 && listed) lead->list[at0 + atomicAdd(&S.n_list, 1u)] = sr_pair(v, i);
-        });
-        const u64 above = sr_reduce(kept_sum, S.red, addu), all = sr_reduce(m_all, S.red, addu);
-        if (tid < cs) {
-            SrShared *o = cl.map_shared_rank(&S, tid);
-            o->slot[0][rank] = above;
-            o->slot[1][rank] = all;
+            if (has_p || s > 0) w = unit_of(v[e]);
+            m_all += v[e] >= xmin ? w : 0;
+            kept += s > 0 ? w : 0;
+            if (s == 0 && listed) lead->list[at0 + atomicAdd(&S.n_list, 1u)] = sr_pair(v[e], i + e);
         }
-        cl.sync();
-        u64 above_all = 0, mass_all = 0;
+    });
+    push_run(kept);
+    m_all = sr_reduce(m_all, S.red, addu);
+    if (tid == 0) lead->slot[1][rank] = m_all;
+    cl.sync();
+    const bool bisect = in_range > SR_LIST;
+    if (bisect) {
+        // over (key, index) pairs: the largest pair whose upper set completes top_k or top_p
+        u64 above = 0, mass = 0;
         for (int i = 0; i < cs; i++) {
-            above_all += S.slot[0][i];
-            mass_all += S.slot[1][i];
+            mass += lead->slot[1][i];
+            for (int j = 0; j < SR_WARPS; j++) above += lead->seg[i * SR_WARPS + j];
         }
-        const u64 need = has_p ? need_of((double)mass_all) : ~0ull;
-        if (in_range == 0) {
-            cut = 0;  // every survivor down to the range's end
-        } else if (listed) {
-            if (rank == 0) {
-                const int n = (int)in_range;
-                for (int i = tid; i < n; i += SR_THREADS) S.wt[i] = unit_of(value_of(S.list[i]));
-                __syncthreads();
-                find_cut(n, above_all, c_above, need, need);
-                if (tid < cs) cl.map_shared_rank(&S, tid)->cut = S.cut;
+        const u64 need = has_p ? need_of((double)mass) : ~0ull;
+        u64 lo_pair = 0, hi_pair = ~0ull;
+        while (hi_pair - lo_pair > 1) {
+            const u64 mid = lo_pair + (hi_pair - lo_pair) / 2;
+            u64 m = 0, n = 0;
+            stream([&](float (&v)[E], int i) {
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (v[e] >= xmin && side(v[e]) == 0 && sr_pair(v[e], i + e) >= mid) {
+                        n++;
+                        if (has_p) m += unit_of(v[e]);
+                    }
+            });
+            m = sr_reduce(m, S.red, addu);
+            n = sr_reduce(n, S.red, addu);
+            cl.sync();  // the slots of the last turn have been read
+            if (tid < cs) {
+                SrShared *o = cl.map_shared_rank(&S, tid);
+                o->slot[0][rank] = m;
+                o->slot[1][rank] = n;
             }
             cl.sync();
-            cut = S.cut;
-        } else {
-            // bisection over (key, index) pairs: the largest pair whose upper set completes top_k or top_p
-            u64 lo_pair = 0, hi_pair = ~0ull;
-            while (hi_pair - lo_pair > 1) {
-                const u64 mid = lo_pair + (hi_pair - lo_pair) / 2;
-                u64 m = 0, n = 0;
-                own([&](float v, int i) {
-                    if (v >= xmin && side(v) == 0 && sr_pair(v, i) >= mid) {
-                        n++;
-                        if (has_p) m += unit_of(v);
-                    }
-                });
-                m = sr_reduce(m, S.red, addu);
-                n = sr_reduce(n, S.red, addu);
-                cl.sync();  // the slots of the last turn have been read
-                if (tid < cs) {
-                    SrShared *o = cl.map_shared_rank(&S, tid);
-                    o->slot[0][rank] = m;
-                    o->slot[1][rank] = n;
-                }
-                cl.sync();
-                m = above_all;
-                n = c_above;
-                for (int i = 0; i < cs; i++) {
-                    m += S.slot[0][i];
-                    n += S.slot[1][i];
-                }
-                if ((rule.top_k && n >= (u64)rule.top_k) || (has_p && m >= need && m > 0)) lo_pair = mid;
-                else hi_pair = mid;
+            m = above;
+            n = c_above;
+            for (int i = 0; i < cs; i++) {
+                m += S.slot[0][i];
+                n += S.slot[1][i];
             }
-            cut = lo_pair;
+            if ((rule.top_k && n >= (u64)rule.top_k) || (has_p && m >= need && m > 0)) lo_pair = mid;
+            else hi_pair = mid;
         }
-        // what stays inside the range
-        if (in_range)
-            own([&](float v, int i) {
-                if (v >= xmin && side(v) == 0 && sr_pair(v, i) >= cut) kept_sum += unit_of(v);
-            });
-    } else {
-        own([&](float v, int) {
-            if (v >= xmin) kept_sum += unit_of(v);
+        cut = lo_pair;
+        stream([&](float (&v)[E], int i) {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (v[e] >= xmin && side(v[e]) == 0 && sr_pair(v[e], i + e) >= cut) kept += unit_of(v[e]);
         });
+        cl.sync();  // the runs' masses have been read
+        push_run(kept);
+        cl.sync();
     }
-    // ---- the draw, in index order: ranks, threads, logits
-    u64 mine;
-    const u64 before = sr_scan(kept_sum, S.red, &mine);
-    cl.sync();  // the slots have been read
-    if (tid < cs) cl.map_shared_rank(&S, tid)->slot[0][rank] = mine;
-    cl.sync();
-    u64 total = 0, lower = 0;
-    for (int i = 0; i < cs; i++) {
-        if (i < rank) lower += S.slot[0][i];
-        total += S.slot[0][i];
+    if (rank != 0) return;
+    // ---- rank 0 alone: the cut, the run that the draw falls into, the logit
+    if (listed) {
+        const int n = (int)in_range;
+        for (int i = tid; i < n; i += SR_THREADS) S.wt[i] = unit_of(value_of(S.list[i]));
+        u64 above = tid < cs * SR_WARPS ? S.seg[tid] : 0, mass = 0;
+        above = sr_reduce(above, S.red, addu);
+        for (int i = 0; i < cs; i++) mass += S.slot[1][i];
+        const u64 need = has_p ? need_of((double)mass) : ~0ull;
+        find_cut(n, above, c_above, need, need);
+        cut = S.cut;
+        for (int i = tid; i < n; i += SR_THREADS)
+            if (S.list[i] >= cut) atomicAdd(&S.seg[(int)~(uint32_t)S.list[i] / run], S.wt[i]);
+        __syncthreads();
     }
+    const u64 mine = tid < cs * SR_WARPS ? S.seg[tid] : 0;
+    u64 total;
+    const u64 before = sr_scan(mine, S.red, &total);
     u64 target = (u64)(rule.u * (double)total);
     if (target >= total) target = total - 1;
-    u64 run = lower + before;
-    if (run <= target && target < run + kept_sum) {
-        bool found = false;
-        own([&](float v, int i) {
-            if (found || !(v >= xmin)) return;
-            const int s = cuts ? side(v) : 1;
-            if (s < 0 || (s == 0 && sr_pair(v, i) < cut)) return;
+    if (before <= target && target < before + mine) {
+        S.where = tid;
+        S.target = target - before;
+    }
+    __syncthreads();
+    // the run, a piece of consecutive logits a thread
+    const int piece = (run + SR_THREADS - 1) / SR_THREADS;
+    const int p0 = S.where * run + tid * piece, p1 = min(min(p0 + piece, (S.where + 1) * run), A.vocab);
+    auto stays = [&](float v, int i) {
+        if (!(v >= xmin)) return false;
+        const int s = cuts ? side(v) : 1;
+        return s > 0 || (s == 0 && in_range > 0 && sr_pair(v, i) >= cut);
+    };
+    u64 sum = 0, all;
+#pragma unroll 4
+    for (int i = p0; i < p1; i++) {
+        const float v = sr_load(x, i);
+        const u64 w = unit_of(v);
+        sum += stays(v, i) ? w : 0;
+    }
+    u64 upto = sr_scan(sum, S.red, &all);
+    target = S.target;
+    if (upto <= target && target < upto + sum) {
+        for (int i = p0; i < p1; i++) {
+            const float v = sr_load(x, i);
+            if (!stays(v, i)) continue;
             const double w = rule.weight(v, mx, S.table);
-            run += RowRule::units(w);
-            if (run > target) {
-                found = true;
+            upto += RowRule::units(w);
+            if (upto > target) {
                 A.tokens[row] = i;
                 if (A.probs) A.probs[row] = (float)(w * SR_UNIT / (double)total);
+                break;
             }
-        });
+        }
     }
 }
 
-// CTAs a row: as many as bring its logits below SR_CHUNK bytes of shared
-// memory a CTA (four CTAs an SM, so that one's steps hide another's), and more
-// while SMs would stay empty and every thread keeps eight logits.
-constexpr int SR_CHUNK = 48 * 1024;
+// CTAs a row: as many as still find a place at once (four CTAs an SM), while
+// every lane keeps at least SR_AHEAD vectors.
 template <typename T> static void launch_sample_rows(fb_ctx *ctx, SampleRowsArgs A, int64_t rows) {
-    const int64_t bytes = (int64_t)A.vocab * (int64_t)sizeof(T);
+    constexpr int step = SR_THREADS * SR_E<T>;  // logits of one step of a CTA
     int cs = 1;
-    while (cs < SR_CLUSTER && bytes > (int64_t)cs * SR_CHUNK) cs *= 2;
-    while (cs < SR_CLUSTER && rows * cs * 2 <= ctx->num_sms && A.vocab >= 2 * cs * SR_THREADS * 8) cs *= 2;
-    const int64_t words = (bytes + 3) / 4;
-    A.words = (int)((words + (int64_t)cs * SR_THREADS - 1) / ((int64_t)cs * SR_THREADS)) | 1;
-    const size_t smem = (size_t)SR_THREADS * A.words * 4;
+    while (cs < SR_CLUSTER && rows * cs * 2 <= 4 * ctx->num_sms && A.vocab > cs * step * SR_AHEAD) cs *= 2;
+    A.steps = (A.vocab + cs * step - 1) / (cs * step);
+    A.chunk = A.steps * step;
+    // groups of SR_AHEAD vectors, longer ones where a thread would have more than SR_GROUPS of them
+    A.gsteps = SR_AHEAD * ((A.steps + SR_AHEAD * SR_GROUPS - 1) / (SR_AHEAD * SR_GROUPS));
+    const size_t smem = (size_t)((A.steps + A.gsteps - 1) / A.gsteps) * SR_THREADS * 4;
     auto kernel = k_sample_rows<T>;
     FB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     if (cs > 8) FB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
