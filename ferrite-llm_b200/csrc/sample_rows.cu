@@ -112,7 +112,7 @@ __device__ __forceinline__ u64 sr_pair(float x, int i) { return ((u64)sr_key(x) 
 
 // A row's settings.
 struct RowRule {
-    double scale, min_p, top_p, t;  // scale = log2(e) 32 / T; min_p 0: off; top_p 2: off
+    double scale, min_p, top_p, t;  // scale = 64 log2(e) / T; min_p 0: off; top_p 2: off
     float c;                        // log2(e) / T
     int top_k;                      // 0: off
     double u;
@@ -123,37 +123,52 @@ struct RowRule {
         const int k = A.top_k ? A.top_k[r] : 0;
         greedy = tt <= 0.f;
         t = (tt != tt || greedy) ? 1.0 : (double)tt;
-        scale = 46.16624130844683 / t;  // 32 log2(e) / T
-        c = (float)fmin(scale * 0.03125, 1e30);  // (finite: 0 c stays 0)
+        scale = 92.33248261689366 / t;  // 64 log2(e) / T
+        c = (float)fmin(fmax(scale * 0.015625, 1e-30), 1e30);  // (bounded: 0 c stays 0, -FLT_MAX c far below any weight)
         min_p = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
         top_p = tp < 1.f ? fmax((double)tp, 0.0) : 2.0;
         top_k = k > 0 && k < A.vocab ? k : 0;
         u = uu > 0.f ? fmin((double)uu, 1.0) : 0.0;
     }
-    // exp((x - mx) / T) = 2^(z / 32), z = scale (x - mx): the table holds 2^(j / 32), and the rest |f| <= 1/2 of
-    // a step is a Taylor polynomial of e^(f ln2 / 32) (argument below 0.011: degree 5 is below 2^-53).
-    // The maximum itself (infinite too) weighs 1, NaN 0.
+    // exp((x - mx) / T) = 2^(z / 64), z = scale (x - mx): the table holds 2^(j / 64), and the rest |r| <= 1/2 of a
+    // step is the Taylor polynomial of e^(r ln2 / 64) (argument below 0.0055: degree 4 leaves 4e-14).  Of an
+    // infinite maximum only the infinite logits weigh, 1 each; NaN weighs 0.
     __device__ __forceinline__ double weight(float x, float mx, const double *table) const {
-        const double z = __dmul_rn((double)x - (double)mx, scale);
-        const double y = fmax(z, -34400.0);  // 2^-1075 (NaN too)
-        const double q = __dadd_rn(y, 6755399441055744.0);  // 1.5 * 2^52: the nearest integer in the low bits
+        if (mx == INFINITY) return x == mx ? 1.0 : 0.0;
+        const double d = (double)x - (double)mx;
+        const double z = __dmul_rn(d, scale);
+        if (!(z > -68800.0)) return 0.0;  // below 2^-1075, NaN
+        const double p = step(d, table, 0);
+        const int e = __double2loint(__fma_rn(d, scale, 6755399441055744.0)) >> 6, e0 = e / 2;
+        return __dmul_rn(__dmul_rn(p, exp64_pow2(e0)), exp64_pow2(e - e0));  // (e reaches -1075)
+    }
+    // 2^(z / 64 - floor) in [1, 2), or with `whole` the whole weight (z / 64 >= -900)
+    __device__ __forceinline__ double step(double d, const double *table, int whole) const {
+        const double q = __fma_rn(d, scale, 6755399441055744.0);  // 1.5 * 2^52: the nearest integer in the low bits
+        const double r = __fma_rn(d, scale, -__dsub_rn(q, 6755399441055744.0));
+        constexpr double L = 0.010830424696249145;  // ln2 / 64
+        double p = __fma_rn(r, L * L * L * L / 24.0, L * L * L / 6.0);
+        p = __fma_rn(p, r, L * L / 2.0);
+        p = __fma_rn(p, r, L);
+        p = __dmul_rn(p, r);
         const int n = __double2loint(q);
-        const double f = __dmul_rn(__dsub_rn(y, __dsub_rn(q, 6755399441055744.0)), 0.021660849392498290);  // ln2 / 32
-        double p = __fma_rn(f, 1.0 / 120.0, 1.0 / 24.0);
-        p = __fma_rn(p, f, 1.0 / 6.0);
-        p = __fma_rn(p, f, 0.5);
-        p = __fma_rn(p, f, 1.0);
-        p = __fma_rn(p, f, 1.0);
-        p = __dmul_rn(p, table[n & 31]);
-        const int e = n >> 5, e0 = e / 2;  // (two factors: e reaches -1075; the second product rounds once)
-        p = __dmul_rn(__dmul_rn(p, exp64_pow2(e0)), exp64_pow2(e - e0));
-        return x == mx ? 1.0 : z > -34400.0 ? p : 0.0;
+        const double t = table[n & 63];
+        p = __fma_rn(t, p, t);
+        return whole ? __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p)) : p;
     }
     static __device__ __forceinline__ u64 units(double w) {
         if (!(w > 0.0)) return 0ull;
         // w 2^43 <= 2^43: adding 2^52 leaves its nearest integer in the low mantissa bits
         const u64 n = (u64)__double_as_longlong(__fma_rn(w, SR_UNIT, 4503599627370496.0)) & 0xfffffffffffffull;
         return n ? n : 1ull;
+    }
+    // units(weight(x)) for a finite maximum; below `vmin` (weights under 2^-60) the long way
+    __device__ __forceinline__ u64 units_of(float x, float mx, float vmin, const double *table) const {
+        const double w = step((double)fmaxf(x, vmin) - (double)mx, table, 1);
+        u64 n = (u64)__double_as_longlong(__fma_rn(w, SR_UNIT, 4503599627370496.0)) & 0xfffffffffffffull;
+        n += n == 0;
+        if (!(x >= vmin)) n = units(weight(x, mx, table));
+        return n;
     }
 };
 
@@ -196,9 +211,10 @@ struct SrShared {
     u64 slot[2][SR_CLUSTER];                   // pushed by every rank
     u64 red[32];
     u64 cut, kept_mass, target;
-    double table[32];
+    double table[64];
     float max_of[SR_CLUSTER], low_of[SR_CLUSTER], mass_of[SR_CLUSTER];
-    float unit_of[SR_CLUSTER];                 // weight of one step of a rank's mass bins
+    float min_of[SR_CLUSTER];
+    uint32_t edge[2];
     uint32_t cnt[2][SR_BINS], mass[2][SR_BINS];
     uint32_t flagged[SR_FLAGGED];              // groups to look into
     unsigned n_flagged, n_list;                // n_list, rank 0: candidates pushed
@@ -263,11 +279,11 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         }
     };
 
-    // ---- the first pass: the groups' maxima, and for top_k with top-p the approximate mass (each thread's relative to
-    // its own running maximum)
+    // ---- the first pass: the groups' maxima, and for top-p without min-p the approximate mass (each thread's
+    // relative to its own running maximum) and the lowest logit
     const bool by_topk = rule.top_k > 0 && rule.top_k <= SR_TOPK && rule.min_p == 0.0 && !rule.greedy;
     const bool has_p = rule.top_p < 1.0, cuts = rule.top_k > 0 || has_p;
-    if (tid < 32) S.table[tid] = exp2((double)tid * 0.03125);
+    if (tid < 64) S.table[tid] = exp2((double)tid * 0.015625);
     if (tid == 0) S.n_list = S.n_flagged = 0;
     S.cnt[0][tid] = S.mass[0][tid] = 0;
     auto ex2 = [](float y) {
@@ -275,9 +291,9 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
         return e;
     };
-    float tmax = -INFINITY, tsum = 0.f;
+    const bool online = has_p && rule.min_p == 0.0 && !rule.greedy;
+    float tmax = -INFINITY, tsum = 0.f, tmin = INFINITY;
     {
-        const bool online = by_topk && has_p;
         for (int g = 0; g < ngroups; g++) {
             float gm = -INFINITY;
             const int s1 = min(A.steps, (g + 1) * A.gsteps);
@@ -299,6 +315,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
                 gm = fmaxf(gm, m);
                 if (online && m > -INFINITY) {
                     const float top = fmaxf(tmax, m);
+                    const float off = -__fmul_rn(top, rule.c);
                     float sum = tsum > 0.f ? __fmul_rn(tsum, ex2(__fmul_rn(__fsub_rn(tmax, top), rule.c))) : 0.f;
 #pragma unroll
                     for (int k = 0; k < SR_AHEAD; k++) {
@@ -306,8 +323,9 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
                         sr_unpack<T>(q[k], v);
 #pragma unroll
                         for (int e = 0; e < E; e++) {
-                            const float p = ex2(__fmul_rn(__fsub_rn(v[e], top), rule.c));
-                            sum += v[e] > -INFINITY ? p : 0.f;
+                            // (NaN and -inf as -FLT_MAX, which weighs nothing)
+                            sum += ex2(__fmaf_rn(fmaxf(v[e], -3.4028235e38f), rule.c, off));
+                            tmin = fminf(tmin, v[e] > -INFINITY ? v[e] : INFINITY);
                         }
                     }
                     tsum = sum;
@@ -348,9 +366,17 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
     };
     const float bmax = sr_reduce(tmax, reinterpret_cast<float *>(S.red), maxf);
     const float blow = sr_reduce(tmax > -INFINITY ? tmax : INFINITY, reinterpret_cast<float *>(S.red), minf);
+    float bsum = 0.f, bmin = INFINITY;
+    if (online) {  // (relative to this CTA's maximum)
+        bsum = sr_reduce(tsum > 0.f ? __fmul_rn(tsum, ex2(__fmul_rn(__fsub_rn(tmax, bmax), rule.c))) : 0.f,
+                         reinterpret_cast<float *>(S.red), addf);
+        bmin = sr_reduce(tmin, reinterpret_cast<float *>(S.red), minf);
+    }
     if (cs > 1) cl.sync();  // every rank has started
     push(&SrShared::max_of, bmax);
     push(&SrShared::low_of, blow);
+    push(&SrShared::mass_of, bsum);
+    push(&SrShared::min_of, bmin);
     cl.sync();
     float mx = -INFINITY, low = INFINITY;  // the largest logit, the lowest of the threads' finite maxima
     for (int i = 0; i < cs; i++) {
@@ -403,7 +429,10 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         __syncthreads();
     }
     const float xmin = rule.min_p > 0.0 ? sr_unkey(S.kmin) : -3.4028235e38f;  // survivors: x >= xmin
-    auto unit_of = [&](float v) { return RowRule::units(rule.weight(v, mx, S.table)); };
+    const float vmin = rule.t < 1e30 ? (float)((double)mx - 41.0 * rule.t) : -3.4028235e38f;  // weight 2^-59
+    auto unit_of = [&](float v) {
+        return mx == INFINITY ? RowRule::units(rule.weight(v, mx, S.table)) : rule.units_of(v, mx, vmin, S.table);
+    };
     // binary32 weight, relative error below 1e-5 wherever it is not negligible
     auto rough = [&](float v) {
         const float e = ex2(__fmul_rn(__fsub_rn(v, mx), rule.c));
@@ -421,6 +450,9 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
     };
     bool few = false;
     float m1 = 0.f;  // approximate mass of the survivors
+    if (online)
+        for (int i = 0; i < cs; i++)
+            if (S.mass_of[i] > 0.f) m1 += __fmul_rn(S.mass_of[i], rough(S.max_of[i]));
     if (rule.min_p > 0.0) {
         few = true;
         if (!look_into([&](float m) { return m >= xmin; },
@@ -441,11 +473,6 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
             const int b = m > -INFINITY ? bin(m) : SR_BINS - 1;
             if (b < SR_BINS - 1) atomicAdd(&S.cnt[0][b], 1u);
         }
-        if (has_p) {
-            const float m = sr_reduce(tsum > 0.f ? __fmul_rn(tsum, rough(tmax)) : 0.f,
-                                      reinterpret_cast<float *>(S.red), addf);
-            push(&SrShared::mass_of, m);
-        }
         cl.sync();
         if (tid == 0) S.last_bin = SR_BINS;
         unsigned n = 0, all;
@@ -454,7 +481,6 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         if (before < (unsigned)rule.top_k && before + n >= (unsigned)rule.top_k) S.last_bin = tid;
         __syncthreads();
         const int last = S.last_bin;
-        for (int i = 0; i < cs; i++) m1 += has_p ? S.mass_of[i] : 0.f;
         if (last < SR_BINS && inv > 0.f) {
             auto in = [&](float v) { return v > -INFINITY && bin(v) <= last; };
             if (!look_into(in, [&](float v, int i) {
@@ -573,25 +599,11 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
 
     // ---- many candidates: the cut's range by bins of the distance to the maximum
     u64 cut = 0;  // the last kept (logit, index) pair
-    float d0[SR_ROUNDS] = {}, inv[SR_ROUNDS] = {};
-    int b0[SR_ROUNDS] = {}, b1[SR_ROUNDS] = {};
-    int rounds = 0;
-    // where a survivor lies: 1 above the range (kept), 0 inside, -1 below
+    // survivors from xa on stay, those in xb .. xa are the range that the cut lies in
+    float xa = cuts ? INFINITY : xmin, xb = xmin;
+    bool to_top = cuts;  // the range still reaches the maximum
+    auto side = [&](float v) { return !to_top && v >= xa ? 1 : v >= xb ? 0 : -1; };
     auto dist = [&](float v) { return v == mx ? 0.f : __fsub_rn(mx, v); };
-    auto bin_in = [&](float d, int r) {
-        return (int)fminf(fmaxf(__fmul_rn(__fsub_rn(d, d0[r]), inv[r]), 0.f), (float)(SR_BINS - 1));
-    };
-    auto side = [&](float v) {
-        const float d = dist(v);
-#pragma unroll
-        for (int r = 0; r < SR_ROUNDS; r++) {
-            if (r >= rounds) break;
-            const int b = bin_in(d, r);
-            if (b < b0[r]) return 1;
-            if (b > b1[r]) return -1;
-        }
-        return 0;
-    };
     // kept mass of every warp's run, to rank 0
     auto push_run = [&](u64 m) {
 #pragma unroll
@@ -600,53 +612,61 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
     };
     unsigned c_above = 0, in_range = 0;
     if (cuts) {
-        // lowest survivor, and the approximate mass
-        float lw = INFINITY, mass = 0.f;
-        stream([&](float (&v)[E], int) {
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const bool in = v[e] >= xmin;
-                lw = in ? fminf(lw, v[e]) : lw;
-                const float p = rough(v[e]);
-                mass += in ? p : 0.f;
-            }
-        });
-        lw = sr_reduce(lw, reinterpret_cast<float *>(S.red), minf);
-        mass = sr_reduce(mass, reinterpret_cast<float *>(S.red), addf);
-        const float step = mass > 0.f ? __fmul_rn(mass, 0x1p-30f) : 0.f;
-        cl.sync();  // the earlier slots have been read
-        push(&SrShared::low_of, lw);
-        push(&SrShared::mass_of, mass);
-        push(&SrShared::unit_of, step);
-        S.cnt[0][tid] = S.mass[0][tid] = 0;
-        cl.sync();
-        low = INFINITY;
-        m1 = 0.f;
-        for (int i = 0; i < cs; i++) {
-            low = fminf(low, S.low_of[i]);
-            m1 += S.mass_of[i];
-        }
-        const float per = step > 0.f ? __fdiv_rn(1.f, step) : 0.f;
-        // weights below 2^-43 share the last bin of the first round
-        float lo = 0.f, hi = fminf(dist(low), __fdiv_rn(30.f, rule.c * 0.6931472f));
-        float m_above = 0.f;
-        for (; rounds < SR_ROUNDS; rounds++) {
-            const int buf = rounds & 1;
-            const float width = hi - lo;
-            const float nd0 = lo, ninv = width > 0.f && width < INFINITY ? __fdiv_rn((float)(SR_BINS - 1), width) : 0.f;
-#pragma unroll
-            for (int r = 0; r < SR_ROUNDS; r++)  // (fixed indexes: the rounds stay in registers)
-                if (r == rounds) {
-                    d0[r] = nd0;
-                    inv[r] = ninv;
-                }
+        // lowest survivor, and the approximate mass, as far as the first pass has not found them
+        if (!online) {
+            float lw = INFINITY, mass = 0.f;
             stream([&](float (&v)[E], int) {
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    if (!(v[e] >= xmin) || side(v[e]) != 0) continue;
-                    const int b = (int)fminf(fmaxf(__fmul_rn(__fsub_rn(dist(v[e]), nd0), ninv), 0.f), (float)(SR_BINS - 1));
-                    atomicAdd(&S.cnt[buf][b], 1u);
-                    if (has_p) atomicAdd(&S.mass[buf][b], __float2uint_rn(__fmul_rn(rough(v[e]), per)));
+                    const bool in = v[e] >= xmin;
+                    lw = in ? fminf(lw, v[e]) : lw;
+                    const float p = rough(v[e]);
+                    mass += in ? p : 0.f;
+                }
+            });
+            lw = sr_reduce(lw, reinterpret_cast<float *>(S.red), minf);
+            mass = sr_reduce(mass, reinterpret_cast<float *>(S.red), addf);
+            cl.sync();  // the earlier values have been read
+            push(&SrShared::min_of, lw);
+            push(&SrShared::mass_of, mass);
+            S.cnt[0][tid] = 0;
+            cl.sync();
+        } else if (by_topk) {
+            cl.sync();  // the counts have been read
+            S.cnt[0][tid] = 0;
+            __syncthreads();
+        }
+        // a rank's approximate mass; its bins count it in units of 2^-30
+        auto mass_at = [&](int i) {
+            const float m = S.mass_of[i];
+            return online && m > 0.f ? __fmul_rn(m, rough(S.max_of[i])) : m;
+        };
+        float lowest = INFINITY;
+        for (int i = 0; i < cs; i++) lowest = fminf(lowest, S.min_of[i]);
+        if (!online) {
+            m1 = 0.f;
+            for (int i = 0; i < cs; i++) m1 += S.mass_of[i];
+        }
+        const float step = __fmul_rn(mass_at(rank), 0x1p-30f), per = step > 0.f ? __fdiv_rn(1.f, step) : 0.f;
+        // weights below 2^-43 share the last bin of the first round
+        float lo = 0.f, hi = fminf(dist(lowest), __fdiv_rn(30.f, rule.c * 0.6931472f));
+        float m_above = 0.f;
+        for (int round = 0; round < SR_ROUNDS; round++) {
+            const int buf = round & 1;
+            const float width = hi - lo;
+            const float inv = width > 0.f && width < INFINITY ? __fdiv_rn((float)(SR_BINS - 1), width) : 0.f;
+            auto bin = [&](float v) {
+                return (int)fminf(fmaxf(__fmul_rn(__fsub_rn(dist(v), lo), inv), 0.f), (float)(SR_BINS - 1));
+            };
+            stream([&](float (&v)[E], int) {
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const int b = bin(v[e]);
+                    const uint32_t m = has_p ? __float2uint_rn(__fmul_rn(rough(v[e]), per)) : 0u;
+                    if (side(v[e]) == 0) {
+                        atomicAdd(&S.cnt[buf][b], 1u);
+                        if (m) atomicAdd(&S.mass[buf][b], m);
+                    }
                 }
             });
             cl.sync();
@@ -656,7 +676,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
                 const SrShared *o = cl.map_shared_rank(&S, i);
                 if (i == rank) n_low = n;
                 n += o->cnt[buf][tid];
-                if (has_p) m += __fmul_rn((float)o->mass[buf][tid], S.unit_of[i]);
+                if (has_p) m += __fmul_rn((float)o->mass[buf][tid], __fmul_rn(mass_at(i), 0x1p-30f));
             }
             const unsigned nb = c_above + sr_scan(n, reinterpret_cast<unsigned *>(S.red), &n_all);
             __syncthreads();
@@ -685,27 +705,39 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
                 S.m_at = mb;
                 S.red[31] = nb;
             }
-            __syncthreads();
-#pragma unroll
-            for (int r = 0; r < SR_ROUNDS; r++)
-                if (r == rounds) {
-                    b0[r] = fb;
-                    b1[r] = lb;
+            // the bins' edges as keys (the lowest logit of a bin below fb, and of one up to lb): bins descend with the
+            // logit, so 32 lanes close in on the first key that satisfies
+            if (warp < 2) {
+                const int bound = warp == 0 ? fb - 1 : lb;
+                uint32_t l = sr_key(xb) - 1, h = to_top ? sr_key(mx) + 1 : sr_key(xa);  // never l, always h
+                while (h - l > 1) {
+                    const uint32_t k = l + (uint32_t)(((u64)(h - l) * (lane + 1)) >> 5);
+                    const bool in = k >= h || (k > l && bin(sr_unkey(k)) <= bound);
+                    const int w = __ffs(__ballot_sync(0xffffffffu, in)) - 1;
+                    const uint32_t nh = __shfl_sync(0xffffffffu, k, w), nl = __shfl_sync(0xffffffffu, k, max(w - 1, 0));
+                    h = min(nh, h);
+                    l = w > 0 ? nl : l;
                 }
-            in_range = fb < SR_BINS ? S.range_count : 0;
-            if (fb >= SR_BINS) {  // nothing completes them: all survivors of this range stay
-                rounds++;
+                if (lane == 0) S.edge[warp] = h;
+            }
+            __syncthreads();
+            if (fb >= SR_BINS) {  // nothing completes them: all survivors stay
+                in_range = 0;
+                xa = xb;
+                to_top = false;
                 break;
             }
+            in_range = S.range_count;
             c_above = (unsigned)S.red[31];
             m_above = S.m_at;
-            if (in_range <= SR_LIST) {
-                rounds++;
-                break;
-            }
+            const uint32_t ka = S.edge[0], kb = S.edge[1];
+            to_top = to_top && ka > sr_key(mx);
+            if (!to_top) xa = sr_unkey(ka);
+            xb = sr_unkey(kb);
+            if (in_range <= SR_LIST) break;
             // the next round divides these bins
             const float w1 = width * (1.f / (SR_BINS - 1));
-            hi = lb >= SR_BINS - 1 ? fmaxf(dist(low), hi) : lo + w1 * (lb + 1);
+            hi = lb >= SR_BINS - 1 ? fmaxf(dist(lowest), hi) : lo + w1 * (lb + 1);
             lo = lo + w1 * fb;
         }
     }
@@ -721,7 +753,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
     stream([&](float (&v)[E], int i) {
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const int s = v[e] >= xmin ? (cuts ? side(v[e]) : 1) : -1;
+            const int s = side(v[e]);
             u64 w = 0;
             if (has_p || s > 0) w = unit_of(v[e]);
             m_all += v[e] >= xmin ? w : 0;
@@ -749,7 +781,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
             stream([&](float (&v)[E], int i) {
 #pragma unroll
                 for (int e = 0; e < E; e++)
-                    if (v[e] >= xmin && side(v[e]) == 0 && sr_pair(v[e], i + e) >= mid) {
+                    if (side(v[e]) == 0 && sr_pair(v[e], i + e) >= mid) {
                         n++;
                         if (has_p) m += unit_of(v[e]);
                     }
@@ -776,7 +808,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         stream([&](float (&v)[E], int i) {
 #pragma unroll
             for (int e = 0; e < E; e++)
-                if (v[e] >= xmin && side(v[e]) == 0 && sr_pair(v[e], i + e) >= cut) kept += unit_of(v[e]);
+                if (side(v[e]) == 0 && sr_pair(v[e], i + e) >= cut) kept += unit_of(v[e]);
         });
         cl.sync();  // the runs' masses have been read
         push_run(kept);
@@ -811,8 +843,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
     const int piece = (run + SR_THREADS - 1) / SR_THREADS;
     const int p0 = S.where * run + tid * piece, p1 = min(min(p0 + piece, (S.where + 1) * run), A.vocab);
     auto stays = [&](float v, int i) {
-        if (!(v >= xmin)) return false;
-        const int s = cuts ? side(v) : 1;
+        const int s = side(v);
         return s > 0 || (s == 0 && in_range > 0 && sr_pair(v, i) >= cut);
     };
     u64 sum = 0, all;
