@@ -7,8 +7,8 @@
 // prefix, so the kept set is the shortest of the three and ends at one (logit,
 // index) pair, the cut.  Masses are 64-bit integers in units of 2^-43 (vocab <=
 // 2^19 keeps them below 2^62), summed in any order with one result; a weight
-// that is not zero counts for one unit at least, so no kept token is
-// unreachable.
+// counts for its whole units and one more (none below e^-745), so no kept token
+// is unreachable.
 //
 // Bound: HBM for many rows (a row streams through registers once; what comes
 // later reads a few of its vectors, or passes that find it in L2); a few rows
@@ -18,13 +18,13 @@
 //  * min-p: the threshold logit is found exactly (the f32 whose binary64 weight
 //    is the first to reach min_p); the survivors are the candidates;
 //  * top_k <= SR_TOPK: at least top_k of the groups' maxima lie above the
-//    threshold that a 256-bin count of these maxima gives, so the cut does too:
+//    threshold that a 512-bin count of these maxima gives, so the cut does too:
 //    the logits above it are the candidates (a little over top_k of them);
-//  * otherwise: counts and approximate masses of 256 bins of the distance to
+//  * otherwise: counts and approximate masses of 512 bins of the distance to
 //    the maximum narrow the cut down to a range of at most SR_LIST logits, all
 //    above it are kept.
-// One CTA ranks the candidates against each other with exact weights (no sort:
-// 512 at most, a few lanes each) and draws; the cluster's other CTAs are gone by
+// One CTA orders the candidates (ranked against each other up to 128, else by a
+// bitonic sort), adds up their exact weights and draws; the cluster's other CTAs are gone by
 // then.  A decision that leans on approximate masses is taken with their error
 // on both sides; where that leaves it open, the exact mass of the row is summed.
 // Rows whose cut falls among more than SR_LIST logits that no bin tells apart are
@@ -45,8 +45,9 @@ constexpr int SR_WARPS = SR_THREADS / 32;
 constexpr int SR_MAX_VOCAB = 1 << 19;
 constexpr int SR_LIST = 512;    // candidates one CTA ranks
 constexpr int SR_EACH = SR_LIST / SR_THREADS;
+constexpr int SR_RANKED = 128;  // up to here every candidate is compared with all others
 constexpr int SR_TOPK = 256;    // top_k up to here goes by the groups' maxima
-constexpr int SR_BINS = 256;
+constexpr int SR_BINS = 512;
 constexpr int SR_CLUSTER = 16;
 constexpr int SR_ROUNDS = 4;    // narrowings before the bisection
 constexpr int SR_GROUPS = 48;   // groups a thread, at most
@@ -93,6 +94,26 @@ template <typename T> __device__ __forceinline__ void sr_get16(const uint4 &q, f
 template <typename T> __device__ __forceinline__ void sr_unpack(const uint4 &q, float (&v)[SR_E<T>]) {
     if constexpr (sizeof(T) == 4) sr_get(q, v);
     else sr_get16<T>(q, v);
+}
+// Larger logit of each place (the other one where one is NaN).
+__device__ __forceinline__ uint32_t sr_max32(uint32_t a, uint32_t b, float) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+__device__ __forceinline__ uint32_t sr_max32(uint32_t a, uint32_t b, __half) {
+    const __half2 m = __hmax2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&m);
+}
+__device__ __forceinline__ uint32_t sr_max32(uint32_t a, uint32_t b, __nv_bfloat16) {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162 *>(&a), *reinterpret_cast<__nv_bfloat162 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&m);
+}
+template <typename T> __device__ __forceinline__ uint4 sr_max(const uint4 &a, const uint4 &b) {
+    return make_uint4(sr_max32(a.x, b.x, T{}), sr_max32(a.y, b.y, T{}), sr_max32(a.z, b.z, T{}), sr_max32(a.w, b.w, T{}));
+}
+// The lowest finite f32 or bf16 in every place.
+template <typename T> __device__ __forceinline__ uint4 sr_lowest() {
+    const uint32_t w = sizeof(T) == 4 ? 0xff7fffffu : 0xff7fff7fu;
+    return make_uint4(w, w, w, w);
 }
 __device__ __forceinline__ float sr_load(const float *p, int i) { return p[i]; }
 __device__ __forceinline__ float sr_load(const __half *p, int i) { return __half2float(p[i]); }
@@ -156,19 +177,11 @@ struct RowRule {
         p = __fma_rn(t, p, t);
         return whole ? __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p)) : p;
     }
-    static __device__ __forceinline__ u64 units(double w) {
-        if (!(w > 0.0)) return 0ull;
-        // w 2^43 <= 2^43: adding 2^52 leaves its nearest integer in the low mantissa bits
-        const u64 n = (u64)__double_as_longlong(__fma_rn(w, SR_UNIT, 4503599627370496.0)) & 0xfffffffffffffull;
-        return n ? n : 1ull;
-    }
-    // units(weight(x)) for a finite maximum; below `vmin` (weights under 2^-60) the long way
-    __device__ __forceinline__ u64 units_of(float x, float mx, float vmin, const double *table) const {
+    // One unit and the whole units of the weight, as a double (exact: at most 2^43 + 1), for a finite maximum and x >=
+    // the lowest logit that weighs at all; below vmin (weights under 2^-59) that is one unit.
+    __device__ __forceinline__ double units_of(float x, float mx, float vmin, const double *table) const {
         const double w = step((double)fmaxf(x, vmin) - (double)mx, table, 1);
-        u64 n = (u64)__double_as_longlong(__fma_rn(w, SR_UNIT, 4503599627370496.0)) & 0xfffffffffffffull;
-        n += n == 0;
-        if (!(x >= vmin)) n = units(weight(x, mx, table));
-        return n;
+        return __dsub_rn(__fma_rd(w, SR_UNIT, 4503599627370496.0), 4503599627370495.0);  // + 2^52 - (2^52 - 1)
     }
 };
 
@@ -213,9 +226,8 @@ struct SrShared {
     u64 cut, kept_mass, target;
     double table[64];
     float max_of[SR_CLUSTER], low_of[SR_CLUSTER], mass_of[SR_CLUSTER];
-    float min_of[SR_CLUSTER];
     uint32_t edge[2];
-    uint32_t cnt[2][SR_BINS], mass[2][SR_BINS];
+    alignas(8) uint32_t cnt[2][SR_BINS], mass[2][SR_BINS];
     uint32_t flagged[SR_FLAGGED];              // groups to look into
     unsigned n_flagged, n_list;                // n_list, rank 0: candidates pushed
     int first_bin, last_bin, where;
@@ -224,9 +236,9 @@ struct SrShared {
     uint32_t kmin;
 };
 
-static_assert(SR_BINS == SR_THREADS && SR_CLUSTER * SR_WARPS <= SR_THREADS, "a thread a bin, a thread a run");
+static_assert(SR_BINS == 2 * SR_THREADS && SR_CLUSTER * SR_WARPS <= SR_THREADS, "a thread two bins, a thread a run");
 
-template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_rows(const SampleRowsArgs A) {
+template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_rows(const SampleRowsArgs A) {
     constexpr int E = SR_E<T>;
     extern __shared__ float gmax[];  // [group][thread] largest logit
     __shared__ SrShared S;
@@ -239,6 +251,10 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
     const int ngroups = (A.steps + A.gsteps - 1) / A.gsteps;
     RowRule rule;
     rule.load(A, row);
+    auto csync = [&]() {
+        if (cs > 1) cl.sync();
+        else __syncthreads();
+    };
     auto addu = [](u64 a, u64 b) { return a + b; };
     auto addf = [](float a, float b) { return a + b; };
     auto maxf = [](float a, float b) { return fmaxf(a, b); };
@@ -280,60 +296,70 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
     };
 
     // ---- the first pass: the groups' maxima, and for top-p without min-p the approximate mass (each thread's
-    // relative to its own running maximum) and the lowest logit
+    // relative to its own running maximum)
     const bool by_topk = rule.top_k > 0 && rule.top_k <= SR_TOPK && rule.min_p == 0.0 && !rule.greedy;
     const bool has_p = rule.top_p < 1.0, cuts = rule.top_k > 0 || has_p;
     if (tid < 64) S.table[tid] = exp2((double)tid * 0.015625);
     if (tid == 0) S.n_list = S.n_flagged = 0;
-    S.cnt[0][tid] = S.mass[0][tid] = 0;
+    for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[0][i] = S.mass[0][i] = 0;
     auto ex2 = [](float y) {
         float e;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
         return e;
     };
     const bool online = has_p && rule.min_p == 0.0 && !rule.greedy;
-    float tmax = -INFINITY, tsum = 0.f, tmin = INFINITY;
+    float tmax = -INFINITY, tsum = 0.f;
     {
-        for (int g = 0; g < ngroups; g++) {
-            float gm = -INFINITY;
-            const int s1 = min(A.steps, (g + 1) * A.gsteps);
-            for (int s = g * A.gsteps; s < s1; s += SR_AHEAD) {
-                const int i0 = base + (s * 32 + lane) * E;
-                if (i0 - lane * E >= A.vocab) break;
-                uint4 q[SR_AHEAD];
-                float m = -INFINITY;
+        // batches of SR_AHEAD vectors, the next one in flight while this one is looked at
+        auto load = [&](int s, uint4 (&q)[SR_AHEAD]) {
+            const int i0 = base + (s * 32 + lane) * E;
 #pragma unroll
-                for (int k = 0; k < SR_AHEAD; k++)
-                    q[k] = s + k < s1 ? fetch(i0 + k * 32 * E) : make_uint4(~0u, ~0u, ~0u, ~0u);
+            for (int k = 0; k < SR_AHEAD; k++)
+                q[k] = s + k < A.steps ? fetch(i0 + k * 32 * E) : make_uint4(~0u, ~0u, ~0u, ~0u);
+        };
+        float gm = -INFINITY;
+        int g = 0, ahead = A.gsteps;  // the group, and its steps to come
+        uint4 q[SR_AHEAD], nq[SR_AHEAD];
+        load(0, q);
+        for (int s = 0; s < A.steps; s += SR_AHEAD) {
+            if (s + SR_AHEAD < A.steps) load(s + SR_AHEAD, nq);
+            uint4 top4 = q[0];
+#pragma unroll
+            for (int k = 1; k < SR_AHEAD; k++) top4 = sr_max<T>(top4, q[k]);
+            float m = -INFINITY;
+            {
+                float v[E];
+                sr_unpack<T>(top4, v);
+#pragma unroll
+                for (int e = 0; e < E; e++) m = fmaxf(m, v[e]);
+            }
+            gm = fmaxf(gm, m);
+            if (online && m > -INFINITY) {
+                const float top = fmaxf(tmax, m);
+                const float off = -__fmul_rn(top, rule.c);
+                float sum = tsum > 0.f ? __fmul_rn(tsum, ex2(__fmul_rn(__fsub_rn(tmax, top), rule.c))) : 0.f;
 #pragma unroll
                 for (int k = 0; k < SR_AHEAD; k++) {
                     float v[E];
-                    sr_unpack<T>(q[k], v);
+                    // NaN and -inf as the lowest f32 or bf16, which weighs nothing at any T (fp16's would)
+                    constexpr bool half = std::is_same<T, __half>::value;
+                    sr_unpack<T>(half ? q[k] : sr_max<T>(q[k], sr_lowest<T>()), v);
 #pragma unroll
-                    for (int e = 0; e < E; e++) m = fmaxf(m, v[e]);
+                    for (int e = 0; e < E; e++)
+                        sum += ex2(__fmaf_rn(half ? fmaxf(v[e], -3.4028235e38f) : v[e], rule.c, off));
                 }
-                gm = fmaxf(gm, m);
-                if (online && m > -INFINITY) {
-                    const float top = fmaxf(tmax, m);
-                    const float off = -__fmul_rn(top, rule.c);
-                    float sum = tsum > 0.f ? __fmul_rn(tsum, ex2(__fmul_rn(__fsub_rn(tmax, top), rule.c))) : 0.f;
-#pragma unroll
-                    for (int k = 0; k < SR_AHEAD; k++) {
-                        float v[E];
-                        sr_unpack<T>(q[k], v);
-#pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            // (NaN and -inf as -FLT_MAX, which weighs nothing)
-                            sum += ex2(__fmaf_rn(fmaxf(v[e], -3.4028235e38f), rule.c, off));
-                            tmin = fminf(tmin, v[e] > -INFINITY ? v[e] : INFINITY);
-                        }
-                    }
-                    tsum = sum;
-                    tmax = top;
-                }
+                tsum = sum;
             }
-            gmax[g * SR_THREADS + tid] = gm;
-            tmax = fmaxf(tmax, gm);
+            tmax = fmaxf(tmax, m);
+            ahead -= SR_AHEAD;
+            if (ahead <= 0 || s + SR_AHEAD >= A.steps) {
+                gmax[g * SR_THREADS + tid] = gm;
+                gm = -INFINITY;
+                g++;
+                ahead = A.gsteps;
+            }
+#pragma unroll
+            for (int k = 0; k < SR_AHEAD; k++) q[k] = nq[k];
         }
     }
     // f(logit, index) over the logits of the groups whose maximum satisfies pred; false: too many such groups
@@ -366,18 +392,15 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
     };
     const float bmax = sr_reduce(tmax, reinterpret_cast<float *>(S.red), maxf);
     const float blow = sr_reduce(tmax > -INFINITY ? tmax : INFINITY, reinterpret_cast<float *>(S.red), minf);
-    float bsum = 0.f, bmin = INFINITY;
-    if (online) {  // (relative to this CTA's maximum)
+    float bsum = 0.f;
+    if (online)  // (relative to this CTA's maximum)
         bsum = sr_reduce(tsum > 0.f ? __fmul_rn(tsum, ex2(__fmul_rn(__fsub_rn(tmax, bmax), rule.c))) : 0.f,
                          reinterpret_cast<float *>(S.red), addf);
-        bmin = sr_reduce(tmin, reinterpret_cast<float *>(S.red), minf);
-    }
-    if (cs > 1) cl.sync();  // every rank has started
+    if (cs > 1) csync();  // every rank has started
     push(&SrShared::max_of, bmax);
     push(&SrShared::low_of, blow);
     push(&SrShared::mass_of, bsum);
-    push(&SrShared::min_of, bmin);
-    cl.sync();
+    csync();
     float mx = -INFINITY, low = INFINITY;  // the largest logit, the lowest of the threads' finite maxima
     for (int i = 0; i < cs; i++) {
         mx = fmaxf(mx, S.max_of[i]);
@@ -396,7 +419,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
             });
         first = sr_reduce(first, S.red, [](u64 a, u64 b) { return a < b ? a : b; });
         if (tid == 0) cl.map_shared_rank(&S, 0)->slot[0][rank] = first;
-        cl.sync();
+        csync();
         if (rank == 0 && tid == 0) {
             for (int i = 0; i < cs; i++) first = min(first, S.slot[0][i]);
             A.tokens[row] = first == ~0ull ? -1 : (int)first;
@@ -430,9 +453,14 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
     }
     const float xmin = rule.min_p > 0.0 ? sr_unkey(S.kmin) : -3.4028235e38f;  // survivors: x >= xmin
     const float vmin = rule.t < 1e30 ? (float)((double)mx - 41.0 * rule.t) : -3.4028235e38f;  // weight 2^-59
-    auto unit_of = [&](float v) {
-        return mx == INFINITY ? RowRule::units(rule.weight(v, mx, S.table)) : rule.units_of(v, mx, vmin, S.table);
+    const float vzero = rule.t < 1e30 ? (float)((double)mx - 745.0 * rule.t) : -3.4028235e38f;  // weighs nothing below
+    // units of a logit as a double: a thread adds up to 2^9 of them exactly (2^52)
+    auto unit_d = [&](float v) {
+        if (mx == INFINITY) return v == mx ? SR_UNIT : 0.0;
+        const double n = rule.units_of(v, mx, vmin, S.table);
+        return v >= vzero ? n : 0.0;  // (NaN and -inf too)
     };
+    auto unit_of = [&](float v) { return (u64)unit_d(v); };
     // binary32 weight, relative error below 1e-5 wherever it is not negligible
     auto rough = [&](float v) {
         const float e = ex2(__fmul_rn(__fsub_rn(v, mx), rule.c));
@@ -464,7 +492,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         few = true;
         const float span = __fsub_rn(mx, low);
         const float inv = span > 0.f && span < INFINITY ? __fdiv_rn((float)(SR_BINS - 1), span) : 0.f;
-        // (distances beyond the threads' lowest maximum share bin 255, which cannot be the threshold)
+        // (distances beyond the threads' lowest maximum share the last bin, which cannot be the threshold)
         auto bin = [&](float v) {
             return v == mx ? 0 : (int)fminf(__fmul_rn(__fsub_rn(mx, v), inv), (float)(SR_BINS - 1));
         };
@@ -473,12 +501,20 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
             const int b = m > -INFINITY ? bin(m) : SR_BINS - 1;
             if (b < SR_BINS - 1) atomicAdd(&S.cnt[0][b], 1u);
         }
-        cl.sync();
+        csync();
         if (tid == 0) S.last_bin = SR_BINS;
-        unsigned n = 0, all;
-        for (int i = 0; i < cs; i++) n += cl.map_shared_rank(&S, i)->cnt[0][tid];
-        const unsigned before = sr_scan(n, reinterpret_cast<unsigned *>(S.red), &all);
-        if (before < (unsigned)rule.top_k && before + n >= (unsigned)rule.top_k) S.last_bin = tid;
+        unsigned n[2] = {0, 0}, all;
+        for (int i = 0; i < cs; i++) {
+            const uint2 c2 = *reinterpret_cast<const uint2 *>(&cl.map_shared_rank(&S, i)->cnt[0][2 * tid]);
+            n[0] += c2.x;
+            n[1] += c2.y;
+        }
+        unsigned before = sr_scan(n[0] + n[1], reinterpret_cast<unsigned *>(S.red), &all);
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            if (before < (unsigned)rule.top_k && before + n[k] >= (unsigned)rule.top_k) S.last_bin = 2 * tid + k;
+            before += n[k];
+        }
         __syncthreads();
         const int last = S.last_bin;
         if (last < SR_BINS && inv > 0.f) {
@@ -494,64 +530,102 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
 
     auto value_of = [](u64 pr) { return sr_unkey((uint32_t)(pr >> 32)); };
     auto need_of = [&](double mass) { return (u64)ceil(rule.top_p * mass); };
-    // The block ranks the n list entries: a group of lanes adds up, for one entry, what pred lets count.
+    // Few entries: the block ranks them, a group of lanes adding up for one entry what counts() lets count.
     auto ranked = [&](int n, auto counts, auto use) {
         int g = 1;  // lanes an entry
         while (g < 32 && g * 2 * n <= SR_THREADS) g *= 2;
-        for (int c = tid / g; c < (n + SR_THREADS / g - 1) / (SR_THREADS / g) * (SR_THREADS / g); c += SR_THREADS / g) {
-            const u64 mine = c < n ? S.list[c] : 0;
-            u64 mass = 0;
-            int number = 0;
-            for (int j = tid & (g - 1); j < n; j += g)
-                if (counts(S.list[j], mine)) {
-                    number++;
-                    mass += S.wt[j];
-                }
-            for (int o = 1; o < g; o <<= 1) {
-                number += __shfl_xor_sync(0xffffffffu, number, o);
-                mass += __shfl_xor_sync(0xffffffffu, mass, o);
+        const int c = tid / g;
+        const u64 mine = c < n ? S.list[c] : 0;
+        u64 mass = 0;
+        int number = 0;
+        for (int j = tid & (g - 1); j < n; j += g)
+            if (counts(S.list[j], mine)) {
+                number++;
+                mass += S.wt[j];
             }
-            if (c < n && (tid & (g - 1)) == 0) use(c, mine, number, mass);
+        for (int o = 1; o < g; o <<= 1) {
+            number += __shfl_xor_sync(0xffffffffu, number, o);
+            mass += __shfl_xor_sync(0xffffffffu, mass, o);
+        }
+        if (c < n && (tid & (g - 1)) == 0) use(c, mine, number, mass);
+    };
+    // More: sorted, larger first(a, b) leading, then each thread's SR_EACH consecutive entries, with the mass before
+    // them.  use(entry, its place, the mass before it, its own).
+    auto sorted = [&](int n, auto larger, auto use) {
+        int p = 2;
+        while (p < n) p <<= 1;
+        for (int i = n + tid; i < p; i += SR_THREADS) S.list[i] = 0;
+        __syncthreads();
+        for (int k = 2; k <= p; k <<= 1)
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                for (int t = tid; t < p / 2; t += SR_THREADS) {
+                    const int i = 2 * t - (t & (j - 1)), o = i + j;
+                    const u64 a = S.list[i], b = S.list[o];
+                    if (larger(b, a) == ((i & k) == 0)) {
+                        S.list[i] = b;
+                        S.list[o] = a;
+                    }
+                }
+                __syncthreads();
+            }
+        u64 w[SR_EACH], sum = 0, all;
+#pragma unroll
+        for (int e = 0; e < SR_EACH; e++) {
+            const int i = tid * SR_EACH + e;
+            w[e] = i < n ? unit_of(value_of(S.list[i])) : 0;
+            sum += w[e];
+        }
+        u64 before = sr_scan(sum, S.red, &all);
+#pragma unroll
+        for (int e = 0; e < SR_EACH; e++) {
+            const int i = tid * SR_EACH + e;
+            if (i < n) use(S.list[i], i, before, w[e]);
+            before += w[e];
         }
     };
     // Where the cut falls in the list, with the mass and count above the list and the needed mass (its bounds lo, hi):
-    // S.cut and, of the list down to it, S.kept_mass.  False where lo and hi do not agree.
+    // S.cut, its place S.first_bin, and of the list down to it S.kept_mass.  False where lo and hi do not agree.
     auto find_cut = [&](int n, u64 m_above, unsigned c_above, u64 lo, u64 hi) {
         if (tid == 0) S.first_bin = S.last_bin = n - 1;
         __syncthreads();
-        int number_of[SR_EACH], k = 0;  // this thread's entries
-        u64 mass_of[SR_EACH], pair_of[SR_EACH];
+        int place[SR_EACH], k = 0;
+        u64 upto[SR_EACH], pair[SR_EACH];
 #pragma unroll
-        for (int e = 0; e < SR_EACH; e++) number_of[e] = -1;
-        ranked(n, [](u64 a, u64 b) { return a > b; }, [&](int c, u64 mine, int number, u64 mass) {
-            const u64 run = m_above + mass + S.wt[c];
+        for (int e = 0; e < SR_EACH; e++) place[e] = -1;
+        auto look = [&](u64 mine, int number, u64 mass, u64 w) {
+            const u64 run = m_above + mass + w;
             const bool full = rule.top_k && c_above + number + 1 >= (unsigned)rule.top_k;
             if (full || (has_p && run >= lo)) atomicMin(&S.first_bin, number);
             if (full || (has_p && run >= hi)) atomicMin(&S.last_bin, number);
 #pragma unroll
             for (int e = 0; e < SR_EACH; e++)
                 if (e == k) {
-                    number_of[e] = number;
-                    mass_of[e] = mass + S.wt[c];
-                    pair_of[e] = mine;
+                    place[e] = number;
+                    upto[e] = mass + w;
+                    pair[e] = mine;
                 }
             k++;
-        });
+        };
+        if (n <= SR_RANKED)
+            ranked(n, [](u64 a, u64 b) { return a > b; },
+                   [&](int c, u64 mine, int number, u64 mass) { look(mine, number, mass, S.wt[c]); });
+        else
+            sorted(n, [](u64 a, u64 b) { return a > b; }, look);
         __syncthreads();
         const int at = S.first_bin;
         if (at != S.last_bin) return false;
 #pragma unroll
         for (int e = 0; e < SR_EACH; e++)
-            if (number_of[e] == at) {
-                S.cut = pair_of[e];
-                S.kept_mass = mass_of[e];
+            if (place[e] == at) {
+                S.cut = pair[e];
+                S.kept_mass = upto[e];
             }
         __syncthreads();
         return true;
     };
 
     if (few) {
-        cl.sync();
+        csync();
         const int n = (int)min(lead->n_list, (unsigned)SR_LIST + 1);
         if (n <= SR_LIST) {
             // rank 0 goes on alone: nothing of the others is read after the barrier above, and a barrier that some
@@ -584,15 +658,21 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
             u64 target = (u64)(rule.u * (double)total);
             if (target >= total) target = total - 1;
             // mass before each kept entry in index order (the low halves hold ~index)
-            ranked(n, [&](u64 a, u64 b) { return a >= cut && (uint32_t)a > (uint32_t)b; },
-                   [&](int c, u64 mine, int, u64 mass) {
-                       if (mine >= cut && mass <= target && target < mass + S.wt[c]) {
-                           A.tokens[row] = (int)~(uint32_t)mine;
-                           if (A.probs)
-                               A.probs[row] = (float)(rule.weight(value_of(mine), mx, S.table) * SR_UNIT / (double)total);
-                       }
-                   });
-            cl.sync();  // the other ranks have read n_list before they left
+            auto draw = [&](u64 mine, int, u64 mass, u64 w) {
+                if (mass <= target && target < mass + w) {
+                    A.tokens[row] = (int)~(uint32_t)mine;
+                    if (A.probs)
+                        A.probs[row] = (float)(rule.weight(value_of(mine), mx, S.table) * SR_UNIT / (double)total);
+                }
+            };
+            if (n <= SR_RANKED)
+                ranked(n, [&](u64 a, u64 b) { return a >= cut && (uint32_t)a > (uint32_t)b; },
+                       [&](int c, u64 mine, int number, u64 mass) {
+                           if (mine >= cut) draw(mine, number, mass, S.wt[c]);
+                       });
+            else
+                sorted(S.first_bin + 1, [](u64 a, u64 b) { return (uint32_t)a > (uint32_t)b; }, draw);
+            csync();  // the other ranks have read n_list before they left
             return;
         }
     }
@@ -603,7 +683,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
     float xa = cuts ? INFINITY : xmin, xb = xmin;
     bool to_top = cuts;  // the range still reaches the maximum
     auto side = [&](float v) { return !to_top && v >= xa ? 1 : v >= xb ? 0 : -1; };
-    auto dist = [&](float v) { return v == mx ? 0.f : __fsub_rn(mx, v); };
+    auto dist = [&](float v) { return __fsub_rn(mx, v); };  // (NaN for an infinite maximum: bin 0)
     // kept mass of every warp's run, to rank 0
     auto push_run = [&](u64 m) {
 #pragma unroll
@@ -614,26 +694,22 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
     if (cuts) {
         // lowest survivor, and the approximate mass, as far as the first pass has not found them
         if (!online) {
-            float lw = INFINITY, mass = 0.f;
+            float mass = 0.f;
             stream([&](float (&v)[E], int) {
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const bool in = v[e] >= xmin;
-                    lw = in ? fminf(lw, v[e]) : lw;
                     const float p = rough(v[e]);
-                    mass += in ? p : 0.f;
+                    mass += v[e] >= xmin ? p : 0.f;
                 }
             });
-            lw = sr_reduce(lw, reinterpret_cast<float *>(S.red), minf);
             mass = sr_reduce(mass, reinterpret_cast<float *>(S.red), addf);
-            cl.sync();  // the earlier values have been read
-            push(&SrShared::min_of, lw);
+            csync();  // the earlier values have been read
             push(&SrShared::mass_of, mass);
-            S.cnt[0][tid] = 0;
-            cl.sync();
+            for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[0][i] = 0;
+            csync();
         } else if (by_topk) {
-            cl.sync();  // the counts have been read
-            S.cnt[0][tid] = 0;
+            csync();  // the counts have been read
+            for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[0][i] = 0;
             __syncthreads();
         }
         // a rank's approximate mass; its bins count it in units of 2^-30
@@ -641,15 +717,18 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
             const float m = S.mass_of[i];
             return online && m > 0.f ? __fmul_rn(m, rough(S.max_of[i])) : m;
         };
-        float lowest = INFINITY;
-        for (int i = 0; i < cs; i++) lowest = fminf(lowest, S.min_of[i]);
         if (!online) {
             m1 = 0.f;
             for (int i = 0; i < cs; i++) m1 += S.mass_of[i];
         }
         const float step = __fmul_rn(mass_at(rank), 0x1p-30f), per = step > 0.f ? __fdiv_rn(1.f, step) : 0.f;
-        // weights below 2^-43 share the last bin of the first round
-        float lo = 0.f, hi = fminf(dist(lowest), __fdiv_rn(30.f, rule.c * 0.6931472f));
+        // The first round's bins reach to weights of 2^-43; with top-p no further than the weights that, all vocab of
+        // them, would not make up what the cut leaves out.  The last bin holds the rest.
+        float lo = 0.f, hi = __fdiv_rn(30.f, rule.c * 0.6931472f);
+        if (has_p) {
+            const float left = __fdiv_rn((float)A.vocab, __fmul_rn(fmaxf((float)(1.0 - rule.top_p), 1e-7f), m1));
+            hi = fminf(hi, __fdiv_rn(fmaxf(__log2f(left), 0.f) + 0.5f, rule.c));
+        }
         float m_above = 0.f;
         for (int round = 0; round < SR_ROUNDS; round++) {
             const int buf = round & 1;
@@ -658,52 +737,84 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
             auto bin = [&](float v) {
                 return (int)fminf(fmaxf(__fmul_rn(__fsub_rn(dist(v), lo), inv), 0.f), (float)(SR_BINS - 1));
             };
+            unsigned n_last = 0;  // (the last bin is a crowded one: counted in registers)
+            float m_last = 0.f;
             stream([&](float (&v)[E], int) {
 #pragma unroll
                 for (int e = 0; e < E; e++) {
                     const int b = bin(v[e]);
-                    const uint32_t m = has_p ? __float2uint_rn(__fmul_rn(rough(v[e]), per)) : 0u;
-                    if (side(v[e]) == 0) {
+                    const float p = has_p ? rough(v[e]) : 0.f;
+                    const bool in = side(v[e]) == 0, last = in && b == SR_BINS - 1;
+                    n_last += last;
+                    m_last += last ? p : 0.f;
+                    if (in && !last) {
                         atomicAdd(&S.cnt[buf][b], 1u);
-                        if (m) atomicAdd(&S.mass[buf][b], m);
+                        if (has_p) atomicAdd(&S.mass[buf][b], __float2uint_rn(__fmul_rn(p, per)));
                     }
                 }
             });
-            cl.sync();
-            unsigned n = 0, n_low = 0, n_all;  // n_low: of the ranks before this one
-            float m = 0.f, m_all;
+            n_last = sr_reduce(n_last, reinterpret_cast<unsigned *>(S.red), [](unsigned a, unsigned b) { return a + b; });
+            m_last = sr_reduce(m_last, reinterpret_cast<float *>(S.red), addf);
+            if (tid == 0) {
+                S.cnt[buf][SR_BINS - 1] = n_last;
+                S.mass[buf][SR_BINS - 1] = __float2uint_rn(__fmul_rn(m_last, per));
+            }
+            csync();
+            // this thread's bins 2 tid, 2 tid + 1: counts of all ranks, and of the ranks before this one
+            unsigned n[2] = {0, 0}, n_low[2] = {0, 0}, n_all;
+            float m[2] = {0.f, 0.f}, m_all;
             for (int i = 0; i < cs; i++) {
                 const SrShared *o = cl.map_shared_rank(&S, i);
-                if (i == rank) n_low = n;
-                n += o->cnt[buf][tid];
-                if (has_p) m += __fmul_rn((float)o->mass[buf][tid], __fmul_rn(mass_at(i), 0x1p-30f));
+                const uint2 c2 = *reinterpret_cast<const uint2 *>(&o->cnt[buf][2 * tid]);
+                if (i == rank) {
+                    n_low[0] = n[0];
+                    n_low[1] = n[1];
+                }
+                n[0] += c2.x;
+                n[1] += c2.y;
+                if (has_p) {
+                    const uint2 m2 = *reinterpret_cast<const uint2 *>(&o->mass[buf][2 * tid]);
+                    const float unit = __fmul_rn(mass_at(i), 0x1p-30f);
+                    m[0] += __fmul_rn((float)m2.x, unit);
+                    m[1] += __fmul_rn((float)m2.y, unit);
+                }
             }
-            const unsigned nb = c_above + sr_scan(n, reinterpret_cast<unsigned *>(S.red), &n_all);
+            unsigned nb = c_above + sr_scan(n[0] + n[1], reinterpret_cast<unsigned *>(S.red), &n_all);
             __syncthreads();
-            const float mb = m_above + sr_scan(m, reinterpret_cast<float *>(S.red), &m_all);
-            // the cut is in the first bin that may complete top_k or top_p, or behind it up to the first that must
-            const float need = (float)rule.top_p * m1, slack = 2e-4f * m1;
-            const bool full = rule.top_k && nb + n >= (unsigned)rule.top_k;
-            const bool may = n && (full || (has_p && mb + m + slack >= need));
-            const bool must = n && (full || (has_p && mb + m - slack >= need));
+            float mb = m_above + sr_scan(m[0] + m[1], reinterpret_cast<float *>(S.red), &m_all);
             if (tid == 0) {
                 S.first_bin = S.last_bin = SR_BINS;
                 S.range_count = S.range_low = 0;
             }
             // (the buffer of the next round was read before this round's barrier)
-            S.cnt[buf ^ 1][tid] = S.mass[buf ^ 1][tid] = 0;
+            for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[buf ^ 1][i] = S.mass[buf ^ 1][i] = 0;
             __syncthreads();
-            if (may) atomicMin(&S.first_bin, tid);
-            if (must) atomicMin(&S.last_bin, tid);
+            // the cut is in the first bin that may complete top_k or top_p, or behind it up to the first that must
+            const float need = (float)rule.top_p * m1, slack = 2e-4f * m1;
+            unsigned nb_of[2];
+            float mb_of[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                nb_of[k] = nb;
+                mb_of[k] = mb;
+                nb += n[k];
+                mb += m[k];
+                const bool full = rule.top_k && nb >= (unsigned)rule.top_k;
+                if (n[k] && (full || (has_p && mb + slack >= need))) atomicMin(&S.first_bin, 2 * tid + k);
+                if (n[k] && (full || (has_p && mb - slack >= need))) atomicMin(&S.last_bin, 2 * tid + k);
+            }
             __syncthreads();
             const int fb = S.first_bin, lb = min(S.last_bin, SR_BINS - 1);
-            if (tid >= fb && tid <= lb) {
-                atomicAdd(&S.range_count, n);
-                atomicAdd(&S.range_low, n_low);
-            }
-            if (tid == fb) {
-                S.m_at = mb;
-                S.red[31] = nb;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                if (2 * tid + k >= fb && 2 * tid + k <= lb) {
+                    atomicAdd(&S.range_count, n[k]);
+                    atomicAdd(&S.range_low, n_low[k]);
+                }
+                if (2 * tid + k == fb) {
+                    S.m_at = mb_of[k];
+                    S.red[31] = nb_of[k];
+                }
             }
             // the bins' edges as keys (the lowest logit of a bin below fb, and of one up to lb): bins descend with the
             // logit, so 32 lanes close in on the first key that satisfies
@@ -737,7 +848,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
             if (in_range <= SR_LIST) break;
             // the next round divides these bins
             const float w1 = width * (1.f / (SR_BINS - 1));
-            hi = lb >= SR_BINS - 1 ? fmaxf(dist(lowest), hi) : lo + w1 * (lb + 1);
+            hi = lb >= SR_BINS - 1 ? fmaxf(__fsub_rn(mx, xb), hi) : lo + w1 * (lb + 1);
             lo = lo + w1 * fb;
         }
     }
@@ -750,21 +861,32 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         __syncthreads();
     }
     u64 kept = 0, m_all = 0;
-    stream([&](float (&v)[E], int i) {
+    {
+        double kept_d = 0.0, all_d = 0.0;
+        int n = 0;
+        stream([&](float (&v)[E], int i) {
+            if (++n > 256 / E) {  // (256 logits of at most 2^43 + 1 are exact in a double)
+                kept += (u64)kept_d;
+                m_all += (u64)all_d;
+                kept_d = all_d = 0.0;
+                n = 1;
+            }
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int s = side(v[e]);
-            u64 w = 0;
-            if (has_p || s > 0) w = unit_of(v[e]);
-            m_all += v[e] >= xmin ? w : 0;
-            kept += s > 0 ? w : 0;
-            if (s == 0 && listed) lead->list[at0 + atomicAdd(&S.n_list, 1u)] = sr_pair(v[e], i + e);
-        }
-    });
+            for (int e = 0; e < E; e++) {
+                const int s = side(v[e]);
+                const double w = has_p || s > 0 ? unit_d(v[e]) : 0.0;
+                if (v[e] >= xmin) all_d = __dadd_rn(all_d, w);
+                if (s > 0) kept_d = __dadd_rn(kept_d, w);
+                if (s == 0 && listed) lead->list[at0 + atomicAdd(&S.n_list, 1u)] = sr_pair(v[e], i + e);
+            }
+        });
+        kept += (u64)kept_d;
+        m_all += (u64)all_d;
+    }
     push_run(kept);
     m_all = sr_reduce(m_all, S.red, addu);
     if (tid == 0) lead->slot[1][rank] = m_all;
-    cl.sync();
+    csync();
     const bool bisect = in_range > SR_LIST;
     if (bisect) {
         // over (key, index) pairs: the largest pair whose upper set completes top_k or top_p
@@ -788,13 +910,13 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
             });
             m = sr_reduce(m, S.red, addu);
             n = sr_reduce(n, S.red, addu);
-            cl.sync();  // the slots of the last turn have been read
+            csync();  // the slots of the last turn have been read
             if (tid < cs) {
                 SrShared *o = cl.map_shared_rank(&S, tid);
                 o->slot[0][rank] = m;
                 o->slot[1][rank] = n;
             }
-            cl.sync();
+            csync();
             m = above;
             n = c_above;
             for (int i = 0; i < cs; i++) {
@@ -810,9 +932,9 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
             for (int e = 0; e < E; e++)
                 if (side(v[e]) == 0 && sr_pair(v[e], i + e) >= cut) kept += unit_of(v[e]);
         });
-        cl.sync();  // the runs' masses have been read
+        csync();  // the runs' masses have been read
         push_run(kept);
-        cl.sync();
+        csync();
     }
     if (rank != 0) return;
     // ---- rank 0 alone: the cut, the run that the draw falls into, the logit
@@ -826,7 +948,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         find_cut(n, above, c_above, need, need);
         cut = S.cut;
         for (int i = tid; i < n; i += SR_THREADS)
-            if (S.list[i] >= cut) atomicAdd(&S.seg[(int)~(uint32_t)S.list[i] / run], S.wt[i]);
+            if (S.list[i] >= cut) atomicAdd(&S.seg[(int)~(uint32_t)S.list[i] / run], unit_of(value_of(S.list[i])));
         __syncthreads();
     }
     const u64 mine = tid < cs * SR_WARPS ? S.seg[tid] : 0;
@@ -859,23 +981,22 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 4) k_sample_
         for (int i = p0; i < p1; i++) {
             const float v = sr_load(x, i);
             if (!stays(v, i)) continue;
-            const double w = rule.weight(v, mx, S.table);
-            upto += RowRule::units(w);
+            upto += unit_of(v);
             if (upto > target) {
                 A.tokens[row] = i;
-                if (A.probs) A.probs[row] = (float)(w * SR_UNIT / (double)total);
+                if (A.probs) A.probs[row] = (float)(rule.weight(v, mx, S.table) * SR_UNIT / (double)total);
                 break;
             }
         }
     }
 }
 
-// CTAs a row: as many as still find a place at once (four CTAs an SM), while
+// CTAs a row: as many as still find a place at once (three CTAs an SM), while
 // every lane keeps at least SR_AHEAD vectors.
 template <typename T> static void launch_sample_rows(fb_ctx *ctx, SampleRowsArgs A, int64_t rows) {
     constexpr int step = SR_THREADS * SR_E<T>;  // logits of one step of a CTA
     int cs = 1;
-    while (cs < SR_CLUSTER && rows * cs * 2 <= 4 * ctx->num_sms && A.vocab > cs * step * SR_AHEAD) cs *= 2;
+    while (cs < SR_CLUSTER && rows * cs * 2 <= 3 * ctx->num_sms && A.vocab > cs * step * SR_AHEAD) cs *= 2;
     A.steps = (A.vocab + cs * step - 1) / (cs * step);
     A.chunk = A.steps * step;
     // groups of SR_AHEAD vectors, longer ones where a thread would have more than SR_GROUPS of them
