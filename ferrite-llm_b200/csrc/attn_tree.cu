@@ -6,33 +6,41 @@
 // and the drafted tokens whose mask bit is set.
 //
 // The (drafted token, query head of the group) pairs of a sequence and kv head
-// are the rows of one matrix product: 128 rows a tile share every key and
-// value that is read.  A verified tree of 32 tokens with 4 heads a group needs
-// 128 multiplications a byte of cache, so up to one full tile the bound is HBM
-// (4 head_dim bytes a key and kv head), beyond it the tensor cores.
+// are the rows of one matrix product, up to 256 rows a group (two tiles of 128,
+// the MMA's M): they share every key and value that is read.  A verified tree of
+// 32 tokens with 4 heads a kv head needs 128 multiplications a byte of cache, so
+// up to one full tile the bound is HBM (4 head_dim bytes a key and kv head),
+// beyond it the tensor cores.
 //
-// Split: the (sequence, kv head, tile, 64-key block) units of a call are
-// counted on the device from the lengths and dealt to one CTA per SM in equal
-// contiguous shares, so unequal lengths and few sequences fill the machine
-// alike.  A (sequence, kv head, tile) group that one CTA holds whole is written
-// directly; the others leave (max, sum, o) partials, at most two a CTA, that a
-// second kernel joins in share order (no atomics: the same bits every time).
-// Calls of at most TR_WHOLE blocks a group deal whole groups and need no join.
+// Split: the (sequence, kv head, row group, 64-key block) units of a call (two
+// for a block that two tiles work on) are counted on the device from the lengths
+// and dealt to one CTA per SM in equal contiguous shares, so unequal lengths and
+// few sequences fill the machine alike.  A row group that one CTA holds whole is
+// written directly; the others leave (max, sum, o) partials, at most two a CTA,
+// that a second kernel joins in share order (no atomics: the same bits every
+// time).  Calls of at most TR_WHOLE blocks a group deal whole groups, unjoined.
 //
-// A CTA, 11 warps: 0..7 softmax (warp w: rows 32 (w % 4) .. + 31, keys 32 (w /
-// 4) .. + 31 of a block), 8 and 10 TMA copies of K and V pages, 9 issues
-// tcgen05.mma and owns the tensor memory.  The dim-major K pages and
-// token-major V pages land in shared memory as the MN-major operands of S = Q
-// K^T and O += P V.  S has two buffers, so the product of block j + 1 runs
-// under the softmax of block j.  The roles run on through the CTA's groups: the
-// next group's keys load and its queries are laid out while a group drains.
+// A CTA, 12 warps: two softmax groups of 4 warps (thread = row), 8 and 10 TMA
+// copies of K and V pages, 9 and 11 issue tcgen05.mma for a group each (9 owns the
+// tensor memory).  With
+// more than 128 rows each softmax group has a tile and both read the same keys;
+// otherwise they take the blocks of one tile in turn, each with its own running
+// maximum, sum and accumulator, merged at the end.  Either way one group's
+// products run under the other's exponentials, which no single chain of blocks
+// could hide.  The dim-major K pages and token-major V pages land in shared
+// memory as the MN-major operands of S = Q K^T and O += P V; the probabilities
+// replace the scores in tensor memory and are the A operand from there.  Scores
+// have two buffers a group.  The roles run on through the CTA's groups: the next
+// group's keys load while one drains.
 //
 // Precision: q is scaled by a power of two a row (to 2^13..2^14 at most) and
-// enters as fp16 high + low parts where it is f32 (f16 and bf16 queries fit
-// the high part); the probabilities are kept 2^7 above the running maximum's
-// unit (at most 2^15), so that high + low fp16 parts hold 22 bits down to 2^-21
-// of the largest; products and sums are f32.  The accumulator is rescaled only
-// when a row's maximum grows by more than 8 (log 2 units).
+// enters as fp16 high + low parts where it is f32 (f16 and bf16 queries fit the
+// high part); the probabilities are kept 2^7 above the running maximum's unit (at
+// most 2^15).  For f32 results they are fp16 high + low parts too, 22 bits down
+// to 2^-21 of the largest; for f16 and bf16 results the high part alone, whose
+// half step of 2^-12 averages out over the keys below the result's own rounding.
+// Products and sums are f32.  The accumulator is rescaled only when a row's
+// maximum grows by more than 8 (log 2 units).
 #include <math.h>
 
 #include "fb_internal.h"
@@ -51,9 +59,10 @@ struct TreeArgs {
     void *out;
     int batch, n_rows, max_new, n_heads, n_kv, max_pages, num_pages, max_seq;
     int group;      // query heads a kv head
+    uint64_t inv_group;  // ceil(2^32 / group)
     int split;      // 1: units are key blocks, 0: whole groups
     int ctas;       // CTAs of the attention kernel
-    int rows_cap;   // row capacity of a partial (multiple of 32, <= 128)
+    int rows_cap;   // row capacity of a partial (multiple of 32, <= 256)
     float *part;    // [2 ctas] partials of (head_dim + 2) rows_cap floats
     float scale;
     bool qvec, ovec;  // q / out rows start on 16 bytes
@@ -61,9 +70,10 @@ struct TreeArgs {
 };
 
 constexpr int TR_ROWS = 128;      // rows a tile (MMA M)
+constexpr int TR_PAIR = 256;      // rows a group: two tiles
 constexpr int TR_KB = 64;         // keys a block
-constexpr int TR_WHOLE = 2;
-constexpr int TR_THREADS = 352;
+constexpr int TR_WHOLE = 4;
+constexpr int TR_THREADS = 384;
 constexpr float TR_NONE = -1e30f;  // running maximum of a row that has seen nothing
 constexpr float TR_LIFT = 7.f;     // probabilities are kept 2^7 above the reference maximum
 
@@ -102,10 +112,11 @@ template <typename T> __device__ __forceinline__ void tr_store8(T *p, bool vec, 
     }
 }
 
-// One sequence of the batch: its new rows, key blocks, row tiles and groups
-// (kv head major, tile minor).  A sequence left out has no groups.
+// One sequence of the batch: its new rows, key blocks, row groups a kv head (the
+// last of `weight` units a block, the others of two).  A sequence left out has
+// none.
 struct TreeSeq {
-    int off, n, len, blocks, tiles, groups;
+    int off, n, len, blocks, pairs, weight;
     __device__ __forceinline__ bool load(const TreeArgs &A, int b) {
         off = A.offsets[b];
         n = A.offsets[b + 1] - off;
@@ -113,42 +124,65 @@ struct TreeSeq {
         const bool ok = off >= 0 && n >= 0 && n <= A.max_new && off <= A.n_rows - n && len >= n && len <= A.max_seq;
         if (!ok) n = len = 0;
         blocks = (len + TR_KB - 1) / TR_KB;
-        tiles = (n * A.group + TR_ROWS - 1) / TR_ROWS;
-        groups = tiles * A.n_kv;
+        const int rows = n * A.group;
+        pairs = (rows + TR_PAIR - 1) / TR_PAIR;
+        weight = rows - (pairs - 1) * TR_PAIR > TR_ROWS ? 2 : 1;
         return ok;
     }
-    __device__ __forceinline__ int per_group(const TreeArgs &A) const { return A.split ? blocks : 1; }
-    __device__ __forceinline__ int units(const TreeArgs &A) const { return groups * per_group(A); }
+    __device__ __forceinline__ int per(const TreeArgs &A) const { return A.split ? blocks : 1; }
+    __device__ __forceinline__ int head_units(const TreeArgs &A) const {
+        return pairs > 0 ? (2 * (pairs - 1) + weight) * per(A) : 0;
+    }
+    __device__ __forceinline__ int units(const TreeArgs &A) const { return head_units(A) * A.n_kv; }
 };
 
-// Units of the whole call (every lane of the warp gets the sum).
-__device__ __forceinline__ int tree_total(const TreeArgs &A, int lane, bool report) {
+// Units of the sequences from `from` on, this lane's part.
+__device__ __forceinline__ int tree_total(const TreeArgs &A, int lane, int from, bool report) {
     int total = 0;
-    for (int b = lane; b < A.batch; b += 32) {
+    for (int b = from + lane; b < A.batch; b += 32) {
         TreeSeq s;
         if (!s.load(A, b) && report) atomicOr(A.err, ERRBIT_BAD_POS);
         total += s.units(A);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     return total;
 }
-// A CTA's share; the join kernel derives the same one.
-__device__ __forceinline__ int tree_quota(const TreeArgs &A, int total) { return (total + A.ctas - 1) / A.ctas; }
+// A CTA's share; the join kernel derives the same one.  With split at least two
+// units, so that none lies inside a block of two.
+__device__ __forceinline__ int tree_quota(const TreeArgs &A, int total) {
+    return max(A.split ? 2 : 1, (total + A.ctas - 1) / A.ctas);
+}
 
-// The segments of a CTA's share [u0, u1): consecutive blocks of one group.
+// The segments of a CTA's share: consecutive blocks of one row group.  A block
+// (without split: a group) belongs to the share that holds its first unit.
 struct TreeWalk {
     TreeSeq s;
-    int b, g, blk0, blk1, left;
-    // warp-collective; u0 < u1 <= total
-    __device__ __forceinline__ void start(const TreeArgs &A, int u0, int u1, int lane) {
-        int base = 0;
+    int b, h, pair, blk0, blk1, left;
+    // warp-collective; this CTA's share.  False: it holds no block's first unit.
+    __device__ __forceinline__ bool start(const TreeArgs &A, int cta, int lane, bool report) {
+        int base = 0, mine = 0;
+        if (lane < A.batch) {  // (the first 32 sequences stay in the lanes' registers)
+            if (!s.load(A, lane) && report) atomicOr(A.err, ERRBIT_BAD_POS);
+            mine = s.units(A);
+        } else {
+            s = TreeSeq{};
+        }
+        const TreeSeq first = s;
+        int total = mine + tree_total(A, lane, 32, report);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        const int quota = tree_quota(A, total);
+        const int64_t u0l = (int64_t)quota * cta;
+        if (u0l >= total) return false;
+        const int u0 = (int)u0l;
+        left = min(total - u0, quota);
         b = 0;
         for (int b0 = 0; b0 < A.batch; b0 += 32) {
-            int mine = 0;
-            if (b0 + lane < A.batch) {
-                s.load(A, b0 + lane);
-                mine = s.units(A);
+            if (b0 > 0) {
+                mine = 0;
+                if (b0 + lane < A.batch) {
+                    s.load(A, b0 + lane);
+                    mine = s.units(A);
+                }
             }
             int incl = mine;
 #pragma unroll
@@ -165,34 +199,66 @@ struct TreeWalk {
             }
             base += __shfl_sync(0xffffffffu, incl, 31);
         }
-        s.load(A, b);
-        const int per = s.per_group(A), r = u0 - base;
-        g = r / per;
-        left = u1 - u0;
-        span(A, r % per);
+        if (b < 32) {
+            s.off = __shfl_sync(0xffffffffu, first.off, b);
+            s.n = __shfl_sync(0xffffffffu, first.n, b);
+            s.len = __shfl_sync(0xffffffffu, first.len, b);
+            s.blocks = __shfl_sync(0xffffffffu, first.blocks, b);
+            s.pairs = __shfl_sync(0xffffffffu, first.pairs, b);
+            s.weight = __shfl_sync(0xffffffffu, first.weight, b);
+        } else {
+            s.load(A, b);
+        }
+        const int per = s.per(A), hu = s.head_units(A);
+        int r = u0 - base;
+        h = r / hu;
+        r -= h * hu;
+        pair = min(r / (2 * per), s.pairs - 1);
+        r -= pair * 2 * per;
+        span(A, r);
+        return blk0 < blk1 || next(A);
     }
-    __device__ __forceinline__ void span(const TreeArgs &A, int first) {
-        blk0 = A.split ? first : 0;
-        blk1 = A.split ? min(s.blocks, blk0 + left) : s.blocks;
-        left -= A.split ? blk1 - blk0 : 1;
+    __device__ __forceinline__ int weight() const { return pair < s.pairs - 1 ? 2 : s.weight; }
+    __device__ __forceinline__ void span(const TreeArgs &A, int r) {
+        const int w = weight(), take = min(left, w * s.per(A) - r);
+        if (A.split) {
+            blk0 = (r + w - 1) / w;
+            blk1 = (r + take + w - 1) / w;
+        } else {
+            blk0 = r == 0 ? 0 : s.blocks;
+            blk1 = s.blocks;
+        }
+        left -= take;
     }
     __device__ __forceinline__ bool next(const TreeArgs &A) {
-        if (left <= 0) return false;
-        if (++g == s.groups) {
-            g = 0;
-            do {
-                if (++b >= A.batch) return false;
-                s.load(A, b);
-            } while (s.units(A) == 0);
-        }
-        span(A, 0);
+        do {
+            if (left <= 0) return false;
+            if (++pair == s.pairs) {
+                pair = 0;
+                if (++h == A.n_kv) {
+                    h = 0;
+                    do {
+                        if (++b >= A.batch) return false;
+                        s.load(A, b);
+                    } while (s.units(A) == 0);
+                }
+            }
+            span(A, 0);
+        } while (blk0 >= blk1);
         return true;
     }
-    __device__ __forceinline__ int head() const { return g / s.tiles; }
-    __device__ __forceinline__ int row0() const { return (g % s.tiles) * TR_ROWS; }
-    __device__ __forceinline__ int rows(const TreeArgs &A) const { return min(TR_ROWS, s.n * A.group - row0()); }
+    __device__ __forceinline__ int row0() const { return pair * TR_PAIR; }
+    __device__ __forceinline__ int rows(const TreeArgs &A) const { return min(TR_PAIR, s.n * A.group - row0()); }
+    __device__ __forceinline__ bool both() const { return weight() == 2; }  // two tiles
+    // blocks that softmax group g works on
+    __device__ __forceinline__ int jobs(int g) const { return both() ? blk1 - blk0 : (blk1 - blk0 + 1 - g) / 2; }
     __device__ __forceinline__ bool whole() const { return blk0 == 0 && blk1 == s.blocks; }
 };
+
+// A row's new row of its sequence: row / group (exact while row group < 2^32).
+__device__ __forceinline__ int tree_token(const TreeArgs &A, int row) {
+    return (int)(((uint64_t)(uint32_t)row * A.inv_group) >> 32);
+}
 
 // Which of the keys p0 .. p0 + 31 new row i of a sequence sees.
 __device__ __forceinline__ uint32_t tree_visible(const TreeArgs &A, const TreeSeq &s, int i, int p0) {
@@ -217,16 +283,43 @@ __device__ __forceinline__ uint32_t tree_visible(const TreeArgs &A, const TreeSe
 }
 
 template <typename T, int HD> struct TreeCfg {
-    static constexpr bool QLO = sizeof(T) == 4;  // f32 queries need a low part
-    static constexpr int ST = HD == 128 && QLO ? 3 : 4;  // K and V stages
+    static constexpr bool LO = sizeof(T) == 4;          // f32: q and the probabilities have low parts
+    static constexpr int ST = HD == 128 && LO ? 3 : 5;  // K and V stages
     static constexpr uint32_t Q_BYTES = TR_ROWS * HD * 2;
-    static constexpr uint32_t KV_BYTES = TR_KB * HD * 2;  // one block of K or V
-    static constexpr uint32_t P_BYTES = TR_ROWS * TR_KB * 2;
-    static constexpr size_t SMEM = 1024 + (QLO ? 2 : 1) * (size_t)Q_BYTES + 2 * ST * (size_t)KV_BYTES + 4 * (size_t)P_BYTES;
+    static constexpr uint32_t TILE_BYTES = (LO ? 2 : 1) * Q_BYTES;  // a tile's queries
+    static constexpr uint32_t KV_BYTES = TR_KB * HD * 2;            // one block of K or V
+    static constexpr size_t SMEM = 1024 + 2 * (size_t)TILE_BYTES + 2 * ST * (size_t)KV_BYTES;
     static_assert(SMEM + 2048 <= 227 * 1024, "tree attention stages must fit");
 };
-constexpr uint32_t TR_TMEM_COLS = 256;  // S buffers at columns 0 and 64, O at 128
-constexpr uint32_t TR_O_COL = 128;
+constexpr uint32_t TR_TMEM_COLS = 512;  // scores (group, buffer) at 128 g + 64 buffer, O of group g at 256 + HD g
+constexpr uint32_t TR_O_COL = 256;
+
+// Bounded wait (~1 s) for waits that are short in the steady state: polls without the suspension of
+// mbar_wait_bounded, which a satisfied wait pays for too.
+__device__ __forceinline__ bool tr_wait(uint64_t *bar, uint32_t parity) {
+    auto poll = [&]() {
+        uint32_t ok;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        return ok != 0;
+    };
+    for (int i = 0; i < 16; i++)
+        if (poll()) return true;
+    return mbar_wait_bounded(bar, parity);
+}
+
+// D += A B with A (fp16 pairs, K-major, a lane a row) in tensor memory.
+__device__ __forceinline__ void umma_f16_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc,
+                                              uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 
 template <typename T, int HD, int PAGE>
 __global__ void __launch_bounds__(TR_THREADS, 1)
@@ -237,45 +330,44 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     constexpr uint32_t IDESC_S = umma_idesc_f16(TR_ROWS, TR_KB, false, true);
     constexpr uint32_t IDESC_O = umma_idesc_f16(TR_ROWS, HD, false, true);
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], s_free[2], p_full[2], p_free[2],
-        q_full, o_free, fin, pair_bar[4];
+    __shared__ uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST];
+    __shared__ uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [group][buffer]
+    __shared__ uint64_t q_full, q_empty, o_free, fin[2], go, pair_bar[4];
     __shared__ uint32_t s_tmem;
-    __shared__ float s_l[2][TR_ROWS];
-    __shared__ uint8_t s_qe[2][TR_ROWS];  // exponent field of a row half's largest query value
+    __shared__ float2 s_ml[TR_ROWS];  // group 1's (max, sum) of one tile's rows
+    __shared__ uint8_t s_qe[2][TR_PAIR];  // [segment parity] exponent field of a row's largest query value
     __shared__ int s_abort_raw, s_odd_raw[2];
-    __shared__ uint8_t s_skip_raw[8];
+    __shared__ uint8_t s_skip_raw[16];
     volatile int &s_abort = s_abort_raw;
-    volatile int *s_odd = s_odd_raw;          // segment (+ 1) that met non-finite values of new rows
-    volatile uint8_t *s_skip = s_skip_raw;    // block: halves whose page id is outside the pool
+    volatile int *s_odd = s_odd_raw;        // segment (+ 1) that met non-finite values of new rows
+    volatile uint8_t *s_skip = s_skip_raw;  // block: halves whose page id is outside the pool
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch();
-    const int total = tree_total(A, lane, blockIdx.x == 0 && warp == 0);
-    const int quota = tree_quota(A, total);
-    const int64_t u0l = (int64_t)quota * blockIdx.x;
-    if (u0l >= total) return;
-    const int u0 = (int)u0l, u1 = min(total - u0, quota) + u0;
+    TreeWalk w;
+    if (!w.start(A, blockIdx.x, lane, blockIdx.x == 0 && warp == 0)) return;
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *sQ = sm;                                         // high parts, then low parts
-    uint8_t *sK = sQ + (C::QLO ? 2 : 1) * C::Q_BYTES;         // [stage]
-    uint8_t *sV = sK + ST * C::KV_BYTES;                      // [stage]: dims 0..63, then 64..127
-    uint8_t *sP = sV + ST * C::KV_BYTES;                      // [buffer][high, low]
+    uint8_t *sQ = sm;                      // [tile][high parts, low parts]
+    uint8_t *sK = sQ + 2 * C::TILE_BYTES;  // [stage]
+    uint8_t *sV = sK + ST * C::KV_BYTES;   // [stage]: dims 0..63, then 64..127
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; i++) {
             mbar_init(&k_full[i], 1);
-            mbar_init(&k_empty[i], 1);
+            mbar_init(&k_empty[i], 2);  // (both MMA warps)
             mbar_init(&v_full[i], 1);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&v_empty[i], 2);
         }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&s_free[i], 8);
-            mbar_init(&p_full[i], 8);
-            mbar_init(&p_free[i], 1);
+        for (int i = 0; i < 4; i++) {
+            mbar_init(&s_full[i >> 1][i & 1], 1);
+            mbar_init(&p_full[i >> 1][i & 1], 4);
+            mbar_init(&o_done[i >> 1][i & 1], 1);
+            mbar_init(&pair_bar[i], 32);
         }
         mbar_init(&q_full, 8);
+        mbar_init(&go, 8);
+        mbar_init(&q_empty, 2);
         mbar_init(&o_free, 8);
-        mbar_init(&fin, 1);
-        for (int i = 0; i < 4; i++) mbar_init(&pair_bar[i], 64);
+        mbar_init(&fin[0], 1);
+        mbar_init(&fin[1], 1);
         mbar_fence_init();
         s_abort = 0;
         s_odd[0] = s_odd[1] = 0;
@@ -286,8 +378,6 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    TreeWalk w;
-    w.start(A, u0, u1, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -301,7 +391,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         int c = 0;  // blocks issued
         bool ok = true;
         do {
-            const int h = w.head(), npg = (w.s.len + PAGE - 1) / PAGE;
+            const int npg = (w.s.len + PAGE - 1) / PAGE;
             const int32_t *bt = A.bt + (int64_t)w.b * A.max_pages;
             int ids = 0, ids0 = -32;  // this lane's id of page ids0 + lane
             for (int blk = w.blk0; ok && blk < w.blk1; blk++, c++) {
@@ -321,17 +411,19 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 }
                 const int st = c % ST;
                 if (lane == 0) {
-                    if (c >= ST) ok = mbar_wait_bounded(&empty[st], (uint32_t)((c / ST) - 1) & 1u);
+                    // (the first queries, two dependent steps from the first scores, are not queued behind the rings)
+                    if (c == 1) ok = tr_wait(&go, 0);
+                    if (c >= ST) ok = ok && tr_wait(&empty[st], (uint32_t)((c / ST) - 1) & 1u);
                     if (ok) {
                         uint8_t *dst = ring + st * C::KV_BYTES;
                         if (isk) {
-                            s_skip[c & 7] = (uint8_t)skip;
+                            s_skip[c & 15] = (uint8_t)skip;
                             if (skip) atomicOr(A.err, ERRBIT_BAD_PAGE);
                         }
                         mbar_expect_tx(&full[st], C::KV_BYTES);
 #pragma unroll
                         for (int i = 0; i < PPB; i++) {
-                            const int row = page[i] * A.n_kv + h;
+                            const int row = page[i] * A.n_kv + w.h;
                             if (isk) {
                                 tma_load_2d(dst + i * (HD * PAGE * 2), &kmap, 0, row * HD, &full[st]);
                             } else {
@@ -349,211 +441,249 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         if (lane == 0) {
             if (!ok) s_abort = 1;
             // copies in flight land before shared memory is released
-            for (int k = c > ST ? c - ST : 0; k < c; k++) mbar_wait_bounded(&full[k % ST], (uint32_t)(k / ST) & 1u);
+            for (int k = c > ST ? c - ST : 0; k < c; k++) tr_wait(&full[k % ST], (uint32_t)(k / ST) & 1u);
         }
-    } else if (warp == 9) {
-        // ---- MMA issue: S of the next block before O of this one, within a segment
+    } else if (warp == 9 || warp == 11) {
+        // ---- MMA issue for group g: its next scores before its products of this block.  (The tensor core runs one
+        // thread's products in order: a score buffer is rewritten after the product that read it.)
         if (lane == 0) {
-            const uint32_t aQ = smem_u32(sQ), aK = smem_u32(sK), aV = smem_u32(sV), aP = smem_u32(sP);
-            auto issue_s = [&](int c) -> bool {
-                const int st = c % ST, sb = c & 1;
-                if (!mbar_wait_bounded(&k_full[st], (uint32_t)(c / ST) & 1u)) return false;
-                if (c >= 2 && !mbar_wait_bounded(&s_free[sb], (uint32_t)((c >> 1) - 1) & 1u)) return false;
-                tc_fence_after();
-#pragma unroll
-                for (int ks = 0; ks < HD / 16; ks++) {  // 16 dims: 16 rows of the dim-major pages
-                    const uint32_t qo = (uint32_t)(ks >> 2) * (TR_ROWS * 128) + (uint32_t)(ks & 3) * 32;
-                    const uint32_t ka = aK + st * C::KV_BYTES + ks * 16 * (PAGE * 2);
-                    const uint64_t db = PAGE == 64 ? umma_desc_mn_sw128(ka, C::KV_BYTES, 1024)
-                                                   : umma_desc_mn_sw64(ka, HD * PAGE * 2, 512);
-                    umma_f16_desc(tmem + sb * TR_KB, umma_desc_sw128(aQ + qo), db, IDESC_S, ks > 0 ? 1u : 0u);
-                    if (C::QLO)
-                        umma_f16_desc(tmem + sb * TR_KB, umma_desc_sw128(aQ + C::Q_BYTES + qo), db, IDESC_S, 1u);
-                }
-                umma_commit(&s_full[sb]);
-                umma_commit(&k_empty[st]);
-                return true;
-            };
-            auto issue_o = [&](int c, bool first) -> bool {
-                const int st = c % ST, pb = c & 1;
-                if (!mbar_wait_bounded(&p_full[pb], (uint32_t)(c >> 1) & 1u)) return false;
-                if (!mbar_wait_bounded(&v_full[st], (uint32_t)(c / ST) & 1u)) return false;
-                tc_fence_after();
-                const uint32_t ph = aP + pb * 2 * C::P_BYTES, pl = ph + C::P_BYTES;
-#pragma unroll
-                for (int ks = 0; ks < TR_KB / 16; ks++) {  // 16 keys
-                    const uint64_t db = umma_desc_mn_sw128(aV + st * C::KV_BYTES + ks * 2048, TR_KB * 128, 1024);
-                    umma_f16_desc(tmem + TR_O_COL, umma_desc_sw128(ph + ks * 32), db, IDESC_O,
-                                  (!first || ks > 0) ? 1u : 0u);
-                    umma_f16_desc(tmem + TR_O_COL, umma_desc_sw128(pl + ks * 32), db, IDESC_O, 1u);
-                }
-                umma_commit(&v_empty[st]);
-                umma_commit(&p_free[pb]);
-                return true;
-            };
+            const int g = warp == 11;
+            // descriptors advance by adding to their address field (16-byte units)
+            const uint64_t dQ = umma_desc_sw128(smem_u32(sQ)), dV = umma_desc_mn_sw128(smem_u32(sV), TR_KB * 128, 1024);
+            const uint64_t dK = PAGE == 64 ? umma_desc_mn_sw128(smem_u32(sK), C::KV_BYTES, 1024)
+                                           : umma_desc_mn_sw64(smem_u32(sK), HD * PAGE * 2, 512);
+            const uint32_t t_s = tmem + 128 * g, t_o = tmem + TR_O_COL + HD * g;
+            int cb = 0, jb = 0, seg = 0;  // blocks and jobs of the segments before this one
             bool ok = true;
-            int c = 0, seg = 0;
             do {
-                ok = mbar_wait_bounded(&q_full, (uint32_t)seg & 1u) && issue_s(c);
-                for (int blk = w.blk0; ok && blk < w.blk1 && !s_abort; blk++, c++) {
-                    if (blk + 1 < w.blk1) ok = issue_s(c + 1);
-                    if (ok && blk == w.blk0 && seg > 0) ok = mbar_wait_bounded(&o_free, (uint32_t)(seg - 1) & 1u);
-                    if (ok) ok = issue_o(c, blk == w.blk0);
-                }
+                const bool both = w.both();
+                const int nj = w.jobs(g), step = both ? 1 : 2;
+                const uint64_t dq = dQ + (both ? g : 0) * (C::TILE_BYTES >> 4);
+                int ks_c = cb + (both ? 0 : g), kst = ks_c % ST, vst = kst;  // the next blocks' ring stages and phases
+                uint32_t kph = (uint32_t)(ks_c / ST) & 1u, vph = kph;
+                auto forward = [&](int &st, uint32_t &ph) {
+                    st += step;
+                    if (st >= ST) {
+                        st -= ST;
+                        ph ^= 1;
+                    }
+                };
+                // a stage is free once both groups are done with it, or with one tile the block's only one
+                auto release = [&](uint64_t *bar) {
+                    umma_commit(bar);
+                    if (!both) mbar_arrive(bar);
+                };
+                auto issue_s = [&](int k) -> bool {
+                    const int j = jb + k;
+                    const uint32_t d = t_s + TR_KB * (j & 1);
+                    const uint64_t kd = dK + kst * (C::KV_BYTES >> 4);
+                    if (!tr_wait(&k_full[kst], kph)) return false;
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ks++) {  // 16 dims: 16 rows of the dim-major pages
+                        const uint32_t qo = ((uint32_t)(ks >> 2) * (TR_ROWS * 128) + (uint32_t)(ks & 3) * 32) >> 4;
+                        const uint64_t db = kd + ks * (16 * PAGE * 2 >> 4);
+                        umma_f16_desc(d, dq + qo, db, IDESC_S, ks > 0 ? 1u : 0u);
+                        if (C::LO) umma_f16_desc(d, dq + (C::Q_BYTES >> 4) + qo, db, IDESC_S, 1u);
+                    }
+                    umma_commit(&s_full[g][j & 1]);
+                    release(&k_empty[kst]);
+                    forward(kst, kph);
+                    if (k + 1 == nj) umma_commit(&q_empty);
+                    return true;
+                };
+                auto issue_o = [&](int k) -> bool {
+                    const int j = jb + k;
+                    const uint32_t p = t_s + TR_KB * (j & 1);
+                    const uint64_t vd = dV + vst * (C::KV_BYTES >> 4);
+                    if (!tr_wait(&v_full[vst], vph)) return false;
+                    if (k == 0 && seg > 0 && !tr_wait(&o_free, (uint32_t)(seg - 1) & 1u)) return false;
+                    if (!tr_wait(&p_full[g][j & 1], (uint32_t)(j >> 1) & 1u)) return false;
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < TR_KB / 16; ks++) {  // 16 keys: 8 columns of fp16 pairs
+                        const uint64_t db = vd + ks * (2048 >> 4);
+                        umma_f16_tmem(t_o, p + 8 * ks, db, IDESC_O, (k > 0 || ks > 0) ? 1u : 0u);
+                        if (C::LO) umma_f16_tmem(t_o, p + 32 + 8 * ks, db, IDESC_O, 1u);
+                    }
+                    umma_commit(&o_done[g][j & 1]);
+                    release(&v_empty[vst]);
+                    forward(vst, vph);
+                    return true;
+                };
+                ok = tr_wait(&q_full, (uint32_t)seg & 1u);
+                if (ok && nj == 0) mbar_arrive(&q_empty);
+                if (ok && nj > 0) ok = issue_s(0);
+                for (int k = 0; ok && k < nj && !s_abort; k++) ok = (k + 1 >= nj || issue_s(k + 1)) && issue_o(k);
+                cb += w.blk1 - w.blk0;
+                jb += nj;
                 seg++;
             } while (ok && !s_abort && w.next(A));
             if (!ok) s_abort = 1;
-            umma_commit(&fin);  // every MMA issued has completed before TMEM is released
-            mbar_wait_bounded(&fin, 0);
+            umma_commit(&fin[g]);  // every MMA issued has completed before TMEM is released
+            mbar_wait_bounded(&fin[g], 0);
         }
     } else {
-        // ---- softmax: thread = row r (TMEM lane) x 32 key columns
+        // ---- softmax: group g, thread = row r of its tile (TMEM lane)
         constexpr unsigned FULL = 0xffffffffu;
-        const int qd = warp & 3, ch = warp >> 2, r = 32 * qd + lane;
+        const int qd = warp & 3, g = warp >> 2, r = 32 * qd + lane;
         const uint32_t lt = tmem + ((uint32_t)(32 * qd) << 16);
+        const uint32_t t_s = lt + 128 * g, t_o = lt + TR_O_COL + HD * g;
+        const float sign = A.scale < 0.f ? -1.f : 1.f;
         uint32_t npair = 0;  // uses of pair_bar[qd]
         bool ok = true;
-        float sl2 = 0.f;     // this row's score unit: scale log2(e) 2^e
-        int c = 0, seg = 0;
-        auto pair_sync = [&]() -> bool {
-            mbar_arrive(&pair_bar[qd]);
-            return mbar_wait_bounded(&pair_bar[qd], npair++ & 1u);
-        };
-        // this thread's half of row r of a group's queries, as fp16 parts scaled by 2^-e
-        auto load_q = [&](const TreeWalk &t) -> bool {
-            const int rows = t.rows(A);
-            if (rows > 32 * qd) {
-                const int rr = t.row0() + min(r, rows - 1);
-                const T *src = static_cast<const T *>(A.q) + (int64_t)(t.s.off + rr / A.group) * A.qt +
-                               (int64_t)(t.head() * A.group + rr % A.group) * HD + ch * (HD / 2);
-                float x[HD / 16][8], mx = 0.f;
+        int cb = 0, jb = 0, seg = 0;  // blocks and this group's jobs of the segments before
+        // The group's queries as fp16 parts scaled by 2^-e: HD / 8 lanes a row, the 8 warps share the rows.
+        auto load_q = [&](const TreeWalk &t, int sg) {
+            constexpr int LPR = HD / 8, RPI = 32 / LPR, NV = sizeof(T) / 2, AHEAD = 16 / NV;  // 64 registers in flight
+            const int rows = t.rows(A), each = (t.both() ? TR_PAIR : TR_ROWS) / 8, d = (lane % LPR) * 8;
+            for (int i0 = 0; i0 < each; i0 += RPI * AHEAD) {
+                uint4 raw[AHEAD][NV];
 #pragma unroll
-                for (int k = 0; k < HD / 16; k++) tr_load8(src + 8 * k, A.qvec, x[k]);
+                for (int k = 0; k < AHEAD; k++) {
+                    const int rr = warp * each + i0 + k * RPI + lane / LPR;
 #pragma unroll
-                for (int k = 0; k < HD / 16; k++)
+                    for (int i = 0; i < NV; i++) raw[k][i] = make_uint4(0, 0, 0, 0);
+                    if (i0 + k * RPI < each && rr < rows) {
+                        const int row = t.row0() + rr, tok = tree_token(A, row);
+                        const T *src = static_cast<const T *>(A.q) + (int64_t)(t.s.off + tok) * A.qt +
+                                       (int64_t)(t.h * A.group + row - tok * A.group) * HD + d;
+                        if (A.qvec) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[k][e]));
-                s_qe[ch][r] = (uint8_t)((__float_as_uint(mx) >> 23) & 255u);
-                if (!pair_sync()) return false;
-                // exponent that brings the row's largest value to 2^13..2^14 (0 and non-finite rows stay)
-                const int ex = max((int)s_qe[0][r], (int)s_qe[1][r]);
-                const int e = (ex == 0 || ex == 255) ? 0 : ex - 127 - 13;
-                // 2^-e in two factors: e reaches -139 and 114
-                const float d0 = __uint_as_float((uint32_t)(127 - e / 2) << 23);
-                const float d1 = __uint_as_float((uint32_t)(127 - (e - e / 2)) << 23);
-                const float u0f = __uint_as_float((uint32_t)(127 + e / 2) << 23);
-                const float u1f = __uint_as_float((uint32_t)(127 + (e - e / 2)) << 23);
-                sl2 = __fmul_rn(__fmul_rn(__fmul_rn(A.scale, 1.4426950408889634f), u0f), u1f);
+                            for (int i = 0; i < NV; i++) raw[k][i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
+                        } else {
+                            T *e = reinterpret_cast<T *>(raw[k]);
 #pragma unroll
-                for (int k = 0; k < HD / 16; k++) {
+                            for (int i = 0; i < 8; i++) e[i] = src[i];
+                        }
+                    }
+                }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[k][i] = __fmul_rn(__fmul_rn(x[k][i], d0), d1);
-                    const int cc = ch * (HD / 16) + k;
-                    const uint32_t off = (uint32_t)(cc >> 3) * (TR_ROWS * 128) + sw128_off(r, cc & 7);
+                for (int k = 0; k < AHEAD; k++) {
+                    if (i0 + k * RPI >= each) break;
+                    const int rr = warp * each + i0 + k * RPI + lane / LPR;
+                    float x[8], mx = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[e] = tr_f32(reinterpret_cast<const T *>(raw[k])[e]);
+                        mx = fmaxf(mx, fabsf(x[e]));
+                    }
+#pragma unroll
+                    for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
+                    // exponent that brings the row's largest value to 2^13..2^14 (0 and non-finite rows stay)
+                    const int ex = (int)((__float_as_uint(mx) >> 23) & 255u);
+                    const int e2 = (ex == 0 || ex == 255) ? 0 : ex - 127 - 13;
+                    // 2^-e in two factors: e reaches -139 and 114
+                    const float f0 = __fmul_rn(sign, __uint_as_float((uint32_t)(127 - e2 / 2) << 23));
+                    const float f1 = __uint_as_float((uint32_t)(127 - (e2 - e2 / 2)) << 23);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = __fmul_rn(__fmul_rn(x[e], f0), f1);
                     uint4 hi, lo;
-                    split8(x[k], hi, lo);
-                    *reinterpret_cast<uint4 *>(sQ + off) = hi;
-                    if (C::QLO) *reinterpret_cast<uint4 *>(sQ + C::Q_BYTES + off) = lo;
+                    split8(x, hi, lo);
+                    uint8_t *dst = sQ + (rr >> 7) * C::TILE_BYTES + (uint32_t)(d >> 6) * (TR_ROWS * 128) +
+                                   sw128_off(rr & 127, (d >> 3) & 7);
+                    *reinterpret_cast<uint4 *>(dst) = hi;
+                    if (C::LO) *reinterpret_cast<uint4 *>(dst + C::Q_BYTES) = lo;
+                    if (d == 0) s_qe[sg & 1][rr] = (uint8_t)ex;
                 }
-                fence_proxy_async_smem();  // the tensor core reads them through the async proxy
             }
+            fence_proxy_async_smem();  // the tensor core reads them through the async proxy
             __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full);
-            return true;
+            if (lane == 0) {
+                mbar_arrive(&q_full);
+                if (sg == 0) mbar_arrive(&go);
+            }
         };
-        ok = load_q(w);
-        bool more = ok;
+        load_q(w, 0);
+        bool more = true;
         while (more) {
-            const int rows = w.rows(A), pre = w.s.len - w.s.n;
-            const bool active = rows > 32 * qd;
-            const int rr = w.row0() + min(r, rows - 1), tok = rr / A.group;
+            const bool both = w.both();
+            const int nj = w.jobs(g), pre = w.s.len - w.s.n;
+            const int tile_rows = w.rows(A) - (both ? TR_ROWS * g : 0);  // of this group's tile
+            const bool active = tile_rows > 32 * qd;
+            const int row = w.row0() + (both ? TR_ROWS * g : 0) + min(r, tile_rows - 1), tok = tree_token(A, row);
+            if (!(ok = tr_wait(&q_full, (uint32_t)seg & 1u))) break;
+            // this row's score unit, |scale| log2(e) 2^e (not 0: masked scores stay -inf)
+            const int ex = s_qe[seg & 1][(both ? TR_ROWS * g : 0) + r];
+            const int e2 = (ex == 0 || ex == 255) ? 0 : ex - 127 - 13;
+            const float sl2 = fmaxf(__fmul_rn(__fmul_rn(__fmul_rn(fabsf(A.scale), 1.4426950408889634f),
+                                                        __uint_as_float((uint32_t)(127 + e2 / 2) << 23)),
+                                              __uint_as_float((uint32_t)(127 + (e2 - e2 / 2)) << 23)),
+                                    1e-37f);
             float m = TR_NONE, l = 0.f;
-            for (int blk = w.blk0; blk < w.blk1; blk++, c++) {
-                const int sb = c & 1, p0 = blk * TR_KB;
-                if (!(ok = mbar_wait_bounded(&s_full[sb], (uint32_t)(c >> 1) & 1u))) break;
+            for (int k = 0; k < nj; k++) {
+                const int j = jb + k, blk = w.blk0 + (both ? k : 2 * k + g), c = cb + (blk - w.blk0), p0 = blk * TR_KB;
+                const uint32_t t_b = t_s + TR_KB * (j & 1);
+                if (!(ok = tr_wait(&s_full[g][j & 1], (uint32_t)(j >> 1) & 1u))) break;
+                if (j >= 2 && !(ok = tr_wait(&o_done[g][j & 1], (uint32_t)((j >> 1) - 1) & 1u))) break;
                 tc_fence_after();
-                const int skip = s_skip[c & 7];
-                float x[32];
-                float bm = TR_NONE;
+                const int skip = s_skip[c & 15];
                 if (active) {
-                    // row maximum of the other half's columns, then this warp's own
-                    const bool all = p0 + TR_KB <= pre && !skip;
-                    const uint32_t vis = all ? FULL : (skip >> ch) & 1 ? 0u : tree_visible(A, w.s, tok, p0 + 32 * ch);
-                    const uint32_t viso =
-                        all ? FULL : (skip >> (ch ^ 1)) & 1 ? 0u : tree_visible(A, w.s, tok, p0 + 32 * (ch ^ 1));
-                    uint32_t sv[32];
-                    tmem_ld32(lt + sb * TR_KB + 32 * (ch ^ 1), sv);
-                    if (all) {
+                    uint32_t sv[64];
+                    tmem_ld64(t_b, sv);
+                    if (p0 + TR_KB > pre || skip) {
+                        const uint32_t v0 = skip & 1 ? 0u : tree_visible(A, w.s, tok, p0);
+                        const uint32_t v1 = skip & 2 ? 0u : tree_visible(A, w.s, tok, p0 + 32);
 #pragma unroll
-                        for (int t = 0; t < 32; t++) bm = fmaxf(bm, __fmul_rn(__uint_as_float(sv[t]), sl2));
-                    } else {
-#pragma unroll
-                        for (int t = 0; t < 32; t++)
-                            bm = fmaxf(bm, (viso >> t) & 1 ? __fmul_rn(__uint_as_float(sv[t]), sl2) : -INFINITY);
+                        for (int t = 0; t < 32; t++) {
+                            if (!((v0 >> t) & 1)) sv[t] = 0xff800000u;  // -inf
+                            if (!((v1 >> t) & 1)) sv[32 + t] = 0xff800000u;
+                        }
                     }
-                    tmem_ld32(lt + sb * TR_KB + 32 * ch, sv);
+                    float b4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int t = 0; t < 32; t++) {
-                        x[t] = __fmul_rn(__uint_as_float(sv[t]), sl2);
-                        if (!all && !((vis >> t) & 1)) x[t] = -INFINITY;
-                        bm = fmaxf(bm, x[t]);
-                    }
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s_free[sb]);  // the MMA of block c + 2 may overwrite it
-                if (active) {
-                    const float mn = fmaxf(m, bm);
-                    const bool need = blk > w.blk0 && mn > m + 8.f;
+                    for (int t = 0; t < 64; t++) b4[t & 3] = fmaxf(b4[t & 3], __uint_as_float(sv[t]));
+                    const float bm = fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
+                    const float mn = fmaxf(m, __fmul_rn(bm, sl2));
+                    const bool need = k > 0 && mn > m + 8.f;
                     if (__any_sync(FULL, need)) {
-                        // rescale this warp's half of the accumulator rows once O of block c - 1 has landed
-                        if (!(ok = mbar_wait_bounded(&p_free[sb ^ 1], (uint32_t)((c - 1) >> 1) & 1u))) break;
+                        // rescale the accumulator rows once the product of this group's last block has landed
+                        if (!(ok = tr_wait(&o_done[g][(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u))) break;
                         tc_fence_after();
                         const float al = need ? exp2_approx(__fsub_rn(m, mn)) : 1.f;
 #pragma unroll 1
-                        for (int k = 0; k < HD / 64; k++) {
+                        for (int i = 0; i < HD / 32; i++) {
                             uint32_t ov[32];
-                            tmem_ld32(lt + TR_O_COL + (HD / 2) * ch + 32 * k, ov);
+                            tmem_ld32(t_o + 32 * i, ov);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) ov[i] = __float_as_uint(__fmul_rn(__uint_as_float(ov[i]), al));
-                            tmem_st32(lt + TR_O_COL + (HD / 2) * ch + 32 * k, ov);
+                            for (int e = 0; e < 32; e++) ov[e] = __float_as_uint(__fmul_rn(__uint_as_float(ov[e]), al));
+                            tmem_st32(t_o + 32 * i, ov);
                         }
-                        tc_fence_before();
                         if (need) {
                             l = __fmul_rn(l, al);
                             m = mn;
                         }
                     }
-                    if (blk == w.blk0) m = mn;
-                }
-                if (c >= 2 && !(ok = mbar_wait_bounded(&p_free[sb], (uint32_t)((c >> 1) - 1) & 1u))) break;
-                if (active) {
-                    // p = 2^(x - m + 7), as fp16 high / low A operands
-                    const float ref = __fsub_rn(m, TR_LIFT);
-                    uint8_t *ph = sP + sb * 2 * C::P_BYTES, *pl = ph + C::P_BYTES;
-                    float ls = 0.f;
+                    if (k == 0) m = mn;
+                    // p = 2^(s sl2 - m + 7): fp16 pairs over the scores, low parts behind the high ones
+                    const float ref = __fsub_rn(TR_LIFT, m);
+                    float l4[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t hi[32], lo[32];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        float p[8];
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            p[e] = exp2_approx(__fsub_rn(x[8 * k + e], ref));
-                            ls = __fadd_rn(ls, p[e]);
+                    for (int t = 0; t < 32; t++) {
+                        const float pa = exp2_approx(__fmaf_rn(__uint_as_float(sv[2 * t]), sl2, ref));
+                        const float pb = exp2_approx(__fmaf_rn(__uint_as_float(sv[2 * t + 1]), sl2, ref));
+                        l4[t & 3] = __fadd_rn(l4[t & 3], __fadd_rn(pa, pb));
+                        const __half2 h2 = __floats2half2_rn(pa, pb);
+                        hi[t] = *reinterpret_cast<const uint32_t *>(&h2);
+                        if (C::LO) {
+                            const float2 hf = __half22float2(h2);
+                            const __half2 q2 = __floats2half2_rn(__fsub_rn(pa, hf.x), __fsub_rn(pb, hf.y));
+                            lo[t] = *reinterpret_cast<const uint32_t *>(&q2);
                         }
-                        uint4 hi, lo;
-                        split8(p, hi, lo);
-                        *reinterpret_cast<uint4 *>(ph + sw128_off(r, 4 * ch + k)) = hi;
-                        *reinterpret_cast<uint4 *>(pl + sw128_off(r, 4 * ch + k)) = lo;
                     }
-                    l = __fadd_rn(l, ls);
+                    l = __fadd_rn(l, __fadd_rn(__fadd_rn(l4[0], l4[1]), __fadd_rn(l4[2], l4[3])));
+                    tmem_st32(t_b, hi);
+                    if (C::LO) tmem_st32(t_b + 32, lo);
                 }
                 if (p0 + TR_KB > pre || skip) {
                     // Values that some row must not see: 0 * NaN would reach it.  Behind the last key and in
                     // skipped pages all are zeroed; at new rows the non-finite ones, which the rows that see
-                    // them get back at the end (s_odd).
+                    // them get back at the end (s_odd).  (With two tiles both groups do it, each before its own
+                    // product: they write the same values, and the flag before them.)
                     const int st = c % ST;
-                    if (!(ok = mbar_wait_bounded(&v_full[st], (uint32_t)(c / ST) & 1u))) break;
-                    for (int i = threadIdx.x; i < (int)C::KV_BYTES / 16; i += 256) {
+                    if (!(ok = tr_wait(&v_full[st], (uint32_t)(c / ST) & 1u))) break;
+                    for (int i = threadIdx.x & 127; i < (int)C::KV_BYTES / 16; i += 128) {
                         const int t = (i >> 3) & 63;
                         uint4 *cell = reinterpret_cast<uint4 *>(sV + st * C::KV_BYTES) + i;
                         if (p0 + t >= w.s.len || ((skip >> (t >> 5)) & 1)) {
@@ -563,69 +693,99 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                             uint32_t *e = reinterpret_cast<uint32_t *>(&v);
                             bool odd = false;
 #pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                if ((e[k] & 0x7C00u) == 0x7C00u) {
-                                    e[k] &= 0xffff0000u;
+                            for (int i4 = 0; i4 < 4; i4++) {
+                                if ((e[i4] & 0x7C00u) == 0x7C00u) {
+                                    e[i4] &= 0xffff0000u;
                                     odd = true;
                                 }
-                                if ((e[k] & 0x7C000000u) == 0x7C000000u) {
-                                    e[k] &= 0xffffu;
+                                if ((e[i4] & 0x7C000000u) == 0x7C000000u) {
+                                    e[i4] &= 0xffffu;
                                     odd = true;
                                 }
                             }
                             if (odd) {
-                                *cell = v;
                                 s_odd[seg & 1] = seg + 1;
+                                __threadfence_block();
+                                *cell = v;
                             }
                         }
                     }
+                    fence_proxy_async_smem();
                 }
-                fence_proxy_async_smem();
+                tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[sb]);
+                if (lane == 0) mbar_arrive(&p_full[g][j & 1]);
             }
             if (!ok) break;
-            // the next group's queries go in while this group's last product runs
+            // the next group's queries go in once this one's last scores are out
             TreeWalk nw = w;
             more = nw.next(A);
-            if (more && !(ok = load_q(nw))) break;
-            // ---- this segment's rows, once its last product has landed
-            if (!(ok = mbar_wait_bounded(&p_free[(c - 1) & 1], (uint32_t)((c - 1) >> 1) & 1u))) break;
+            if (more) {
+                if (!(ok = tr_wait(&q_empty, (uint32_t)seg & 1u))) break;
+                load_q(nw, seg + 1);
+            }
+            // ---- this segment's rows, once the last products have landed
+            if (nj > 0) {
+                const int j = jb + nj - 1;
+                if (!(ok = tr_wait(&o_done[g][j & 1], (uint32_t)(j >> 1) & 1u))) break;
+            }
+            // One tile: group 0 takes over group 1's part (if that had a block) and writes the rows.
+            const bool two = !both && w.jobs(1) > 0;
+            float w0 = 1.f, w1 = 0.f;
+            if (two) {
+                if (g == 1) {
+                    s_ml[r] = make_float2(m, l);
+                    tc_fence_before();
+                    mbar_arrive(&pair_bar[qd]);
+                } else {
+                    if (!(ok = tr_wait(&pair_bar[qd], npair & 1u))) break;
+                    const float2 o = s_ml[r];
+                    const float mm = fmaxf(m, o.x);
+                    w0 = exp2f(__fsub_rn(m, mm));
+                    w1 = exp2f(__fsub_rn(o.x, mm));
+                    m = mm;
+                    l = __fmaf_rn(w0, l, __fmul_rn(w1, o.y));
+                }
+                npair++;
+            }
             tc_fence_after();
-            if (active) {
-                s_l[ch][r] = l;
-                if (!(ok = pair_sync())) break;
-                l = __fadd_rn(s_l[0][r], s_l[1][r]);
-                const bool odd = s_odd[seg & 1] == seg + 1;
-                const bool whole = !A.split || w.whole();
+            if (active && (both || g == 0)) {
+                const bool odd = s_odd[seg & 1] == seg + 1, whole = !A.split || w.whole();
                 const float inv = l > 0.f ? __fdiv_rn(1.f, l) : 0.f;
-                float *part = A.part + (int64_t)(2 * blockIdx.x + (seg > 0)) * (HD + 2) * A.rows_cap;
-                const int h = w.head();
+                const int pr = (both ? TR_ROWS * g : 0) + r;  // row of the partial
+                float *part = A.part + (int64_t)(2 * blockIdx.x + (w.blk0 == 0)) * (HD + 2) * A.rows_cap;
                 T *orow = static_cast<T *>(A.out) + (int64_t)(w.s.off + tok) * A.ot +
-                          (int64_t)(h * A.group + rr % A.group) * HD;
+                          (int64_t)(w.h * A.group + row - tok * A.group) * HD;
 #pragma unroll 1
-                for (int k = 0; k < HD / 64; k++) {
+                for (int d0 = 0; d0 < HD; d0 += 32) {
                     uint32_t ov[32];
-                    const int d0 = (HD / 2) * ch + 32 * k;
-                    tmem_ld32(lt + TR_O_COL + d0, ov);
-                    if (odd) {
-                        for (int j = max(0, w.blk0 * TR_KB - pre); j < min(w.s.n, w.blk1 * TR_KB - pre); j++) {
-                            const int p = pre + j, page = A.bt[(int64_t)w.b * A.max_pages + p / PAGE];
-                            if (page < 0 || page >= A.num_pages || !(tree_visible(A, w.s, tok, p) & 1)) continue;
-                            const __half *v = A.vpool + (((int64_t)page * A.n_kv + h) * PAGE + p % PAGE) * HD + d0;
+                    tmem_ld32(t_o + d0, ov);
+                    if (two) {
+                        uint32_t o1[32];
+                        tmem_ld32(t_o + HD + d0, o1);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) {
-                                const float x = __half2float(v[i]);
-                                if (!isfinite(x)) ov[i] = __float_as_uint(__fadd_rn(__uint_as_float(ov[i]), x));
+                        for (int i = 0; i < 32; i++)
+                            ov[i] = __float_as_uint(
+                                __fmaf_rn(w1, __uint_as_float(o1[i]), __fmul_rn(w0, __uint_as_float(ov[i]))));
+                    }
+                    if (odd) {
+                        for (int i = max(0, w.blk0 * TR_KB - pre); i < min(w.s.n, w.blk1 * TR_KB - pre); i++) {
+                            const int p = pre + i, page = A.bt[(int64_t)w.b * A.max_pages + p / PAGE];
+                            if (page < 0 || page >= A.num_pages || !(tree_visible(A, w.s, tok, p) & 1)) continue;
+                            const __half *v = A.vpool + (((int64_t)page * A.n_kv + w.h) * PAGE + p % PAGE) * HD + d0;
+#pragma unroll
+                            for (int e = 0; e < 32; e++) {
+                                const float x = __half2float(v[e]);
+                                if (!isfinite(x)) ov[e] = __float_as_uint(__fadd_rn(__uint_as_float(ov[e]), x));
                             }
                         }
                     }
                     if (!whole) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)  // [dim / 4][row]: a warp stores 512 bytes at once
-                            reinterpret_cast<uint4 *>(part)[(int64_t)((d0 + i) >> 2) * A.rows_cap + r] =
+                            reinterpret_cast<uint4 *>(part)[(int64_t)((d0 + i) >> 2) * A.rows_cap + pr] =
                                 make_uint4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
-                    } else if (r < rows) {
+                    } else if (r < tile_rows) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {
                             float y[8];
@@ -635,12 +795,14 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                         }
                     }
                 }
-                if (!whole && ch == 0)
-                    reinterpret_cast<float2 *>(part + (int64_t)HD * A.rows_cap)[r] = make_float2(m, l);
+                if (!whole)
+                    reinterpret_cast<float2 *>(part + (int64_t)HD * A.rows_cap)[pr] = make_float2(m, l);
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&o_free);
+            cb += w.blk1 - w.blk0;
+            jb += nj;
             w = nw;
             seg++;
         }
@@ -656,18 +818,18 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     }
 }
 
-// Joins the partials of the groups that several CTAs hold.  grid (row tiles a
-// sequence x rows_cap / 32 x dim quarters, n_kv, batch): lane = row, warp =
-// HD / 64 four-dim columns.
+// Joins the partials of the row groups that several CTAs hold.  grid (row groups a
+// kv head x rows_cap / 32 x dim quarters, n_kv, batch): lane = row, warp = HD / 64
+// four-dim columns.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ TreeArgs A) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int quarter = blockIdx.x & 3, rest = blockIdx.x >> 2;
-    const int slabs = A.rows_cap / 32, slab = rest % slabs, tile = rest / slabs;
+    const int slabs = A.rows_cap / 32, slab = rest % slabs, pair = rest / slabs;
     const int b = blockIdx.z;
     TreeSeq s;
     s.load(A, b);
-    const int row0 = tile * TR_ROWS + 32 * slab;
+    const int row0 = pair * TR_PAIR + 32 * slab;
     if (row0 >= s.n * A.group) return;
     // units before this sequence, and in all
     int before = 0, total = 0;
@@ -684,13 +846,14 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
         before += __shfl_xor_sync(0xffffffffu, before, o);
     }
     const int quota = tree_quota(A, total);
-    const int gs = before + (blockIdx.y * s.tiles + tile) * s.blocks, ge = gs + s.blocks;  // the group's units
-    const int c0 = gs / quota, c1 = (ge - 1) / quota;
+    const int wt = pair < s.pairs - 1 ? 2 : s.weight;
+    const int gs = before + blockIdx.y * s.head_units(A) + pair * 2 * s.blocks;  // the group's first unit
+    const int c0 = gs / quota, c1 = (gs + wt * (s.blocks - 1)) / quota;          // CTAs of its first and last block
     if (c0 == c1) return;  // written by its CTA
     const int r = 32 * slab + lane;
     const int64_t slot = (int64_t)(HD + 2) * A.rows_cap;
-    // a CTA's first segment is its partial 0: every one but the first CTA's starts with this group
-    auto part = [&](int c) { return A.part + (2 * (int64_t)c + (c * (int64_t)quota < gs)) * slot; };
+    // the CTA with the group's first block keeps it as its partial 1, the others as their 0
+    auto part = [&](int c) { return A.part + (2 * (int64_t)c + (c == c0)) * slot; };
     pdl_wait();
     float M = TR_NONE;
     for (int c = c0; c <= c1; c++) M = fmaxf(M, reinterpret_cast<const float2 *>(part(c) + (int64_t)HD * A.rows_cap)[r].x);
@@ -718,8 +881,9 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
     const int rr = row0 + lane;
     if (rr >= s.n * A.group) return;
     const float inv = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
-    T *out = static_cast<T *>(A.out) + (int64_t)(s.off + rr / A.group) * A.ot +
-             (int64_t)(blockIdx.y * A.group + rr % A.group) * HD + 4 * col0;
+    const int tok = tree_token(A, rr);
+    T *out = static_cast<T *>(A.out) + (int64_t)(s.off + tok) * A.ot +
+             (int64_t)(blockIdx.y * A.group + rr - tok * A.group) * HD + 4 * col0;
 #pragma unroll
     for (int k = 0; k < N; k++) {
         tr_put(out + 4 * k, __fmul_rn(o[k].x, inv));
@@ -731,21 +895,22 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
 
 // What a call of these sizes launches.
 struct TreePlan {
-    int split, ctas, rows_cap, tiles;
+    int split, ctas, rows_cap, pairs;
     int64_t ws;
 };
 static TreePlan tree_plan(const fb_ctx *ctx, int batch, int max_new, int n_heads, int n_kv, int head_dim,
                           int max_seq_len) {
     TreePlan p{};
     const int64_t rows = (int64_t)max_new * (n_heads / n_kv);
-    const int64_t tiles = (rows + TR_ROWS - 1) / TR_ROWS, blocks = (max_seq_len + TR_KB - 1) / TR_KB;
-    const int64_t groups = tiles * n_kv * batch;
-    FB_REQUIRE(groups * blocks < ((int64_t)1 << 31) - 4096 && tiles <= 65535, "attn_tree: batch too large");
+    const int64_t pairs = (rows + TR_PAIR - 1) / TR_PAIR, blocks = (max_seq_len + TR_KB - 1) / TR_KB;
+    const int64_t groups = pairs * n_kv * batch;
+    FB_REQUIRE(2 * groups * blocks < ((int64_t)1 << 31) - 4096 && pairs <= 65535, "attn_tree: batch too large");
+    FB_REQUIRE((rows + TR_PAIR) * (n_heads / n_kv) < ((int64_t)1 << 32), "attn_tree: too many rows");
     p.split = blocks > TR_WHOLE;
-    const int64_t units = p.split ? groups * blocks : groups;
+    const int64_t units = 2 * groups * (p.split ? blocks : 1);
     p.ctas = (int)(units < ctx->num_sms ? units : ctx->num_sms);
-    p.tiles = (int)tiles;
-    p.rows_cap = (int)(rows >= TR_ROWS ? TR_ROWS : (rows + 31) / 32 * 32);
+    p.pairs = (int)pairs;
+    p.rows_cap = (int)(rows >= TR_PAIR ? TR_PAIR : (rows + 31) / 32 * 32);
     p.ws = p.split ? (int64_t)2 * p.ctas * (head_dim + 2) * p.rows_cap * 4 : 0;
     return p;
 }
@@ -763,7 +928,7 @@ static void launch_tree(fb_ctx *ctx, const TreeArgs &A, const TreePlan &plan, co
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = ctx->pdl ? 1 : 0;
-    cfg.gridDim = dim3((unsigned)(plan.tiles * (plan.rows_cap / 32) * 4), (unsigned)A.n_kv, (unsigned)A.batch);
+    cfg.gridDim = dim3((unsigned)(plan.pairs * (plan.rows_cap / 32) * 4), (unsigned)A.n_kv, (unsigned)A.batch);
     cfg.blockDim = dim3(128);
     cfg.stream = ctx->stream;
     cfg.attrs = attr;
@@ -853,6 +1018,7 @@ int fb_attn_tree(fb_ctx *ctx, int dtype, const void *q_dev, int64_t q_token_stri
                    "attn_tree: the workspace must be 16-byte aligned and hold fb_attn_tree_workspace bytes (" +
                        std::to_string(plan.ws) + ")");
         A.group = n_heads / n_kv_heads;
+        A.inv_group = (((uint64_t)1 << 32) + A.group - 1) / A.group;
         A.split = plan.split;
         A.ctas = plan.ctas;
         A.rows_cap = plan.rows_cap;
