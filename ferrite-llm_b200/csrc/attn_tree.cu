@@ -43,6 +43,8 @@
 // maximum grows by more than 8 (log 2 units).
 #include <math.h>
 
+#include <type_traits>
+
 #include "fb_internal.h"
 #include "kq_common.cuh"
 #include "tc_common.cuh"
@@ -562,28 +564,34 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 for (int k = 0; k < AHEAD; k++) {
                     if (i0 + k * RPI >= each) break;
                     const int rr = warp * each + i0 + k * RPI + lane / LPR;
-                    float x[8], mx = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        x[e] = tr_f32(reinterpret_cast<const T *>(raw[k])[e]);
-                        mx = fmaxf(mx, fabsf(x[e]));
-                    }
-#pragma unroll
-                    for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
-                    // exponent that brings the row's largest value to 2^13..2^14 (0 and non-finite rows stay)
-                    const int ex = (int)((__float_as_uint(mx) >> 23) & 255u);
-                    const int e2 = (ex == 0 || ex == 255) ? 0 : ex - 127 - 13;
-                    // 2^-e in two factors: e reaches -139 and 114
-                    const float f0 = __fmul_rn(sign, __uint_as_float((uint32_t)(127 - e2 / 2) << 23));
-                    const float f1 = __uint_as_float((uint32_t)(127 - (e2 - e2 / 2)) << 23);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = __fmul_rn(__fmul_rn(x[e], f0), f1);
                     uint4 hi, lo;
-                    split8(x, hi, lo);
+                    int ex = 0;  // (f16 queries enter as they are)
+                    if constexpr (std::is_same<T, __half>::value) {
+                        const uint32_t flip = A.scale < 0.f ? 0x80008000u : 0u;
+                        hi = make_uint4(raw[k][0].x ^ flip, raw[k][0].y ^ flip, raw[k][0].z ^ flip, raw[k][0].w ^ flip);
+                    } else {
+                        float x[8], mx = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            x[e] = tr_f32(reinterpret_cast<const T *>(raw[k])[e]);
+                            mx = fmaxf(mx, fabsf(x[e]));
+                        }
+#pragma unroll
+                        for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
+                        // exponent that brings the row's largest value to 2^13..2^14 (0 and non-finite rows stay)
+                        ex = (int)((__float_as_uint(mx) >> 23) & 255u);
+                        const int e2 = (ex == 0 || ex == 255) ? 0 : ex - 127 - 13;
+                        // 2^-e in two factors: e reaches -139 and 114
+                        const float f0 = __fmul_rn(sign, __uint_as_float((uint32_t)(127 - e2 / 2) << 23));
+                        const float f1 = __uint_as_float((uint32_t)(127 - (e2 - e2 / 2)) << 23);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] = __fmul_rn(__fmul_rn(x[e], f0), f1);
+                        split8(x, hi, lo);
+                    }
                     uint8_t *dst = sQ + (rr >> 7) * C::TILE_BYTES + (uint32_t)(d >> 6) * (TR_ROWS * 128) +
                                    sw128_off(rr & 127, (d >> 3) & 7);
                     *reinterpret_cast<uint4 *>(dst) = hi;
-                    if (C::LO) *reinterpret_cast<uint4 *>(dst + C::Q_BYTES) = lo;
+                    if constexpr (C::LO) *reinterpret_cast<uint4 *>(dst + C::Q_BYTES) = lo;
                     if (d == 0) s_qe[sg & 1][rr] = (uint8_t)ex;
                 }
             }
@@ -594,14 +602,111 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 if (sg == 0) mbar_arrive(&go);
             }
         };
-        load_q(w, 0);
-        bool more = true;
-        while (more) {
+        // A pass: the next segment's queries go in once this one's last scores are out, then this one's rows are
+        // written, then the next one's blocks.
+        TreeWalk nw = w;
+        bool first = true, more = true, active = false;
+        int nj = 0, tile_rows = 0, row = 0, tok = 0;
+        float m = TR_NONE, l = 0.f;
+        for (;;) {
+            if (more) {
+                if (!first && !(ok = tr_wait(&q_empty, (uint32_t)seg & 1u))) break;
+                load_q(nw, first ? 0 : seg + 1);
+            }
+            if (!first) {
+                const bool both = w.both();
+                const int pre = w.s.len - w.s.n;
+                // ---- this segment's rows, once the last products have landed
+                if (nj > 0) {
+                    const int j = jb + nj - 1;
+                    if (!(ok = tr_wait(&o_done[g][j & 1], (uint32_t)(j >> 1) & 1u))) break;
+                }
+                // One tile: group 0 takes over group 1's part (if that had a block) and writes the rows.
+                const bool two = !both && w.jobs(1) > 0;
+                float w0 = 1.f, w1 = 0.f;
+                if (two) {
+                    if (g == 1) {
+                        s_ml[r] = make_float2(m, l);
+                        tc_fence_before();
+                        mbar_arrive(&pair_bar[qd]);
+                    } else {
+                        if (!(ok = tr_wait(&pair_bar[qd], npair & 1u))) break;
+                        const float2 o = s_ml[r];
+                        const float mm = fmaxf(m, o.x);
+                        w0 = exp2f(__fsub_rn(m, mm));
+                        w1 = exp2f(__fsub_rn(o.x, mm));
+                        m = mm;
+                        l = __fmaf_rn(w0, l, __fmul_rn(w1, o.y));
+                    }
+                    npair++;
+                }
+                tc_fence_after();
+                if (active && (both || g == 0)) {
+                    const bool odd = s_odd[seg & 1] == seg + 1, whole = !A.split || w.whole();
+                    const float inv = l > 0.f ? __fdiv_rn(1.f, l) : 0.f;
+                    const int pr = (both ? TR_ROWS * g : 0) + r;  // row of the partial
+                    float *part = A.part + (int64_t)(2 * blockIdx.x + (w.blk0 == 0)) * (HD + 2) * A.rows_cap;
+                    T *orow = static_cast<T *>(A.out) + (int64_t)(w.s.off + tok) * A.ot +
+                              (int64_t)(w.h * A.group + row - tok * A.group) * HD;
+#pragma unroll 1
+                    for (int d0 = 0; d0 < HD; d0 += 32) {
+                        uint32_t ov[32];
+                        tmem_ld32(t_o + d0, ov);
+                        if (two) {
+                            uint32_t o1[32];
+                            tmem_ld32(t_o + HD + d0, o1);
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                ov[i] = __float_as_uint(
+                                    __fmaf_rn(w1, __uint_as_float(o1[i]), __fmul_rn(w0, __uint_as_float(ov[i]))));
+                        }
+                        if (odd) {
+                            for (int i = max(0, w.blk0 * TR_KB - pre); i < min(w.s.n, w.blk1 * TR_KB - pre); i++) {
+                                const int p = pre + i, page = A.bt[(int64_t)w.b * A.max_pages + p / PAGE];
+                                if (page < 0 || page >= A.num_pages || !(tree_visible(A, w.s, tok, p) & 1)) continue;
+                                const __half *v = A.vpool + (((int64_t)page * A.n_kv + w.h) * PAGE + p % PAGE) * HD + d0;
+#pragma unroll
+                                for (int e = 0; e < 32; e++) {
+                                    const float x = __half2float(v[e]);
+                                    if (!isfinite(x)) ov[e] = __float_as_uint(__fadd_rn(__uint_as_float(ov[e]), x));
+                                }
+                            }
+                        }
+                        if (!whole) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4)  // [dim / 4][row]: a warp stores 512 bytes at once
+                                reinterpret_cast<uint4 *>(part)[(int64_t)((d0 + i) >> 2) * A.rows_cap + pr] =
+                                    make_uint4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
+                        } else if (r < tile_rows) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                float y[8];
+#pragma unroll
+                                for (int e = 0; e < 8; e++) y[e] = __fmul_rn(__uint_as_float(ov[i + e]), inv);
+                                tr_store8(orow + d0 + i, A.ovec, y);
+                            }
+                        }
+                    }
+                    if (!whole)
+                        reinterpret_cast<float2 *>(part + (int64_t)HD * A.rows_cap)[pr] = make_float2(m, l);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&o_free);
+                cb += w.blk1 - w.blk0;
+                jb += nj;
+                seg++;
+            }
+            if (!more) break;
+            first = false;
+            w = nw;
             const bool both = w.both();
-            const int nj = w.jobs(g), pre = w.s.len - w.s.n;
-            const int tile_rows = w.rows(A) - (both ? TR_ROWS * g : 0);  // of this group's tile
-            const bool active = tile_rows > 32 * qd;
-            const int row = w.row0() + (both ? TR_ROWS * g : 0) + min(r, tile_rows - 1), tok = tree_token(A, row);
+            const int pre = w.s.len - w.s.n;
+            nj = w.jobs(g);
+            tile_rows = w.rows(A) - (both ? TR_ROWS * g : 0);  // of this group's tile
+            active = tile_rows > 32 * qd;
+            row = w.row0() + (both ? TR_ROWS * g : 0) + min(r, tile_rows - 1);
+            tok = tree_token(A, row);
             if (!(ok = tr_wait(&q_full, (uint32_t)seg & 1u))) break;
             // this row's score unit, |scale| log2(e) 2^e (not 0: masked scores stay -inf)
             const int ex = s_qe[seg & 1][(both ? TR_ROWS * g : 0) + r];
@@ -610,12 +715,14 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                                                         __uint_as_float((uint32_t)(127 + e2 / 2) << 23)),
                                               __uint_as_float((uint32_t)(127 + (e2 - e2 / 2)) << 23)),
                                     1e-37f);
-            float m = TR_NONE, l = 0.f;
+            m = TR_NONE;
+            l = 0.f;
             for (int k = 0; k < nj; k++) {
                 const int j = jb + k, blk = w.blk0 + (both ? k : 2 * k + g), c = cb + (blk - w.blk0), p0 = blk * TR_KB;
                 const uint32_t t_b = t_s + TR_KB * (j & 1);
+                // (these scores were issued behind the group's product of job j - 2: that one has landed too, so of
+                // the o_done phases only those of j - 1 and j can be open below)
                 if (!(ok = tr_wait(&s_full[g][j & 1], (uint32_t)(j >> 1) & 1u))) break;
-                if (j >= 2 && !(ok = tr_wait(&o_done[g][j & 1], (uint32_t)((j >> 1) - 1) & 1u))) break;
                 tc_fence_after();
                 const int skip = s_skip[c & 15];
                 if (active) {
@@ -717,94 +824,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 if (lane == 0) mbar_arrive(&p_full[g][j & 1]);
             }
             if (!ok) break;
-            // the next group's queries go in once this one's last scores are out
-            TreeWalk nw = w;
             more = nw.next(A);
-            if (more) {
-                if (!(ok = tr_wait(&q_empty, (uint32_t)seg & 1u))) break;
-                load_q(nw, seg + 1);
-            }
-            // ---- this segment's rows, once the last products have landed
-            if (nj > 0) {
-                const int j = jb + nj - 1;
-                if (!(ok = tr_wait(&o_done[g][j & 1], (uint32_t)(j >> 1) & 1u))) break;
-            }
-            // One tile: group 0 takes over group 1's part (if that had a block) and writes the rows.
-            const bool two = !both && w.jobs(1) > 0;
-            float w0 = 1.f, w1 = 0.f;
-            if (two) {
-                if (g == 1) {
-                    s_ml[r] = make_float2(m, l);
-                    tc_fence_before();
-                    mbar_arrive(&pair_bar[qd]);
-                } else {
-                    if (!(ok = tr_wait(&pair_bar[qd], npair & 1u))) break;
-                    const float2 o = s_ml[r];
-                    const float mm = fmaxf(m, o.x);
-                    w0 = exp2f(__fsub_rn(m, mm));
-                    w1 = exp2f(__fsub_rn(o.x, mm));
-                    m = mm;
-                    l = __fmaf_rn(w0, l, __fmul_rn(w1, o.y));
-                }
-                npair++;
-            }
-            tc_fence_after();
-            if (active && (both || g == 0)) {
-                const bool odd = s_odd[seg & 1] == seg + 1, whole = !A.split || w.whole();
-                const float inv = l > 0.f ? __fdiv_rn(1.f, l) : 0.f;
-                const int pr = (both ? TR_ROWS * g : 0) + r;  // row of the partial
-                float *part = A.part + (int64_t)(2 * blockIdx.x + (w.blk0 == 0)) * (HD + 2) * A.rows_cap;
-                T *orow = static_cast<T *>(A.out) + (int64_t)(w.s.off + tok) * A.ot +
-                          (int64_t)(w.h * A.group + row - tok * A.group) * HD;
-#pragma unroll 1
-                for (int d0 = 0; d0 < HD; d0 += 32) {
-                    uint32_t ov[32];
-                    tmem_ld32(t_o + d0, ov);
-                    if (two) {
-                        uint32_t o1[32];
-                        tmem_ld32(t_o + HD + d0, o1);
-#pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            ov[i] = __float_as_uint(
-                                __fmaf_rn(w1, __uint_as_float(o1[i]), __fmul_rn(w0, __uint_as_float(ov[i]))));
-                    }
-                    if (odd) {
-                        for (int i = max(0, w.blk0 * TR_KB - pre); i < min(w.s.n, w.blk1 * TR_KB - pre); i++) {
-                            const int p = pre + i, page = A.bt[(int64_t)w.b * A.max_pages + p / PAGE];
-                            if (page < 0 || page >= A.num_pages || !(tree_visible(A, w.s, tok, p) & 1)) continue;
-                            const __half *v = A.vpool + (((int64_t)page * A.n_kv + w.h) * PAGE + p % PAGE) * HD + d0;
-#pragma unroll
-                            for (int e = 0; e < 32; e++) {
-                                const float x = __half2float(v[e]);
-                                if (!isfinite(x)) ov[e] = __float_as_uint(__fadd_rn(__uint_as_float(ov[e]), x));
-                            }
-                        }
-                    }
-                    if (!whole) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4)  // [dim / 4][row]: a warp stores 512 bytes at once
-                            reinterpret_cast<uint4 *>(part)[(int64_t)((d0 + i) >> 2) * A.rows_cap + pr] =
-                                make_uint4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
-                    } else if (r < tile_rows) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            float y[8];
-#pragma unroll
-                            for (int e = 0; e < 8; e++) y[e] = __fmul_rn(__uint_as_float(ov[i + e]), inv);
-                            tr_store8(orow + d0 + i, A.ovec, y);
-                        }
-                    }
-                }
-                if (!whole)
-                    reinterpret_cast<float2 *>(part + (int64_t)HD * A.rows_cap)[pr] = make_float2(m, l);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&o_free);
-            cb += w.blk1 - w.blk0;
-            jb += nj;
-            w = nw;
-            seg++;
         }
         if (!ok) s_abort = 1;
     }
@@ -854,28 +874,42 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
     const int64_t slot = (int64_t)(HD + 2) * A.rows_cap;
     // the CTA with the group's first block keeps it as its partial 1, the others as their 0
     auto part = [&](int c) { return A.part + (2 * (int64_t)c + (c == c0)) * slot; };
+    // the parts' (max, sum) of the slab's rows, all loads in flight together
+    extern __shared__ float2 s_part[];  // [part][row]
     pdl_wait();
+    const int parts = c1 - c0 + 1;
+    for (int i = threadIdx.x; i < parts * 32; i += 128)
+        s_part[i] = reinterpret_cast<const float2 *>(part(c0 + i / 32) + (int64_t)HD * A.rows_cap)[32 * slab + (i & 31)];
+    __syncthreads();
     float M = TR_NONE;
-    for (int c = c0; c <= c1; c++) M = fmaxf(M, reinterpret_cast<const float2 *>(part(c) + (int64_t)HD * A.rows_cap)[r].x);
+    for (int c = 0; c < parts; c++) M = fmaxf(M, s_part[32 * c + lane].x);
     float L = 0.f;
     constexpr int N = HD / 64;  // float4 columns a thread
     float4 o[N];
 #pragma unroll
     for (int k = 0; k < N; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
     const int col0 = quarter * (HD / 16) + warp * N;
-#pragma unroll 4
-    for (int c = c0; c <= c1; c++) {
-        const float *p = part(c);
-        const float2 ml = reinterpret_cast<const float2 *>(p + (int64_t)HD * A.rows_cap)[r];
-        const float wgt = exp2f(__fsub_rn(ml.x, M));
-        L = __fmaf_rn(wgt, ml.y, L);
+    for (int c = 0; c < parts; c += 8) {
+        float4 v[8][N];
 #pragma unroll
-        for (int k = 0; k < N; k++) {
-            const float4 v = reinterpret_cast<const float4 *>(p)[(int64_t)(col0 + k) * A.rows_cap + r];
-            o[k].x = __fmaf_rn(wgt, v.x, o[k].x);
-            o[k].y = __fmaf_rn(wgt, v.y, o[k].y);
-            o[k].z = __fmaf_rn(wgt, v.z, o[k].z);
-            o[k].w = __fmaf_rn(wgt, v.w, o[k].w);
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (c + i < parts)
+                    v[i][k] = reinterpret_cast<const float4 *>(part(c0 + c + i))[(int64_t)(col0 + k) * A.rows_cap + r];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (c + i >= parts) break;
+            const float2 ml = s_part[32 * (c + i) + lane];
+            const float wgt = exp2f(__fsub_rn(ml.x, M));
+            L = __fmaf_rn(wgt, ml.y, L);
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                o[k].x = __fmaf_rn(wgt, v[i][k].x, o[k].x);
+                o[k].y = __fmaf_rn(wgt, v[i][k].y, o[k].y);
+                o[k].z = __fmaf_rn(wgt, v[i][k].z, o[k].z);
+                o[k].w = __fmaf_rn(wgt, v[i][k].w, o[k].w);
+            }
         }
     }
     const int rr = row0 + lane;
@@ -930,6 +964,7 @@ static void launch_tree(fb_ctx *ctx, const TreeArgs &A, const TreePlan &plan, co
     attr[0].val.programmaticStreamSerializationAllowed = ctx->pdl ? 1 : 0;
     cfg.gridDim = dim3((unsigned)(plan.pairs * (plan.rows_cap / 32) * 4), (unsigned)A.n_kv, (unsigned)A.batch);
     cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = (size_t)plan.ctas * 32 * sizeof(float2);  // (a group has at most one part a CTA)
     cfg.stream = ctx->stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
