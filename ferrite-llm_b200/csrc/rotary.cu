@@ -249,32 +249,161 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// grid (pages a sequence's new rows can touch, kv head groups, batch): a block
-// writes the new rows that fall into one page, for heads_per_block heads.
-// K is staged as f32 rows in shared memory and leaves transposed (the pages
-// are dim-major): 8 lanes write the 128 bytes of a dimension's 64 tokens.
-template <typename T, int HD>
-__global__ void __launch_bounds__(KVA_THREADS)
-    k_kv_append(const __grid_constant__ RotaryParams P, const __grid_constant__ AppendArgs A) {
-    extern __shared__ float kva_smem[];
-    constexpr int PITCH = HD + 1;
-    float *rows = kva_smem;                                             // [page][PITCH]
-    float2 *trig = reinterpret_cast<float2 *>(kva_smem + A.page * PITCH + (A.page * PITCH & 1));  // [page][half + 1]
+// The part of a sequence's new rows that falls into this block's page: cache
+// positions from .. to - 1, the page's id, the first row.  False: nothing to do.
+__device__ __forceinline__ bool append_span(const AppendArgs &A, int &from, int &to, int &phys, int &row0) {
     const int b = blockIdx.z;
     const int off = A.offsets[b], n = A.offsets[b + 1] - off, len = A.lens[b];
     if (off < 0 || n < 0 || n > A.max_new || off > A.n_rows - n || len < n || len > A.max_pages * A.page) {
         if (threadIdx.x == 0) atomicOr(A.err, ERRBIT_BAD_POS);
-        return;
+        return false;
     }
     const int p0 = len - n, pg = p0 / A.page + blockIdx.x;
-    const int from = max(p0, pg * A.page), to = min(len, (pg + 1) * A.page);
-    if (from >= to) return;
-    const int phys = A.bt[(int64_t)b * A.max_pages + pg];
+    from = max(p0, pg * A.page);
+    to = min(len, (pg + 1) * A.page);
+    if (from >= to) return false;
+    phys = A.bt[(int64_t)b * A.max_pages + pg];
     if (phys < 0 || phys >= A.num_pages) {
         if (threadIdx.x == 0) atomicOr(A.err, ERRBIT_BAD_PAGE);
-        return;
+        return false;
     }
-    const int cnt = to - from, t0 = from - pg * A.page, row0 = off + from - p0;
+    row0 = off + from - p0;
+    return true;
+}
+
+// Eight values of a row as they are stored.
+template <typename T> struct Raw8 {
+    uint4 q[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) q[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = to_f32(reinterpret_cast<const T *>(q)[i]);
+    }
+};
+
+// grid (pages a sequence's new rows can touch, kv head groups, batch): a block
+// writes the new rows that fall into one page, for up to KVA_HEADS heads.  A warp
+// takes 8 rows x 4 units (8 dimensions, in mode 1 with the 8 they are paired
+// with): the angles of a unit are computed once and serve all heads; the rotated
+// keys go as fp16 into a [dim][token] tile whose 16-byte token chunks are
+// exchanged by the dimension's chunk (both the scattered 2-byte stores and the
+// rows' 16-byte loads then touch every bank once).  The pages are dim-major: 8
+// lanes write the 128 bytes of a dimension's 64 tokens.
+constexpr int KVA_HEADS = 4;
+template <typename T, int HD, int PAGE, int MODE>
+__global__ void __launch_bounds__(KVA_THREADS)
+    k_kv_append(const __grid_constant__ RotaryParams P, const __grid_constant__ AppendArgs A) {
+    extern __shared__ __align__(16) uint8_t kva_tile[];  // [head][HD][PAGE] fp16
+    constexpr int CH = PAGE / 8;
+    int from, to, phys, row0;
+    if (!append_span(A, from, to, phys, row0)) return;
+    const int cnt = to - from, t0 = from % PAGE;
+    const int h0 = blockIdx.y * A.heads_per_block, nh = min(A.heads_per_block, A.n_kv - h0);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const T *kr = static_cast<const T *>(A.k) + (int64_t)row0 * A.kt + (int64_t)h0 * HD;
+    const T *vr = static_cast<const T *>(A.v) + (int64_t)row0 * A.vt + (int64_t)h0 * HD;
+    __half *kp = A.kpool + ((int64_t)phys * A.n_kv + h0) * HD * PAGE;
+    __half *vp = A.vpool + ((int64_t)phys * A.n_kv + h0) * HD * PAGE + (int64_t)t0 * HD;
+    const int half = P.rot / 2;
+    // units of a row: mode 1 rot / 16 pairs of chunks and the chunks behind them, mode 0 all chunks
+    const int paired = MODE == 1 ? P.rot / 16 : 0, nu = paired + (MODE == 1 ? (HD - P.rot) / 8 : HD / 8);
+    const int ug = (nu + 3) / 4, tg = (cnt + 7) / 8;
+    auto put = [&](int h, int c, int t, const float (&v)[8]) {  // chunk c of head h, token t of the page
+        __half *tile = reinterpret_cast<__half *>(kva_tile) + h * HD * PAGE;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int d = 8 * c + i;
+            tile[d * PAGE + (((t >> 3) ^ (c & (CH - 1))) << 3) + (t & 7)] = __float2half_rn(v[i]);
+        }
+    };
+    for (int wt = warp; wt < ug * tg; wt += KVA_THREADS / 32) {
+        const int u = (wt % ug) * 4 + (lane & 3), t = (wt / ug) * 8 + (lane >> 2);
+        if (u >= nu || t >= cnt) continue;
+        const bool pair = u < paired;
+        const int c = MODE == 1 ? (pair ? u : 2 * paired + (u - paired)) : u;  // the unit's (first) chunk
+        const int c2 = c + (MODE == 1 ? half / 8 : 0);
+        const bool turn = MODE == 1 ? pair : 8 * c < P.rot;
+        const T *src = kr + t * A.kt;
+        constexpr int AH = 2;  // heads in flight
+        Raw8<T> a[AH], b[AH];
+        auto fetch = [&](int h) {
+#pragma unroll
+            for (int k = 0; k < AH; k++)
+                if (h + k < nh) {
+                    a[k].load(src + (h + k) * HD + 8 * c);
+                    if (MODE == 1 && pair) b[k].load(src + (h + k) * HD + 8 * c2);
+                }
+        };
+        fetch(0);
+        constexpr int NP = MODE == 1 ? 8 : 4;
+        float2 cs[NP];
+        if (turn) {
+            const int pos = A.positions ? A.positions[row0 + t] : from + t;
+#pragma unroll
+            for (int i = 0; i < NP; i++) cs[i] = rotary_trig(P, MODE == 1 ? 8 * c + i : 4 * c + i, pos);
+        }
+        for (int h = 0; h < nh; h += AH) {
+            if (h > 0) fetch(h);
+#pragma unroll
+            for (int k = 0; k < AH; k++) {
+                if (h + k >= nh) break;
+                float x[8], y[8];
+                a[k].get(x);
+                if (MODE == 1 && pair) b[k].get(y);
+                if (turn) {
+#pragma unroll
+                    for (int i = 0; i < NP; i++) {
+                        float &p0 = MODE == 1 ? x[i] : x[(2 * i) & 7], &p1 = MODE == 1 ? y[i] : x[(2 * i + 1) & 7];
+                        const float x0 = p0, x1 = p1;
+                        p0 = __fsub_rn(__fmul_rn(x0, cs[i].x), __fmul_rn(x1, cs[i].y));
+                        p1 = __fadd_rn(__fmul_rn(x0, cs[i].y), __fmul_rn(x1, cs[i].x));
+                    }
+                }
+                put(h + k, c, t0 + t, x);
+                if (MODE == 1 && pair) put(h + k, c2, t0 + t, y);
+            }
+        }
+    }
+    // V rows, as they come
+    for (int e = threadIdx.x; e < cnt * nh * (HD / 8); e += KVA_THREADS) {
+        const int c = e % (HD / 8), q = e / (HD / 8), h = q % nh, t = q / nh;
+        Raw8<T> raw;
+        raw.load(vr + t * A.vt + h * HD + 8 * c);
+        float v[8];
+        raw.get(v);
+        *reinterpret_cast<uint4 *>(vp + (int64_t)h * HD * PAGE + t * HD + 8 * c) = pack8(v);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < nh * HD * CH; e += KVA_THREADS) {
+        const int c = e % CH, d = e / CH;  // (heads follow one another in the tile and in the page)
+        if (8 * c + 8 <= t0 || 8 * c >= t0 + cnt) continue;
+        const __half *src = reinterpret_cast<const __half *>(kva_tile) + d * PAGE + ((c ^ ((d >> 3) & (CH - 1))) << 3);
+        __half *dst = kp + (int64_t)d * PAGE + 8 * c;
+        if (8 * c >= t0 && 8 * c + 8 <= t0 + cnt) {
+            *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (8 * c + j >= t0 && 8 * c + j < t0 + cnt) dst[j] = src[j];
+        }
+    }
+}
+
+// The general form: any rot_dim, any alignment.  K is staged as f32 rows in shared
+// memory and rotated on its way out.
+template <typename T, int HD>
+__global__ void __launch_bounds__(KVA_THREADS)
+    k_kv_append_any(const __grid_constant__ RotaryParams P, const __grid_constant__ AppendArgs A) {
+    extern __shared__ float kva_smem[];
+    constexpr int PITCH = HD + 1;
+    float *rows = kva_smem;                                             // [page][PITCH]
+    float2 *trig = reinterpret_cast<float2 *>(kva_smem + A.page * PITCH + (A.page * PITCH & 1));  // [page][half + 1]
+    int from, to, phys, row0;
+    if (!append_span(A, from, to, phys, row0)) return;
+    const int cnt = to - from, t0 = from % A.page;
     const int half = P.rot / 2;
     for (int e = threadIdx.x; e < cnt * half; e += KVA_THREADS) {
         const int t = e / half, i = e - t * half;
@@ -334,17 +463,25 @@ __global__ void __launch_bounds__(KVA_THREADS)
     }
 }
 
-template <typename T, int HD>
+template <typename T, int HD, int PAGE>
 static void launch_append(fb_ctx *ctx, const RotaryParams &P, AppendArgs A, int batch) {
-    const int tiles = (A.max_new + A.page - 2) / A.page + 1;
-    // heads of a block share its angles; fewer blocks than two a SM would leave SMs idle
+    const int tiles = (A.max_new + PAGE - 2) / PAGE + 1;
+    // heads of a block share its angles; with fewer than two blocks a SM each has a block of its own
     const int64_t blocks = (int64_t)tiles * batch * A.n_kv;
-    int hpb = (int)(blocks / (2 * ctx->num_sms));
-    A.heads_per_block = hpb < 1 ? 1 : hpb > A.n_kv ? A.n_kv : hpb;
-    const size_t smem = (size_t)(A.page * (HD + 1) + 1) * 4 + (size_t)A.page * (P.rot / 2 + 1) * 8;
-    FB_CUDA(cudaFuncSetAttribute(k_kv_append<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const int64_t hpb = blocks / (2 * ctx->num_sms);
+    A.heads_per_block = hpb < 1 ? 1 : hpb > A.n_kv ? A.n_kv : (int)hpb;
+    // 16-byte loads and whole chunks of 8 dimensions (of either half in mode 1)
+    const bool fast = A.vec && P.rot % (P.mode == 1 ? 16 : 8) == 0;
+    if (fast && A.heads_per_block > KVA_HEADS) A.heads_per_block = KVA_HEADS;
     const dim3 grid((unsigned)tiles, (unsigned)((A.n_kv + A.heads_per_block - 1) / A.heads_per_block), (unsigned)batch);
-    k_kv_append<T, HD><<<grid, KVA_THREADS, smem, ctx->stream>>>(P, A);
+    auto go = [&](auto kernel, size_t smem) {
+        FB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        kernel<<<grid, KVA_THREADS, smem, ctx->stream>>>(P, A);
+    };
+    const size_t tile = (size_t)A.heads_per_block * HD * PAGE * 2;
+    if (!fast) go(k_kv_append_any<T, HD>, (size_t)(PAGE * (HD + 1) + 1) * 4 + (size_t)PAGE * (P.rot / 2 + 1) * 8);
+    else if (P.mode == 1) go(k_kv_append<T, HD, PAGE, 1>, tile);
+    else go(k_kv_append<T, HD, PAGE, 0>, tile);
     FB_CUDA(cudaGetLastError());
 }
 
@@ -502,8 +639,10 @@ int fb_kv_append(fb_ctx *ctx, const fb_rotary *r, int dtype, const void *k_dev, 
         const RotaryParams P = rotary_params(r);
         auto go = [&](auto t) {
             using T = decltype(t);
-            if (head_dim == 128) launch_append<T, 128>(ctx, P, A, batch);
-            else launch_append<T, 64>(ctx, P, A, batch);
+            if (head_dim == 128 && page_size == 64) launch_append<T, 128, 64>(ctx, P, A, batch);
+            else if (head_dim == 128) launch_append<T, 128, 32>(ctx, P, A, batch);
+            else if (page_size == 64) launch_append<T, 64, 64>(ctx, P, A, batch);
+            else launch_append<T, 64, 32>(ctx, P, A, batch);
         };
         if (dtype == FB_F32) go(float{});
         else if (dtype == FB_F16) go(__half{});
