@@ -344,9 +344,6 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     volatile int *s_odd = s_odd_raw;        // segment (+ 1) that met non-finite values of new rows
     volatile uint8_t *s_skip = s_skip_raw;  // block: halves whose page id is outside the pool
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_launch();
-    TreeWalk w;
-    if (!w.start(A, blockIdx.x, lane, blockIdx.x == 0 && warp == 0)) return;
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *sQ = sm;                      // [tile][high parts, low parts]
     uint8_t *sK = sQ + 2 * C::TILE_BYTES;  // [stage]
@@ -380,12 +377,18 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    pdl_wait();    // (the set-up above overlaps the predecessor's end)
+    pdl_launch();  // (now: the join reads the lengths before it waits)
+    TreeWalk w;
+    const bool share = w.start(A, blockIdx.x, lane, blockIdx.x == 0 && warp == 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    if (warp == 8 || warp == 10) {
+    if (!share) {
+        // nothing to do: straight to the release of the tensor memory
+    } else if (warp == 8 || warp == 10) {
         // ---- TMA: K pages (warp 8), V pages (warp 10); the lanes read 32 page ids ahead
         const bool isk = warp == 8;
         uint64_t *full = isk ? k_full : v_full, *empty = isk ? k_empty : v_empty;
@@ -954,21 +957,13 @@ static void launch_tree(fb_ctx *ctx, const TreeArgs &A, const TreePlan &plan, co
                         const CUtensorMap &vmap) {
     constexpr size_t smem = TreeCfg<T, HD>::SMEM;
     FB_CUDA(cudaFuncSetAttribute(k_attn_tree<T, HD, PAGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    k_attn_tree<T, HD, PAGE><<<plan.ctas, TR_THREADS, smem, ctx->stream>>>(kmap, vmap, A);
-    FB_CUDA(cudaGetLastError());
+    launch_with(ctx->stream, ctx->pdl, k_attn_tree<T, HD, PAGE>, dim3((unsigned)plan.ctas), TR_THREADS, smem, 1, kmap, vmap,
+               A);
     if (!plan.split) return;
-    // the join's blocks start while the attention drains and wait for it (programmatic dependent launch)
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = ctx->pdl ? 1 : 0;
-    cfg.gridDim = dim3((unsigned)(plan.pairs * (plan.rows_cap / 32) * 4), (unsigned)A.n_kv, (unsigned)A.batch);
-    cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = (size_t)plan.ctas * 32 * sizeof(float2);  // (a group has at most one part a CTA)
-    cfg.stream = ctx->stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    FB_CUDA(cudaLaunchKernelEx(&cfg, k_attn_tree_join<T, HD>, A));
+    // the join's blocks start while the attention drains and wait for it
+    launch_with(ctx->stream, ctx->pdl, k_attn_tree_join<T, HD>,
+               dim3((unsigned)(plan.pairs * (plan.rows_cap / 32) * 4), (unsigned)A.n_kv, (unsigned)A.batch), 128,
+               (size_t)plan.ctas * 32 * sizeof(float2), 1, A);  // (a group has at most one part a CTA)
 }
 
 static void check_tree_shape(int batch, int max_new, int n_heads, int n_kv, int head_dim, int page_size,

@@ -69,6 +69,31 @@ struct DeviceGuard {
     DeviceGuard &operator=(const DeviceGuard &) = delete;
 };
 
+// Launches a kernel with its attributes.  pdl: it reads and writes nothing before
+// its pdl_wait(), so it may be brought up while its predecessor on the stream
+// still runs (fb_ctx_set_pdl); it calls pdl_launch() after that wait, so that what
+// comes before it is complete for its dependents too.  cluster > 1: CTAs a
+// thread-block cluster.
+template <class... P, class... A>
+void launch_with(cudaStream_t stream, bool pdl, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem,
+                unsigned cluster, const A &...args) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    FB_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+}
+
 // A device buffer owned by the library.
 struct DevBuf {
     void *ptr = nullptr;

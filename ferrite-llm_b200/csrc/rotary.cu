@@ -115,80 +115,93 @@ template <typename T, bool VEC, int MODE> struct RotUnit {
     }
 };
 
-// Thread = (token of the block, head slot, unit of a head), unit fastest; it
-// walks the heads hslot, hslot + step, ... with the angles of its pairs in
-// registers.  The block's angles are computed once into shared memory.
+// grid (tiles of tt tokens, shares of a tile's (token, head) items): thread = (item
+// slot, unit of a head), unit fastest.  A unit is a rotated one or, behind those
+// and unless the rotation is in place, a vector to copy.  A thread has the values
+// of up to ROT_AHEAD items in flight while the tile's angles are computed, an
+// angle a thread.
+constexpr int ROT_AHEAD = 2;
 template <typename T, bool VEC, int MODE>
 __global__ void __launch_bounds__(ROT_THREADS)
     k_rotary(const __grid_constant__ RotaryParams P, const T *x, int64_t xt, int64_t xh, T *y, int64_t yt, int64_t yh,
-             const int32_t *__restrict__ positions, int64_t n_tok, int n_heads, int dim, int tt, int hs) {
+             const int32_t *__restrict__ positions, int64_t n_tok, int n_heads, int dim, int tt, int items) {
     using U = RotUnit<T, VEC, MODE>;
-    constexpr int AHEAD = 4;  // heads a thread has in flight
     extern __shared__ float2 trig[];  // [tt][rot / 2]
-    const int half = P.rot / 2, uph = half / U::NP;
+    const int half = P.rot / 2, turned = half / U::NP;
+    const bool copies = x != y && VEC;
+    const int units = turned + (copies ? (dim - P.rot) / U::V : 0), slots = ROT_THREADS / units;
     const int64_t tok0 = (int64_t)blockIdx.x * tt;
-    const int unit = threadIdx.x % uph, slot = threadIdx.x / uph;
-    const int tl = slot / hs;
-    const int64_t tok = tok0 + tl;
-    const int h0 = slot % hs + blockIdx.y * hs, step = hs * gridDim.y;
-    const bool active = tl < tt && tok < n_tok;
-    U w[AHEAD];
+    const int unit = threadIdx.x % units, slot = threadIdx.x / units;
+    const int ntok = (int)min((int64_t)tt, n_tok - tok0);
+    const int first = blockIdx.y * items, last = min(first + items, ntok * n_heads);
+    const bool turn = unit < turned, active = slot < slots;
+    const int rest0 = P.rot + (unit - turned) * U::V;  // of a copied vector
+    U w[ROT_AHEAD];
+    auto fetch = [&](int i0) {
 #pragma unroll
-    for (int k = 0; k < AHEAD; k++)
-        if (active && h0 + k * step < n_heads) w[k].load(x + tok * xt + (h0 + k * step) * xh, unit, P.rot);
-    for (int e = threadIdx.x; e < tt * half; e += ROT_THREADS) {
+        for (int k = 0; k < ROT_AHEAD; k++) {
+            const int i = i0 + k * slots;
+            if (!active || i >= last) continue;
+            const int t = i / n_heads;
+            const T *src = x + (tok0 + t) * xt + (i - t * n_heads) * xh;
+            if (turn) w[k].load(src, unit, P.rot);
+            else if constexpr (VEC) *reinterpret_cast<uint4 *>(w[k].a) = *reinterpret_cast<const uint4 *>(src + rest0);
+        }
+    };
+    fetch(first + slot);
+    for (int e = threadIdx.x; e < ntok * half; e += ROT_THREADS) {
         const int t = e / half;
-        if (tok0 + t < n_tok) trig[e] = rotary_trig(P, e - t * half, positions[tok0 + t]);
+        trig[e] = rotary_trig(P, e - t * half, positions[tok0 + t]);
     }
     __syncthreads();
-    if (active) {
-        float2 cs[U::NP];
+    for (int i0 = first + slot; i0 < last; i0 += ROT_AHEAD * slots) {
+        if (i0 != first + slot) fetch(i0);
 #pragma unroll
-        for (int i = 0; i < U::NP; i++) cs[i] = trig[tl * half + unit * U::NP + i];
-        for (int h = h0; h < n_heads; h += AHEAD * step) {
-            if (h != h0)
+        for (int k = 0; k < ROT_AHEAD; k++) {
+            const int i = i0 + k * slots;
+            if (!active || i >= last) break;
+            const int t = i / n_heads;
+            T *dst = y + (tok0 + t) * yt + (i - t * n_heads) * yh;
+            if (turn) {
+                float2 cs[U::NP];
 #pragma unroll
-                for (int k = 0; k < AHEAD; k++)
-                    if (h + k * step < n_heads) w[k].load(x + tok * xt + (h + k * step) * xh, unit, P.rot);
-#pragma unroll
-            for (int k = 0; k < AHEAD; k++)
-                if (h + k * step < n_heads) {
-                    w[k].turn(cs);
-                    w[k].store(y + tok * yt + (h + k * step) * yh, unit, P.rot);
-                }
+                for (int j = 0; j < U::NP; j++) cs[j] = trig[t * half + unit * U::NP + j];
+                w[k].turn(cs);
+                w[k].store(dst, unit, P.rot);
+            } else if constexpr (VEC) {
+                *reinterpret_cast<uint4 *>(dst + rest0) = *reinterpret_cast<const uint4 *>(w[k].a);
+            }
         }
     }
-    // dimensions behind the rotated ones, unless the rotation is in place
-    const int rest = (dim - P.rot) / U::V;
-    if (x != y && rest > 0) {
-        const int heads = (n_heads - blockIdx.y + gridDim.y - 1) / gridDim.y;  // this block's share
-        for (int e = threadIdx.x; e < tt * heads * rest; e += ROT_THREADS) {
-            const int d = e % rest, q = e / rest, h = (q % heads) * gridDim.y + blockIdx.y;
-            const int64_t t = tok0 + q / heads;
-            if (t >= n_tok) break;
-            const T *src = x + t * xt + h * xh + P.rot;
-            T *dst = y + t * yt + h * yh + P.rot;
-            if constexpr (VEC) reinterpret_cast<uint4 *>(dst)[d] = reinterpret_cast<const uint4 *>(src)[d];
-            else dst[d] = src[d];
-        }
+    if constexpr (!VEC) {  // element by element: the dimensions behind the rotated ones
+        const int rest = dim - P.rot;
+        if (x != y && rest > 0)
+            for (int e = threadIdx.x; e < (last - first) * rest; e += ROT_THREADS) {
+                const int d = P.rot + e % rest, i = first + e / rest, t = i / n_heads, h = i - t * n_heads;
+                y[(tok0 + t) * yt + h * yh + d] = x[(tok0 + t) * xt + h * xh + d];
+            }
     }
 }
 
 template <typename T, bool VEC, int MODE>
 static void launch_rotary_as(fb_ctx *ctx, const RotaryParams &P, const T *x, int64_t xt, int64_t xh, T *y, int64_t yt,
                              int64_t yh, const int32_t *positions, int64_t n_tok, int n_heads, int dim) {
-    const int uph = P.rot / 2 / RotUnit<T, VEC, MODE>::NP;  // 1..128
-    const int hs = n_heads < ROT_THREADS / uph ? n_heads : ROT_THREADS / uph;
-    int tt = ROT_THREADS / (uph * hs);
-    // few tokens: fewer of them a block, then the heads over several blocks, until every SM has one
-    while (tt > 1 && (n_tok + tt - 1) / tt < ctx->num_sms) tt = (tt + 1) / 2;
+    using U = RotUnit<T, VEC, MODE>;
+    const int units = P.rot / 2 / U::NP + (VEC && x != y ? (dim - P.rot) / U::V : 0);  // 1..256
+    const int slots = ROT_THREADS / units;
+    // tokens a block: as many as keep ROT_AHEAD items a thread in flight (and 2048 angles at most), fewer
+    // while blocks are scarcer than two a SM; then a token's heads over several blocks
+    int tt = (ROT_AHEAD * slots + n_heads - 1) / n_heads;
+    if (tt > 4096 / P.rot) tt = 4096 / P.rot;
+    while (tt > 1 && (n_tok + tt - 1) / tt < 2 * ctx->num_sms) tt = (tt + 1) / 2;
     const int64_t gx = (n_tok + tt - 1) / tt;
     FB_REQUIRE(gx <= 0x7fffffff, "rotary_apply: too many tokens");
-    int64_t gy = (n_heads + hs - 1) / hs;
+    int64_t gy = (tt * (int64_t)n_heads + slots - 1) / slots;  // blocks with an item a thread
     if (gx * gy > ctx->num_sms) gy = gx >= ctx->num_sms ? 1 : ctx->num_sms / gx;
+    const int items = (int)((tt * (int64_t)n_heads + gy - 1) / gy);
     const size_t smem = (size_t)tt * (P.rot / 2) * sizeof(float2);
     k_rotary<T, VEC, MODE><<<dim3((unsigned)gx, (unsigned)gy), ROT_THREADS, smem, ctx->stream>>>(
-        P, x, xt, xh, y, yt, yh, positions, n_tok, n_heads, dim, tt, hs);
+        P, x, xt, xh, y, yt, yh, positions, n_tok, n_heads, dim, tt, items);
     FB_CUDA(cudaGetLastError());
 }
 
@@ -198,9 +211,10 @@ static void launch_rotary(fb_ctx *ctx, const RotaryParams &P, const void *xv, in
     constexpr int V = 16 / (int)sizeof(T);
     const T *x = static_cast<const T *>(xv);
     T *y = static_cast<T *>(yv);
-    // 16-byte accesses: every head starts on 16 bytes and the rotated part (its halves in mode 1) is whole vectors
+    // 16-byte accesses: every head starts on 16 bytes, the rotated part (its halves in mode 1) is whole vectors, and
+    // a head is no more of them than a block has threads
     const bool vec = (((uintptr_t)xv | (uintptr_t)yv) & 15) == 0 && (xt | xh | yt | yh) % V == 0 && dim % V == 0 &&
-                     (P.mode == 1 ? P.rot / 2 : P.rot) % V == 0;
+                     (P.mode == 1 ? P.rot / 2 : P.rot) % V == 0 && dim / V <= ROT_THREADS;
     auto go = [&](auto v, auto m) {
         launch_rotary_as<T, decltype(v)::value, decltype(m)::value>(ctx, P, x, xt, xh, y, yt, yh, positions, n_tok,
                                                                     n_heads, dim);
@@ -477,12 +491,12 @@ static void launch_append(fb_ctx *ctx, const RotaryParams &P, AppendArgs A, int 
     auto go = [&](auto kernel, size_t smem) {
         FB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         kernel<<<grid, KVA_THREADS, smem, ctx->stream>>>(P, A);
+        FB_CUDA(cudaGetLastError());
     };
     const size_t tile = (size_t)A.heads_per_block * HD * PAGE * 2;
     if (!fast) go(k_kv_append_any<T, HD>, (size_t)(PAGE * (HD + 1) + 1) * 4 + (size_t)PAGE * (P.rot / 2 + 1) * 8);
     else if (P.mode == 1) go(k_kv_append<T, HD, PAGE, 1>, tile);
     else go(k_kv_append<T, HD, PAGE, 0>, tile);
-    FB_CUDA(cudaGetLastError());
 }
 
 }  // namespace fb

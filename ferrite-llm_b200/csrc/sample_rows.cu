@@ -1005,19 +1005,7 @@ template <typename T> static void launch_sample_rows(fb_ctx *ctx, SampleRowsArgs
     auto kernel = k_sample_rows<T>;
     FB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     if (cs > 8) FB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)cs;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(rows * cs));
-    cfg.blockDim = dim3(SR_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = ctx->stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    FB_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const SampleRowsArgs)A));
+    launch_with(ctx->stream, false, kernel, dim3((unsigned)(rows * cs)), SR_THREADS, smem, (unsigned)cs, A);
 }
 
 }  // namespace fb
