@@ -257,6 +257,11 @@ struct TreeWalk {
     __device__ __forceinline__ bool whole() const { return blk0 == 0 && blk1 == s.blocks; }
 };
 
+// The power of two that a row's queries are divided by, from the exponent field of
+// their largest magnitude: it comes to 2^13..2^14 (rows below 2^-107 less, which
+// costs them no bit; 0 and non-finite ones stay).
+__device__ __forceinline__ int tree_shift(int ex) { return ex == 0 || ex == 255 ? 0 : max(ex - 127 - 13, -120); }
+
 // A row's new row of its sequence: row / group (exact while row group < 2^32).
 __device__ __forceinline__ int tree_token(const TreeArgs &A, int row) {
     return (int)(((uint64_t)(uint32_t)row * A.inv_group) >> 32);
@@ -538,65 +543,89 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         uint32_t npair = 0;  // uses of pair_bar[qd]
         bool ok = true;
         int cb = 0, jb = 0, seg = 0;  // blocks and this group's jobs of the segments before
-        // The group's queries as fp16 parts scaled by 2^-e: HD / 8 lanes a row, the 8 warps share the rows.
+        // The group's queries as fp16 parts scaled by 2^-e: HD / 8 lanes a row, the 8 warps share the rows.  f32: two
+        // batches of loads through registers (128 KB for two tiles: L2's rate, shared by all CTAs, bounds them).  16-bit:
+        // copied as they are into their places, all copies in flight together, and (bf16) turned in place by the
+        // thread that copied them, in rolled loops: code that runs once a segment arrives more slowly than it executes.
         auto load_q = [&](const TreeWalk &t, int sg) {
-            constexpr int LPR = HD / 8, RPI = 32 / LPR, NV = sizeof(T) / 2, AHEAD = 16 / NV;  // 64 registers in flight
+            constexpr int LPR = HD / 8, RPI = 32 / LPR;
             const int rows = t.rows(A), each = (t.both() ? TR_PAIR : TR_ROWS) / 8, d = (lane % LPR) * 8;
-            for (int i0 = 0; i0 < each; i0 += RPI * AHEAD) {
-                uint4 raw[AHEAD][NV];
+            const T *base = static_cast<const T *>(A.q) + (int64_t)t.s.off * A.qt + (int64_t)t.h * A.group * HD + d;
+            auto place = [&](int rr) {
+                return sQ + (rr >> 7) * C::TILE_BYTES + (uint32_t)(d >> 6) * (TR_ROWS * 128) +
+                       sw128_off(rr & 127, (d >> 3) & 7);
+            };
+            auto source = [&](int rr) {
+                const int row = t.row0() + rr, tok = tree_token(A, row);
+                return base + (int64_t)tok * A.qt + (int64_t)(row - tok * A.group) * HD;
+            };
+            auto turn = [&](float (&x)[8], int rr, uint4 &hi, uint4 &lo) {
+                float mx = 0.f;
 #pragma unroll
-                for (int k = 0; k < AHEAD; k++) {
-                    const int rr = warp * each + i0 + k * RPI + lane / LPR;
+                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[e]));
 #pragma unroll
-                    for (int i = 0; i < NV; i++) raw[k][i] = make_uint4(0, 0, 0, 0);
-                    if (i0 + k * RPI < each && rr < rows) {
-                        const int row = t.row0() + rr, tok = tree_token(A, row);
-                        const T *src = static_cast<const T *>(A.q) + (int64_t)(t.s.off + tok) * A.qt +
-                                       (int64_t)(t.h * A.group + row - tok * A.group) * HD + d;
-                        if (A.qvec) {
+                for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
+                const int ex = (int)((__float_as_uint(mx) >> 23) & 255u);
+                const float f = __fmul_rn(sign, __uint_as_float((uint32_t)(127 - tree_shift(ex)) << 23));
 #pragma unroll
-                            for (int i = 0; i < NV; i++) raw[k][i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
-                        } else {
-                            T *e = reinterpret_cast<T *>(raw[k]);
+                for (int e = 0; e < 8; e++) x[e] = __fmul_rn(x[e], f);
+                split8(x, hi, lo);
+                if (d == 0) s_qe[sg & 1][rr] = (uint8_t)ex;
+            };
+            if constexpr (C::LO) {
+                constexpr int AHEAD = 8;
+                for (int i0 = 0; i0 < each; i0 += RPI * AHEAD) {
+                    float x[AHEAD][8];
 #pragma unroll
-                            for (int i = 0; i < 8; i++) e[i] = src[i];
-                        }
+                    for (int k = 0; k < AHEAD; k++) {
+                        const int rr = warp * each + i0 + k * RPI + lane / LPR;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[k][e] = 0.f;
+                        if (i0 + k * RPI < each && rr < rows) tr_load8(source(rr), A.qvec, x[k]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < AHEAD; k++) {
+                        if (i0 + k * RPI >= each) break;
+                        const int rr = warp * each + i0 + k * RPI + lane / LPR;
+                        uint4 hi, lo;
+                        turn(x[k], rr, hi, lo);
+                        *reinterpret_cast<uint4 *>(place(rr)) = hi;
+                        *reinterpret_cast<uint4 *>(place(rr) + C::Q_BYTES) = lo;
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < AHEAD; k++) {
-                    if (i0 + k * RPI >= each) break;
-                    const int rr = warp * each + i0 + k * RPI + lane / LPR;
-                    uint4 hi, lo;
-                    int ex = 0;  // (f16 queries enter as they are)
-                    if constexpr (std::is_same<T, __half>::value) {
-                        const uint32_t flip = A.scale < 0.f ? 0x80008000u : 0u;
-                        hi = make_uint4(raw[k][0].x ^ flip, raw[k][0].y ^ flip, raw[k][0].z ^ flip, raw[k][0].w ^ flip);
+            } else {
+#pragma unroll 1
+                for (int i0 = 0; i0 < each; i0 += RPI) {
+                    const int rr = warp * each + i0 + lane / LPR;
+                    uint8_t *dst = place(rr);
+                    if (rr >= rows) {
+                        *reinterpret_cast<uint4 *>(dst) = make_uint4(0, 0, 0, 0);
+                    } else if (A.qvec) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(source(rr))
+                                     : "memory");
                     } else {
-                        float x[8], mx = 0.f;
+                        const T *src = source(rr);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            x[e] = tr_f32(reinterpret_cast<const T *>(raw[k])[e]);
-                            mx = fmaxf(mx, fabsf(x[e]));
-                        }
-#pragma unroll
-                        for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
-                        // exponent that brings the row's largest value to 2^13..2^14 (0 and non-finite rows stay)
-                        ex = (int)((__float_as_uint(mx) >> 23) & 255u);
-                        const int e2 = (ex == 0 || ex == 255) ? 0 : ex - 127 - 13;
-                        // 2^-e in two factors: e reaches -139 and 114
-                        const float f0 = __fmul_rn(sign, __uint_as_float((uint32_t)(127 - e2 / 2) << 23));
-                        const float f1 = __uint_as_float((uint32_t)(127 - (e2 - e2 / 2)) << 23);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] = __fmul_rn(__fmul_rn(x[e], f0), f1);
-                        split8(x, hi, lo);
+                        for (int i = 0; i < 8; i++) reinterpret_cast<T *>(dst)[i] = src[i];
                     }
-                    uint8_t *dst = sQ + (rr >> 7) * C::TILE_BYTES + (uint32_t)(d >> 6) * (TR_ROWS * 128) +
-                                   sw128_off(rr & 127, (d >> 3) & 7);
-                    *reinterpret_cast<uint4 *>(dst) = hi;
-                    if constexpr (C::LO) *reinterpret_cast<uint4 *>(dst + C::Q_BYTES) = lo;
-                    if (d == 0) s_qe[sg & 1][rr] = (uint8_t)ex;
                 }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                constexpr bool half = std::is_same<T, __half>::value;  // (f16 queries enter as they are)
+                if (!half || A.scale < 0.f)
+#pragma unroll 2
+                    for (int i0 = 0; i0 < each; i0 += RPI) {
+                        const int rr = warp * each + i0 + lane / LPR;
+                        uint4 *dst = reinterpret_cast<uint4 *>(place(rr));
+                        if constexpr (half) {
+                            const uint4 q = *dst;
+                            *dst = make_uint4(q.x ^ 0x80008000u, q.y ^ 0x80008000u, q.z ^ 0x80008000u, q.w ^ 0x80008000u);
+                        } else {
+                            float x[8];
+                            uint4 lo;
+                            tr_load8(reinterpret_cast<const T *>(dst), true, x);
+                            turn(x, rr, *dst, lo);
+                        }
+                    }
             }
             fence_proxy_async_smem();  // the tensor core reads them through the async proxy
             __syncwarp();
@@ -712,12 +741,12 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             tok = tree_token(A, row);
             if (!(ok = tr_wait(&q_full, (uint32_t)seg & 1u))) break;
             // this row's score unit, |scale| log2(e) 2^e (not 0: masked scores stay -inf)
-            const int ex = s_qe[seg & 1][(both ? TR_ROWS * g : 0) + r];
-            const int e2 = (ex == 0 || ex == 255) ? 0 : ex - 127 - 13;
-            const float sl2 = fmaxf(__fmul_rn(__fmul_rn(__fmul_rn(fabsf(A.scale), 1.4426950408889634f),
-                                                        __uint_as_float((uint32_t)(127 + e2 / 2) << 23)),
-                                              __uint_as_float((uint32_t)(127 + (e2 - e2 / 2)) << 23)),
-                                    1e-37f);
+            float sl2 = __fmul_rn(fabsf(A.scale), 1.4426950408889634f);
+            if constexpr (!std::is_same<T, __half>::value) {
+                const int e2 = tree_shift(s_qe[seg & 1][(both ? TR_ROWS * g : 0) + r]);
+                sl2 = __fmul_rn(sl2, __uint_as_float((uint32_t)(127 + e2) << 23));
+            }
+            sl2 = fmaxf(sl2, 1e-37f);
             m = TR_NONE;
             l = 0.f;
             for (int k = 0; k < nj; k++) {
@@ -842,12 +871,15 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 }
 
 // Joins the partials of the row groups that several CTAs hold.  grid (row groups a
-// kv head x rows_cap / 32 x dim quarters, n_kv, batch): lane = row, warp = HD / 64
-// four-dim columns.
+// kv head x rows_cap / 32 x HD / 16, n_kv, batch): lane = row, warp = one column of
+// four dimensions; the parts are read in batches of JOIN, all loads of one in
+// flight together.
+constexpr int JOIN = 8;
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ TreeArgs A) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int quarter = blockIdx.x & 3, rest = blockIdx.x >> 2;
+    constexpr int CG = HD / 16;  // column groups
+    const int cgroup = blockIdx.x % CG, rest = blockIdx.x / CG;
     const int slabs = A.rows_cap / 32, slab = rest % slabs, pair = rest / slabs;
     const int b = blockIdx.z;
     TreeSeq s;
@@ -877,57 +909,49 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
     const int64_t slot = (int64_t)(HD + 2) * A.rows_cap;
     // the CTA with the group's first block keeps it as its partial 1, the others as their 0
     auto part = [&](int c) { return A.part + (2 * (int64_t)c + (c == c0)) * slot; };
-    // the parts' (max, sum) of the slab's rows, all loads in flight together
-    extern __shared__ float2 s_part[];  // [part][row]
     pdl_wait();
-    const int parts = c1 - c0 + 1;
-    for (int i = threadIdx.x; i < parts * 32; i += 128)
-        s_part[i] = reinterpret_cast<const float2 *>(part(c0 + i / 32) + (int64_t)HD * A.rows_cap)[32 * slab + (i & 31)];
-    __syncthreads();
-    float M = TR_NONE;
-    for (int c = 0; c < parts; c++) M = fmaxf(M, s_part[32 * c + lane].x);
-    float L = 0.f;
-    constexpr int N = HD / 64;  // float4 columns a thread
-    float4 o[N];
+    const int col = cgroup * 4 + warp;
+    float M = TR_NONE, L = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = c0; c <= c1; c += JOIN) {
+        float2 ml[JOIN];
+        float4 v[JOIN];
 #pragma unroll
-    for (int k = 0; k < N; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int col0 = quarter * (HD / 16) + warp * N;
-    for (int c = 0; c < parts; c += 8) {
-        float4 v[8][N];
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int k = 0; k < N; k++)
-                if (c + i < parts)
-                    v[i][k] = reinterpret_cast<const float4 *>(part(c0 + c + i))[(int64_t)(col0 + k) * A.rows_cap + r];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (c + i >= parts) break;
-            const float2 ml = s_part[32 * (c + i) + lane];
-            const float wgt = exp2f(__fsub_rn(ml.x, M));
-            L = __fmaf_rn(wgt, ml.y, L);
-#pragma unroll
-            for (int k = 0; k < N; k++) {
-                o[k].x = __fmaf_rn(wgt, v[i][k].x, o[k].x);
-                o[k].y = __fmaf_rn(wgt, v[i][k].y, o[k].y);
-                o[k].z = __fmaf_rn(wgt, v[i][k].z, o[k].z);
-                o[k].w = __fmaf_rn(wgt, v[i][k].w, o[k].w);
+        for (int i = 0; i < JOIN; i++)
+            if (c + i <= c1) {
+                const float *p = part(c + i);
+                ml[i] = reinterpret_cast<const float2 *>(p + (int64_t)HD * A.rows_cap)[r];
+                v[i] = reinterpret_cast<const float4 *>(p)[(int64_t)col * A.rows_cap + r];
             }
-        }
+        float mn = M;
+#pragma unroll
+        for (int i = 0; i < JOIN; i++)
+            if (c + i <= c1) mn = fmaxf(mn, ml[i].x);
+        const float al = exp2f(__fsub_rn(M, mn));  // (1 where nothing has been seen yet: there is nothing to scale)
+        M = mn;
+        L = __fmul_rn(L, al);
+        o = make_float4(__fmul_rn(o.x, al), __fmul_rn(o.y, al), __fmul_rn(o.z, al), __fmul_rn(o.w, al));
+#pragma unroll
+        for (int i = 0; i < JOIN; i++)
+            if (c + i <= c1) {
+                const float wgt = exp2f(__fsub_rn(ml[i].x, M));
+                L = __fmaf_rn(wgt, ml[i].y, L);
+                o.x = __fmaf_rn(wgt, v[i].x, o.x);
+                o.y = __fmaf_rn(wgt, v[i].y, o.y);
+                o.z = __fmaf_rn(wgt, v[i].z, o.z);
+                o.w = __fmaf_rn(wgt, v[i].w, o.w);
+            }
     }
     const int rr = row0 + lane;
     if (rr >= s.n * A.group) return;
     const float inv = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
     const int tok = tree_token(A, rr);
     T *out = static_cast<T *>(A.out) + (int64_t)(s.off + tok) * A.ot +
-             (int64_t)(blockIdx.y * A.group + rr - tok * A.group) * HD + 4 * col0;
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-        tr_put(out + 4 * k, __fmul_rn(o[k].x, inv));
-        tr_put(out + 4 * k + 1, __fmul_rn(o[k].y, inv));
-        tr_put(out + 4 * k + 2, __fmul_rn(o[k].z, inv));
-        tr_put(out + 4 * k + 3, __fmul_rn(o[k].w, inv));
-    }
+             (int64_t)(blockIdx.y * A.group + rr - tok * A.group) * HD + 4 * col;
+    tr_put(out, __fmul_rn(o.x, inv));
+    tr_put(out + 1, __fmul_rn(o.y, inv));
+    tr_put(out + 2, __fmul_rn(o.z, inv));
+    tr_put(out + 3, __fmul_rn(o.w, inv));
 }
 
 // What a call of these sizes launches.
@@ -962,8 +986,8 @@ static void launch_tree(fb_ctx *ctx, const TreeArgs &A, const TreePlan &plan, co
     if (!plan.split) return;
     // the join's blocks start while the attention drains and wait for it
     launch_with(ctx->stream, ctx->pdl, k_attn_tree_join<T, HD>,
-               dim3((unsigned)(plan.pairs * (plan.rows_cap / 32) * 4), (unsigned)A.n_kv, (unsigned)A.batch), 128,
-               (size_t)plan.ctas * 32 * sizeof(float2), 1, A);  // (a group has at most one part a CTA)
+               dim3((unsigned)(plan.pairs * (plan.rows_cap / 32) * (HD / 16)), (unsigned)A.n_kv, (unsigned)A.batch), 128,
+               0, 1, A);
 }
 
 static void check_tree_shape(int batch, int max_new, int n_heads, int n_kv, int head_dim, int page_size,
