@@ -337,7 +337,10 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     constexpr uint32_t IDESC_S = umma_idesc_f16(TR_ROWS, TR_KB, false, true);
     constexpr uint32_t IDESC_O = umma_idesc_f16(TR_ROWS, HD, false, true);
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST];
+    // A stage's full barrier alternates between two: a waiter meets its block's phase there without having waited for
+    // the block before it in that stage (with one tile the groups take every other block).  The barrier's own last
+    // block, 2 ST back, has been consumed by then: a block is loaded only once the one ST back has been.
+    __shared__ uint64_t k_full[2 * ST], k_empty[ST], v_full[2 * ST], v_empty[ST];
     __shared__ uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [group][buffer]
     __shared__ uint64_t q_full, q_empty, o_free, fin[2], go, pair_bar[4];
     __shared__ uint32_t s_tmem;
@@ -356,8 +359,10 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; i++) {
             mbar_init(&k_full[i], 1);
+            mbar_init(&k_full[ST + i], 1);
             mbar_init(&k_empty[i], 2);  // (both MMA warps)
             mbar_init(&v_full[i], 1);
+            mbar_init(&v_full[ST + i], 1);
             mbar_init(&v_empty[i], 2);
         }
         for (int i = 0; i < 4; i++) {
@@ -419,7 +424,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                         page[i] = 0;
                     }
                 }
-                const int st = c % ST;
+                const int st = c % ST, fb = c % (2 * ST);
                 if (lane == 0) {
                     // (the first queries, two dependent steps from the first scores, are not queued behind the rings)
                     if (c == 1) ok = tr_wait(&go, 0);
@@ -430,17 +435,17 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                             s_skip[c & 15] = (uint8_t)skip;
                             if (skip) atomicOr(A.err, ERRBIT_BAD_PAGE);
                         }
-                        mbar_expect_tx(&full[st], C::KV_BYTES);
+                        mbar_expect_tx(&full[fb], C::KV_BYTES);
 #pragma unroll
                         for (int i = 0; i < PPB; i++) {
                             const int row = page[i] * A.n_kv + w.h;
                             if (isk) {
-                                tma_load_2d(dst + i * (HD * PAGE * 2), &kmap, 0, row * HD, &full[st]);
+                                tma_load_2d(dst + i * (HD * PAGE * 2), &kmap, 0, row * HD, &full[fb]);
                             } else {
 #pragma unroll
                                 for (int d = 0; d < HD / 64; d++)
                                     tma_load_2d(dst + d * (TR_KB * 128) + i * (PAGE * 128), &vmap, 64 * d, row * PAGE,
-                                                &full[st]);
+                                                &full[fb]);
                             }
                         }
                     }
@@ -451,7 +456,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         if (lane == 0) {
             if (!ok) s_abort = 1;
             // copies in flight land before shared memory is released
-            for (int k = c > ST ? c - ST : 0; k < c; k++) tr_wait(&full[k % ST], (uint32_t)(k / ST) & 1u);
+            for (int k = c > ST ? c - ST : 0; k < c; k++)
+                mbar_wait_bounded(&full[k % (2 * ST)], (uint32_t)(k / (2 * ST)) & 1u);
         }
     } else if (warp == 9 || warp == 11) {
         // ---- MMA issue for group g: its next scores before its products of this block.  (The tensor core runs one
@@ -469,12 +475,14 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 const bool both = w.both();
                 const int nj = w.jobs(g), step = both ? 1 : 2;
                 const uint64_t dq = dQ + (both ? g : 0) * (C::TILE_BYTES >> 4);
-                int ks_c = cb + (both ? 0 : g), kst = ks_c % ST, vst = kst;  // the next blocks' ring stages and phases
-                uint32_t kph = (uint32_t)(ks_c / ST) & 1u, vph = kph;
-                auto forward = [&](int &st, uint32_t &ph) {
-                    st += step;
-                    if (st >= ST) {
-                        st -= ST;
+                // the next blocks' full barriers and phases
+                const int c0 = cb + (both ? 0 : g);
+                int kf = c0 % (2 * ST), vf = kf;
+                uint32_t kph = (uint32_t)(c0 / (2 * ST)) & 1u, vph = kph;
+                auto forward = [&](int &f, uint32_t &ph) {
+                    f += step;
+                    if (f >= 2 * ST) {
+                        f -= 2 * ST;
                         ph ^= 1;
                     }
                 };
@@ -486,8 +494,9 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 auto issue_s = [&](int k) -> bool {
                     const int j = jb + k;
                     const uint32_t d = t_s + TR_KB * (j & 1);
-                    const uint64_t kd = dK + kst * (C::KV_BYTES >> 4);
-                    if (!tr_wait(&k_full[kst], kph)) return false;
+                    const int st = kf >= ST ? kf - ST : kf;
+                    const uint64_t kd = dK + st * (C::KV_BYTES >> 4);
+                    if (!tr_wait(&k_full[kf], kph)) return false;
                     tc_fence_after();
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ks++) {  // 16 dims: 16 rows of the dim-major pages
@@ -497,16 +506,17 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                         if (C::LO) umma_f16_desc(d, dq + (C::Q_BYTES >> 4) + qo, db, IDESC_S, 1u);
                     }
                     umma_commit(&s_full[g][j & 1]);
-                    release(&k_empty[kst]);
-                    forward(kst, kph);
+                    release(&k_empty[st]);
+                    forward(kf, kph);
                     if (k + 1 == nj) umma_commit(&q_empty);
                     return true;
                 };
                 auto issue_o = [&](int k) -> bool {
                     const int j = jb + k;
                     const uint32_t p = t_s + TR_KB * (j & 1);
-                    const uint64_t vd = dV + vst * (C::KV_BYTES >> 4);
-                    if (!tr_wait(&v_full[vst], vph)) return false;
+                    const int st = vf >= ST ? vf - ST : vf;
+                    const uint64_t vd = dV + st * (C::KV_BYTES >> 4);
+                    if (!tr_wait(&v_full[vf], vph)) return false;
                     if (k == 0 && seg > 0 && !tr_wait(&o_free, (uint32_t)(seg - 1) & 1u)) return false;
                     if (!tr_wait(&p_full[g][j & 1], (uint32_t)(j >> 1) & 1u)) return false;
                     tc_fence_after();
@@ -517,8 +527,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                         if (C::LO) umma_f16_tmem(t_o, p + 32 + 8 * ks, db, IDESC_O, 1u);
                     }
                     umma_commit(&o_done[g][j & 1]);
-                    release(&v_empty[vst]);
-                    forward(vst, vph);
+                    release(&v_empty[st]);
+                    forward(vf, vph);
                     return true;
                 };
                 ok = tr_wait(&q_full, (uint32_t)seg & 1u);
@@ -821,7 +831,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     // them get back at the end (s_odd).  (With two tiles both groups do it, each before its own
                     // product: they write the same values, and the flag before them.)
                     const int st = c % ST;
-                    if (!(ok = tr_wait(&v_full[st], (uint32_t)(c / ST) & 1u))) break;
+                    if (!(ok = tr_wait(&v_full[c % (2 * ST)], (uint32_t)(c / (2 * ST)) & 1u))) break;
                     for (int i = threadIdx.x & 127; i < (int)C::KV_BYTES / 16; i += 128) {
                         const int t = (i >> 3) & 63;
                         uint4 *cell = reinterpret_cast<uint4 *>(sV + st * C::KV_BYTES) + i;

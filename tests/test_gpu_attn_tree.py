@@ -284,3 +284,26 @@ def test_same_bits_every_time_on_streams_and_in_graphs(fbctx, torch_cuda):
             assert np.array_equal(c.out.double().cpu().numpy(), p)
     for ctx in ctxs:
         assert ctx.error_word() == 0
+
+
+@pytest.mark.parametrize("kind,page,qheads", [("f16", 32, 32), ("f32", 64, 32), ("bf16", 64, 64)])
+def test_same_bits_over_many_runs(fbctx, torch_cuda, kind, page, qheads):
+    """Unequal lengths whose one-tile groups start on every ring stage: keys that arrive out of order change nothing."""
+    torch = torch_cuda
+    rng = np.random.default_rng(16)
+    new = [int(n) for n in rng.integers(1, 34, 12)]
+    B = Batch(rng, new, [n + int(x) for n, x in zip(new, rng.integers(60, 5000, 12))], 8, 128, page)
+    qd, q = rounded(torch, rng.normal(0, 1, (B.total, qheads, 128)), kind)
+    mask = tree_mask(rng, new, 2)
+    c = Call(torch, fbctx, B, qd, mask, kind, qheads, words=2)
+    first = c.result(0.09)
+    assert np.isfinite(first).all()
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    want = c.out.clone()
+    for i in range(150):
+        c.out.fill_(7.0)
+        if i % 3 == 0:
+            flush.fill_(i)  # keys from memory one time, from L2 another
+        c.go(0.09)
+        assert torch.equal(c.out, want), f"run {i}"
+    assert fbctx.error_word() == 0
