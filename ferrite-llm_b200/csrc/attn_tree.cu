@@ -22,12 +22,13 @@
 //
 // A CTA, 12 warps: two softmax groups of 4 warps (thread = row), 8 and 10 TMA
 // copies of K and V pages, 9 and 11 issue tcgen05.mma for a group each (9 owns the
-// tensor memory).  With
-// more than 128 rows each softmax group has a tile and both read the same keys;
-// otherwise they take the blocks of one tile in turn, each with its own running
-// maximum, sum and accumulator, merged at the end.  Either way one group's
-// products run under the other's exponentials, which no single chain of blocks
-// could hide.  The dim-major K pages and token-major V pages land in shared
+// tensor memory).  For 16-bit
+// results: with more than 128 rows each softmax group has a tile and both read
+// the same keys; otherwise they take the blocks of one tile in turn, each with its
+// own running maximum, sum and accumulator, merged at the end.  Either way one
+// group's products run under the other's exponentials, which no single chain of
+// blocks could hide.  For f32 results: one tile, one group takes the exponentials
+// and the other the products (below).  The dim-major K pages and token-major V pages land in shared
 // memory as the MN-major operands of S = Q K^T and O += P V; the probabilities
 // replace the scores in tensor memory and are the A operand from there.  Scores
 // have two buffers a group.  The roles run on through the CTA's groups: the next
@@ -39,8 +40,13 @@
 // most 2^15).  For f32 results they are fp16 high + low parts too, 22 bits down
 // to 2^-21 of the largest; for f16 and bf16 results the high part alone, whose
 // half step of 2^-12 averages out over the keys below the result's own rounding.
-// Products and sums are f32.  The accumulator is rescaled only when a row's
-// maximum grows by more than 8 (log 2 units).
+// Products and sums are f32.  The tensor core truncates its sums, by 2^-25 of
+// them on average at each instruction, always towards zero: over 100 blocks that
+// is 10^-5 (7.4e-6 measured in the 2-norm at 30000 keys), nothing beside a 16-bit
+// result's rounding, but not f32's.  So f32 results have each block's product
+// start from zero and the second group adds it to its registers, a rounded FMA an
+// element (6.6e-7 there).  Where the tensor core does accumulate, the sums are
+// rescaled only when a row's maximum grows by more than 8 (log 2 units).
 #include <math.h>
 
 #include <type_traits>
@@ -64,6 +70,7 @@ struct TreeArgs {
     uint64_t inv_group;  // ceil(2^32 / group)
     int split;      // 1: units are key blocks, 0: whole groups
     int ctas;       // CTAs of the attention kernel
+    int grows;      // rows a group: 128 (f32) or 256
     int rows_cap;   // row capacity of a partial (multiple of 32, <= 256)
     float *part;    // [2 ctas] partials of (head_dim + 2) rows_cap floats
     float scale;
@@ -72,7 +79,7 @@ struct TreeArgs {
 };
 
 constexpr int TR_ROWS = 128;      // rows a tile (MMA M)
-constexpr int TR_PAIR = 256;      // rows a group: two tiles
+constexpr int TR_PAIR = 256;      // rows a group at most: two tiles
 constexpr int TR_KB = 64;         // keys a block
 constexpr int TR_WHOLE = 4;
 constexpr int TR_THREADS = 384;
@@ -115,10 +122,10 @@ template <typename T> __device__ __forceinline__ void tr_store8(T *p, bool vec, 
 }
 
 // One sequence of the batch: its new rows, key blocks, row groups a kv head (the
-// last of `weight` units a block, the others of two).  A sequence left out has
+// last of `weight` units a block, the others of `full`).  A sequence left out has
 // none.
 struct TreeSeq {
-    int off, n, len, blocks, pairs, weight;
+    int off, n, len, blocks, pairs, weight, full;
     __device__ __forceinline__ bool load(const TreeArgs &A, int b) {
         off = A.offsets[b];
         n = A.offsets[b + 1] - off;
@@ -127,13 +134,14 @@ struct TreeSeq {
         if (!ok) n = len = 0;
         blocks = (len + TR_KB - 1) / TR_KB;
         const int rows = n * A.group;
-        pairs = (rows + TR_PAIR - 1) / TR_PAIR;
-        weight = rows - (pairs - 1) * TR_PAIR > TR_ROWS ? 2 : 1;
+        full = A.grows / TR_ROWS;
+        pairs = (rows + A.grows - 1) / A.grows;
+        weight = rows - (pairs - 1) * A.grows > TR_ROWS ? 2 : 1;
         return ok;
     }
     __device__ __forceinline__ int per(const TreeArgs &A) const { return A.split ? blocks : 1; }
     __device__ __forceinline__ int head_units(const TreeArgs &A) const {
-        return pairs > 0 ? (2 * (pairs - 1) + weight) * per(A) : 0;
+        return pairs > 0 ? (full * (pairs - 1) + weight) * per(A) : 0;
     }
     __device__ __forceinline__ int units(const TreeArgs &A) const { return head_units(A) * A.n_kv; }
 };
@@ -148,10 +156,10 @@ __device__ __forceinline__ int tree_total(const TreeArgs &A, int lane, int from,
     }
     return total;
 }
-// A CTA's share; the join kernel derives the same one.  With split at least two
-// units, so that none lies inside a block of two.
+// A CTA's share; the join kernel derives the same one.  With split and blocks of
+// two units at least two, so that none lies inside such a block.
 __device__ __forceinline__ int tree_quota(const TreeArgs &A, int total) {
-    return max(A.split ? 2 : 1, (total + A.ctas - 1) / A.ctas);
+    return max(A.split && A.grows > TR_ROWS ? 2 : 1, (total + A.ctas - 1) / A.ctas);
 }
 
 // The segments of a CTA's share: consecutive blocks of one row group.  A block
@@ -208,6 +216,7 @@ struct TreeWalk {
             s.blocks = __shfl_sync(0xffffffffu, first.blocks, b);
             s.pairs = __shfl_sync(0xffffffffu, first.pairs, b);
             s.weight = __shfl_sync(0xffffffffu, first.weight, b);
+            s.full = A.grows / TR_ROWS;
         } else {
             s.load(A, b);
         }
@@ -215,12 +224,12 @@ struct TreeWalk {
         int r = u0 - base;
         h = r / hu;
         r -= h * hu;
-        pair = min(r / (2 * per), s.pairs - 1);
-        r -= pair * 2 * per;
+        pair = min(r / (s.full * per), s.pairs - 1);
+        r -= pair * s.full * per;
         span(A, r);
         return blk0 < blk1 || next(A);
     }
-    __device__ __forceinline__ int weight() const { return pair < s.pairs - 1 ? 2 : s.weight; }
+    __device__ __forceinline__ int weight() const { return pair < s.pairs - 1 ? s.full : s.weight; }
     __device__ __forceinline__ void span(const TreeArgs &A, int r) {
         const int w = weight(), take = min(left, w * s.per(A) - r);
         if (A.split) {
@@ -249,8 +258,8 @@ struct TreeWalk {
         } while (blk0 >= blk1);
         return true;
     }
-    __device__ __forceinline__ int row0() const { return pair * TR_PAIR; }
-    __device__ __forceinline__ int rows(const TreeArgs &A) const { return min(TR_PAIR, s.n * A.group - row0()); }
+    __device__ __forceinline__ int row0(const TreeArgs &A) const { return pair * A.grows; }
+    __device__ __forceinline__ int rows(const TreeArgs &A) const { return min(A.grows, s.n * A.group - row0(A)); }
     __device__ __forceinline__ bool both() const { return weight() == 2; }  // two tiles
     // blocks that softmax group g works on
     __device__ __forceinline__ int jobs(int g) const { return both() ? blk1 - blk0 : (blk1 - blk0 + 1 - g) / 2; }
@@ -291,14 +300,15 @@ __device__ __forceinline__ uint32_t tree_visible(const TreeArgs &A, const TreeSe
 
 template <typename T, int HD> struct TreeCfg {
     static constexpr bool LO = sizeof(T) == 4;          // f32: q and the probabilities have low parts
-    static constexpr int ST = HD == 128 && LO ? 3 : 5;  // K and V stages
+    static constexpr int ST = HD == 128 && LO ? 4 : 5;  // K and V stages
     static constexpr uint32_t Q_BYTES = TR_ROWS * HD * 2;
     static constexpr uint32_t TILE_BYTES = (LO ? 2 : 1) * Q_BYTES;  // a tile's queries
     static constexpr uint32_t KV_BYTES = TR_KB * HD * 2;            // one block of K or V
-    static constexpr size_t SMEM = 1024 + 2 * (size_t)TILE_BYTES + 2 * ST * (size_t)KV_BYTES;
+    static constexpr int TILES = LO ? 1 : 2;  // row tiles a group
+    static constexpr size_t SMEM = 1024 + TILES * (size_t)TILE_BYTES + 2 * ST * (size_t)KV_BYTES;
     static_assert(SMEM + 2048 <= 227 * 1024, "tree attention stages must fit");
 };
-constexpr uint32_t TR_TMEM_COLS = 512;  // scores (group, buffer) at 128 g + 64 buffer, O of group g at 256 + HD g
+constexpr uint32_t TR_TMEM_COLS = 512;  // scores (group, buffer) at 128 g + 64 buffer, O of group (f32: buffer) g at 256 + HD g
 constexpr uint32_t TR_O_COL = 256;
 
 // Bounded wait (~1 s) for waits that are short in the steady state: polls without the suspension of
@@ -343,8 +353,11 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     __shared__ uint64_t k_full[2 * ST], k_empty[ST], v_full[2 * ST], v_empty[ST];
     __shared__ uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [group][buffer]
     __shared__ uint64_t q_full, q_empty, o_free, fin[2], go, pair_bar[4];
+    // f32: a block's product has been read; a segment's (max, sum) are there, have been read ([parity])
+    __shared__ uint64_t o_read[C::LO ? 2 : 1], ml_full[C::LO ? 2 : 1], ml_read[C::LO ? 2 : 1];
     __shared__ uint32_t s_tmem;
-    __shared__ float2 s_ml[TR_ROWS];  // group 1's (max, sum) of one tile's rows
+    __shared__ float2 s_ml[C::LO ? 2 : 1][TR_ROWS];  // (max, sum) of a tile's rows: of group 1; f32: [segment parity]
+    __shared__ float s_al[C::LO ? 4 : 1][TR_ROWS];   // f32: [job mod 4] what the rows' sums so far are scaled by
     __shared__ uint8_t s_qe[2][TR_PAIR];  // [segment parity] exponent field of a row's largest query value
     __shared__ int s_abort_raw, s_odd_raw[2];
     __shared__ uint8_t s_skip_raw[16];
@@ -353,17 +366,17 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
     volatile uint8_t *s_skip = s_skip_raw;  // block: halves whose page id is outside the pool
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *sQ = sm;                      // [tile][high parts, low parts]
-    uint8_t *sK = sQ + 2 * C::TILE_BYTES;  // [stage]
-    uint8_t *sV = sK + ST * C::KV_BYTES;   // [stage]: dims 0..63, then 64..127
+    uint8_t *sQ = sm;                             // [tile][high parts, low parts]
+    uint8_t *sK = sQ + C::TILES * C::TILE_BYTES;  // [stage]
+    uint8_t *sV = sK + ST * C::KV_BYTES;          // [stage]: dims 0..63, then 64..127
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; i++) {
             mbar_init(&k_full[i], 1);
             mbar_init(&k_full[ST + i], 1);
-            mbar_init(&k_empty[i], 2);  // (both MMA warps)
+            mbar_init(&k_empty[i], C::LO ? 1 : 2);  // (both MMA warps)
             mbar_init(&v_full[i], 1);
             mbar_init(&v_full[ST + i], 1);
-            mbar_init(&v_empty[i], 2);
+            mbar_init(&v_empty[i], C::LO ? 1 : 2);
         }
         for (int i = 0; i < 4; i++) {
             mbar_init(&s_full[i >> 1][i & 1], 1);
@@ -373,7 +386,12 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         }
         mbar_init(&q_full, 8);
         mbar_init(&go, 8);
-        mbar_init(&q_empty, 2);
+        mbar_init(&q_empty, C::LO ? 1 : 2);
+        for (int i = 0; i < (C::LO ? 2 : 1); i++) {
+            mbar_init(&o_read[i], 4);
+            mbar_init(&ml_full[i], 4);
+            mbar_init(&ml_read[i], 4);
+        }
         mbar_init(&o_free, 8);
         mbar_init(&fin[0], 1);
         mbar_init(&fin[1], 1);
@@ -459,7 +477,68 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             for (int k = c > ST ? c - ST : 0; k < c; k++)
                 mbar_wait_bounded(&full[k % (2 * ST)], (uint32_t)(k / (2 * ST)) & 1u);
         }
-    } else if (warp == 9 || warp == 11) {
+    } else if (C::LO && warp >= 8) {
+        // ---- f32, MMA issue (warp 9): the next block's scores before this one's product, which starts from zero in
+        // one of two buffers: the tensor core truncates every addition to an accumulator (2^-24 of it), which over a
+        // long context would add up, so the blocks are summed with rounding elsewhere.
+        if (warp == 9 && lane == 0) {
+            const uint64_t dQ = umma_desc_sw128(smem_u32(sQ)), dV = umma_desc_mn_sw128(smem_u32(sV), TR_KB * 128, 1024);
+            const uint64_t dK = PAGE == 64 ? umma_desc_mn_sw128(smem_u32(sK), C::KV_BYTES, 1024)
+                                           : umma_desc_mn_sw64(smem_u32(sK), HD * PAGE * 2, 512);
+            int j = 0, seg = 0;  // blocks of the segments before this one
+            bool ok = true;
+            auto issue_s = [&](int c) -> bool {
+                const int st = c % ST, f = c % (2 * ST);
+                const uint32_t d = tmem + TR_KB * (c & 1);
+                const uint64_t kd = dK + st * (C::KV_BYTES >> 4);
+                if (!tr_wait(&k_full[f], (uint32_t)(c / (2 * ST)) & 1u)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int i = 0; i < 2 * (HD / 16); i++) {  // the low parts first: small sums lose less
+                    const int ks = i % (HD / 16);
+                    const uint32_t qo = ((uint32_t)(ks >> 2) * (TR_ROWS * 128) + (uint32_t)(ks & 3) * 32 +
+                                         (i < HD / 16 ? C::Q_BYTES : 0)) >> 4;
+                    umma_f16_desc(d, dQ + qo, kd + ks * (16 * PAGE * 2 >> 4), IDESC_S, i > 0 ? 1u : 0u);
+                }
+                umma_commit(&s_full[0][c & 1]);
+                umma_commit(&k_empty[st]);
+                return true;
+            };
+            auto issue_o = [&](int c) -> bool {
+                const int st = c % ST, f = c % (2 * ST);
+                const uint32_t p = tmem + TR_KB * (c & 1), d = tmem + TR_O_COL + HD * (c & 1);
+                const uint64_t vd = dV + st * (C::KV_BYTES >> 4);
+                if (!tr_wait(&v_full[f], (uint32_t)(c / (2 * ST)) & 1u)) return false;
+                if (c >= 2 && !tr_wait(&o_read[c & 1], (uint32_t)((c >> 1) - 1) & 1u)) return false;
+                if (!tr_wait(&p_full[0][c & 1], (uint32_t)(c >> 1) & 1u)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int i = 0; i < 2 * (TR_KB / 16); i++) {  // 16 keys: 8 columns of fp16 pairs; low parts first
+                    const int ks = i % (TR_KB / 16);
+                    umma_f16_tmem(d, p + (i < TR_KB / 16 ? 32 : 0) + 8 * ks, vd + ks * (2048 >> 4), IDESC_O, i > 0 ? 1u : 0u);
+                }
+                umma_commit(&o_done[0][c & 1]);
+                umma_commit(&v_empty[st]);
+                return true;
+            };
+            do {
+                const int nb = w.blk1 - w.blk0;
+                ok = tr_wait(&q_full, (uint32_t)seg & 1u) && issue_s(j);
+                if (ok && nb == 1) umma_commit(&q_empty);
+                for (int k = 0; ok && k < nb && !s_abort; k++, j++) {
+                    if (k + 1 < nb) {
+                        ok = issue_s(j + 1);
+                        if (k + 2 == nb) umma_commit(&q_empty);
+                    }
+                    ok = ok && issue_o(j);
+                }
+                seg++;
+            } while (ok && !s_abort && w.next(A));
+            if (!ok) s_abort = 1;
+            umma_commit(&fin[0]);  // every MMA issued has completed before TMEM is released
+            mbar_wait_bounded(&fin[0], 0);
+        }
+    } else if (!C::LO && (warp == 9 || warp == 11)) {
         // ---- MMA issue for group g: its next scores before its products of this block.  (The tensor core runs one
         // thread's products in order: a score buffer is rewritten after the product that read it.)
         if (lane == 0) {
@@ -553,20 +632,20 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         uint32_t npair = 0;  // uses of pair_bar[qd]
         bool ok = true;
         int cb = 0, jb = 0, seg = 0;  // blocks and this group's jobs of the segments before
-        // The group's queries as fp16 parts scaled by 2^-e: HD / 8 lanes a row, the 8 warps share the rows.  f32: two
+        // The group's queries as fp16 parts scaled by 2^-e: HD / 8 lanes a row, the first 8 (or 4) warps share the rows.  f32: two
         // batches of loads through registers (128 KB for two tiles: L2's rate, shared by all CTAs, bounds them).  16-bit:
         // copied as they are into their places, all copies in flight together, and (bf16) turned in place by the
         // thread that copied them, in rolled loops: code that runs once a segment arrives more slowly than it executes.
-        auto load_q = [&](const TreeWalk &t, int sg) {
+        auto load_q = [&](const TreeWalk &t, int sg, int warps) {
             constexpr int LPR = HD / 8, RPI = 32 / LPR;
-            const int rows = t.rows(A), each = (t.both() ? TR_PAIR : TR_ROWS) / 8, d = (lane % LPR) * 8;
+            const int rows = t.rows(A), each = (t.both() ? TR_PAIR : TR_ROWS) / warps, d = (lane % LPR) * 8;
             const T *base = static_cast<const T *>(A.q) + (int64_t)t.s.off * A.qt + (int64_t)t.h * A.group * HD + d;
             auto place = [&](int rr) {
                 return sQ + (rr >> 7) * C::TILE_BYTES + (uint32_t)(d >> 6) * (TR_ROWS * 128) +
                        sw128_off(rr & 127, (d >> 3) & 7);
             };
             auto source = [&](int rr) {
-                const int row = t.row0() + rr, tok = tree_token(A, row);
+                const int row = t.row0(A) + rr, tok = tree_token(A, row);
                 return base + (int64_t)tok * A.qt + (int64_t)(row - tok * A.group) * HD;
             };
             auto turn = [&](float (&x)[8], int rr, uint4 &hi, uint4 &lo) {
@@ -641,9 +720,215 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&q_full);
+                if (warps == 4) mbar_arrive(&q_full);  // (8 arrivals)
                 if (sg == 0) mbar_arrive(&go);
             }
         };
+        // a row's score unit, |scale| log2(e) 2^e (not 0: masked scores stay -inf)
+        auto unit_of = [&](int sg, int rr) {
+            float u = __fmul_rn(fabsf(A.scale), 1.4426950408889634f);
+            if constexpr (!std::is_same<T, __half>::value)
+                u = __fmul_rn(u, __uint_as_float((uint32_t)(127 + tree_shift(s_qe[sg & 1][rr])) << 23));
+            return fmaxf(u, 1e-37f);
+        };
+        // Values of block c that some row must not see: 0 * NaN would reach it.  Behind the last key and in skipped
+        // pages all are zeroed; at new rows the non-finite ones, which the rows that see them get back at the end
+        // (s_odd).  By the 128 threads of a softmax group.  (With two tiles both groups do it, each before its own
+        // product: they write the same values, and the flag before them.)
+        auto mend_values = [&](const TreeWalk &t, int c, int p0, int skip, int sg) -> bool {
+            const int st = c % ST, pre = t.s.len - t.s.n;
+            if (!tr_wait(&v_full[c % (2 * ST)], (uint32_t)(c / (2 * ST)) & 1u)) return false;
+            for (int i = threadIdx.x & 127; i < (int)C::KV_BYTES / 16; i += 128) {
+                const int k = (i >> 3) & 63;
+                uint4 *cell = reinterpret_cast<uint4 *>(sV + st * C::KV_BYTES) + i;
+                if (p0 + k >= t.s.len || ((skip >> (k >> 5)) & 1)) {
+                    *cell = make_uint4(0, 0, 0, 0);
+                } else if (p0 + k >= pre) {
+                    uint4 v = *cell;
+                    uint32_t *e = reinterpret_cast<uint32_t *>(&v);
+                    bool odd = false;
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; i4++) {
+                        if ((e[i4] & 0x7C00u) == 0x7C00u) {
+                            e[i4] &= 0xffff0000u;
+                            odd = true;
+                        }
+                        if ((e[i4] & 0x7C000000u) == 0x7C000000u) {
+                            e[i4] &= 0xffffu;
+                            odd = true;
+                        }
+                    }
+                    if (odd) {
+                        s_odd[sg & 1] = sg + 1;
+                        __threadfence_block();
+                        *cell = v;
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            return true;
+        };
+        // What a row gets back of the non-finite values it sees: dimensions d0 .. d0 + 31.
+        auto give_back = [&](const TreeWalk &t, int tok, int d0, float (&o)[32]) {
+            const int pre = t.s.len - t.s.n;
+            for (int i = max(0, t.blk0 * TR_KB - pre); i < min(t.s.n, t.blk1 * TR_KB - pre); i++) {
+                const int p = pre + i, page = A.bt[(int64_t)t.b * A.max_pages + p / PAGE];
+                if (page < 0 || page >= A.num_pages || !(tree_visible(A, t.s, tok, p) & 1)) continue;
+                const __half *v = A.vpool + (((int64_t)page * A.n_kv + t.h) * PAGE + p % PAGE) * HD + d0;
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    const float x = __half2float(v[e]);
+                    if (!isfinite(x)) o[e] = __fadd_rn(o[e], x);
+                }
+            }
+        };
+        auto hide = [&](const TreeWalk &t, int tok, int p0, int skip, uint32_t (&sv)[64]) {  // scores of unseen keys
+            const uint32_t v0 = skip & 1 ? 0u : tree_visible(A, t.s, tok, p0);
+            const uint32_t v1 = skip & 2 ? 0u : tree_visible(A, t.s, tok, p0 + 32);
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                if (!((v0 >> i) & 1)) sv[i] = 0xff800000u;  // -inf
+                if (!((v1 >> i) & 1)) sv[32 + i] = 0xff800000u;
+            }
+        };
+        auto largest = [&](const uint32_t (&sv)[64]) {
+            float b4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int t = 0; t < 64; t++) b4[t & 3] = fmaxf(b4[t & 3], __uint_as_float(sv[t]));
+            return fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
+        };
+        // p = 2^(s u - m + 7) as fp16 pairs over the scores, low parts behind the high ones; their sum
+        auto exponentials = [&](const uint32_t (&sv)[64], float u, float m, uint32_t t_b) {
+            const float ref = __fsub_rn(TR_LIFT, m);
+            float l4[4] = {0.f, 0.f, 0.f, 0.f};
+            uint32_t hi[32], lo[32];
+#pragma unroll
+            for (int t = 0; t < 32; t++) {
+                const float pa = exp2_approx(__fmaf_rn(__uint_as_float(sv[2 * t]), u, ref));
+                const float pb = exp2_approx(__fmaf_rn(__uint_as_float(sv[2 * t + 1]), u, ref));
+                l4[t & 3] = __fadd_rn(l4[t & 3], __fadd_rn(pa, pb));
+                const __half2 h2 = __floats2half2_rn(pa, pb);
+                hi[t] = *reinterpret_cast<const uint32_t *>(&h2);
+                if (C::LO) {
+                    const float2 hf = __half22float2(h2);
+                    const __half2 q2 = __floats2half2_rn(__fsub_rn(pa, hf.x), __fsub_rn(pb, hf.y));
+                    lo[t] = *reinterpret_cast<const uint32_t *>(&q2);
+                }
+            }
+            tmem_st32(t_b, hi);
+            if (C::LO) tmem_st32(t_b + 32, lo);
+            return __fadd_rn(__fadd_rn(l4[0], l4[1]), __fadd_rn(l4[2], l4[3]));
+        };
+        if constexpr (C::LO) {
+            // ---- f32: group 0 turns scores into probabilities, group 1 sums the blocks' products in registers
+            load_q(w, 0, 8);
+            if (g == 0) {
+                for (;; seg++) {
+                    const int nb = w.blk1 - w.blk0, pre = w.s.len - w.s.n, rows = w.rows(A);
+                    const bool active = rows > 32 * qd;
+                    const int row = w.row0(A) + min(r, rows - 1), tok = tree_token(A, row);
+                    if (!(ok = tr_wait(&q_full, (uint32_t)seg & 1u))) break;
+                    // (what segment seg - 2 left for group 1 has been taken)
+                    if (seg >= 2 && !(ok = tr_wait(&ml_read[seg & 1], (uint32_t)((seg >> 1) - 1) & 1u))) break;
+                    const float u = unit_of(seg, r);
+                    float m = TR_NONE, l = 0.f;
+                    for (int k = 0; k < nb; k++) {
+                        const int j = jb + k, p0 = (w.blk0 + k) * TR_KB;
+                        const uint32_t t_b = lt + TR_KB * (j & 1);
+                        if (!(ok = tr_wait(&s_full[0][j & 1], (uint32_t)(j >> 1) & 1u))) break;
+                        tc_fence_after();
+                        const int skip = s_skip[j & 15];
+                        const bool odd = p0 + TR_KB > pre || skip;
+                        if (active) {
+                            uint32_t sv[64];
+                            tmem_ld64(t_b, sv);
+                            if (odd) hide(w, tok, p0, skip, sv);
+                            const float mn = fmaxf(m, __fmul_rn(largest(sv), u));
+                            const float al = exp2f(__fsub_rn(m, mn));
+                            m = mn;
+                            // (four blocks in flight at most: the product of block j - 2 waits for the reader of j - 4)
+                            s_al[j & 3][r] = al;
+                            l = __fmaf_rn(l, al, exponentials(sv, u, m, t_b));
+                        }
+                        if (odd && !(ok = mend_values(w, j, p0, skip, seg))) break;
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_full[0][j & 1]);
+                    }
+                    if (!ok) break;
+                    s_ml[seg & 1][r] = make_float2(m, l);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ml_full[seg & 1]);
+                    jb += nb;
+                    // the next segment's queries, once this one's last scores are out
+                    if (!w.next(A) || !(ok = tr_wait(&q_empty, (uint32_t)seg & 1u))) break;
+                    load_q(w, seg + 1, 4);
+                }
+            } else {
+                float acc[HD];
+                for (;; seg++) {
+                    const int nb = w.blk1 - w.blk0, rows = w.rows(A);
+                    const bool active = rows > 32 * qd;
+                    const int row = w.row0(A) + min(r, rows - 1), tok = tree_token(A, row);
+#pragma unroll
+                    for (int e = 0; e < HD; e++) acc[e] = 0.f;
+                    for (int k = 0; k < nb; k++) {
+                        const int j = jb + k;
+                        if (!(ok = tr_wait(&o_done[0][j & 1], (uint32_t)(j >> 1) & 1u))) break;
+                        tc_fence_after();
+                        if (active) {
+                            const float al = s_al[j & 3][r];
+#pragma unroll
+                            for (int i = 0; i < HD / 16; i++) {
+                                uint32_t ov[16];
+                                tmem_ld16(lt + TR_O_COL + HD * (j & 1) + 16 * i, ov);
+#pragma unroll
+                                for (int e = 0; e < 16; e++)
+                                    acc[16 * i + e] = __fmaf_rn(acc[16 * i + e], al, __uint_as_float(ov[e]));
+                            }
+                        }
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&o_read[j & 1]);
+                    }
+                    if (!ok) break;
+                    jb += nb;
+                    // ---- this segment's rows
+                    if (!(ok = tr_wait(&ml_full[seg & 1], (uint32_t)(seg >> 1) & 1u))) break;
+                    const float2 ml = s_ml[seg & 1][r];
+                    const bool odd = s_odd[seg & 1] == seg + 1, whole = !A.split || w.whole();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ml_read[seg & 1]);
+                    const float inv = ml.y > 0.f ? __fdiv_rn(1.f, ml.y) : 0.f;
+                    float *part = A.part + (int64_t)(2 * blockIdx.x + (w.blk0 == 0)) * (HD + 2) * A.rows_cap;
+                    T *orow = static_cast<T *>(A.out) + (int64_t)(w.s.off + tok) * A.ot +
+                              (int64_t)(w.h * A.group + row - tok * A.group) * HD;
+                    if (active) {
+#pragma unroll
+                        for (int d0 = 0; d0 < HD; d0 += 32) {
+                            float (&o)[32] = *reinterpret_cast<float (*)[32]>(&acc[d0]);
+                            if (odd) give_back(w, tok, d0, o);
+                            if (!whole) {
+#pragma unroll
+                                for (int i = 0; i < 32; i += 4)  // [dim / 4][row]: a warp stores 512 bytes at once
+                                    reinterpret_cast<float4 *>(part)[(int64_t)((d0 + i) >> 2) * A.rows_cap + r] =
+                                        make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                            } else if (r < rows) {
+#pragma unroll
+                                for (int i = 0; i < 32; i += 8) {
+                                    float y[8];
+#pragma unroll
+                                    for (int e = 0; e < 8; e++) y[e] = __fmul_rn(o[i + e], inv);
+                                    tr_store8(orow + d0 + i, A.ovec, y);
+                                }
+                            }
+                        }
+                        if (!whole) reinterpret_cast<float2 *>(part + (int64_t)HD * A.rows_cap)[r] = ml;
+                    }
+                    if (!w.next(A)) break;
+                }
+            }
+        } else {
         // A pass: the next segment's queries go in once this one's last scores are out, then this one's rows are
         // written, then the next one's blocks.
         TreeWalk nw = w;
@@ -653,11 +938,10 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         for (;;) {
             if (more) {
                 if (!first && !(ok = tr_wait(&q_empty, (uint32_t)seg & 1u))) break;
-                load_q(nw, first ? 0 : seg + 1);
+                load_q(nw, first ? 0 : seg + 1, 8);
             }
             if (!first) {
                 const bool both = w.both();
-                const int pre = w.s.len - w.s.n;
                 // ---- this segment's rows, once the last products have landed
                 if (nj > 0) {
                     const int j = jb + nj - 1;
@@ -668,12 +952,12 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 float w0 = 1.f, w1 = 0.f;
                 if (two) {
                     if (g == 1) {
-                        s_ml[r] = make_float2(m, l);
+                        s_ml[0][r] = make_float2(m, l);
                         tc_fence_before();
                         mbar_arrive(&pair_bar[qd]);
                     } else {
                         if (!(ok = tr_wait(&pair_bar[qd], npair & 1u))) break;
-                        const float2 o = s_ml[r];
+                        const float2 o = s_ml[0][r];
                         const float mm = fmaxf(m, o.x);
                         w0 = exp2f(__fsub_rn(m, mm));
                         w1 = exp2f(__fsub_rn(o.x, mm));
@@ -703,16 +987,12 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                                     __fmaf_rn(w1, __uint_as_float(o1[i]), __fmul_rn(w0, __uint_as_float(ov[i]))));
                         }
                         if (odd) {
-                            for (int i = max(0, w.blk0 * TR_KB - pre); i < min(w.s.n, w.blk1 * TR_KB - pre); i++) {
-                                const int p = pre + i, page = A.bt[(int64_t)w.b * A.max_pages + p / PAGE];
-                                if (page < 0 || page >= A.num_pages || !(tree_visible(A, w.s, tok, p) & 1)) continue;
-                                const __half *v = A.vpool + (((int64_t)page * A.n_kv + w.h) * PAGE + p % PAGE) * HD + d0;
+                            float o[32];
 #pragma unroll
-                                for (int e = 0; e < 32; e++) {
-                                    const float x = __half2float(v[e]);
-                                    if (!isfinite(x)) ov[e] = __float_as_uint(__fadd_rn(__uint_as_float(ov[e]), x));
-                                }
-                            }
+                            for (int e = 0; e < 32; e++) o[e] = __uint_as_float(ov[e]);
+                            give_back(w, tok, d0, o);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) ov[e] = __float_as_uint(o[e]);
                         }
                         if (!whole) {
 #pragma unroll
@@ -747,16 +1027,10 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             nj = w.jobs(g);
             tile_rows = w.rows(A) - (both ? TR_ROWS * g : 0);  // of this group's tile
             active = tile_rows > 32 * qd;
-            row = w.row0() + (both ? TR_ROWS * g : 0) + min(r, tile_rows - 1);
+            row = w.row0(A) + (both ? TR_ROWS * g : 0) + min(r, tile_rows - 1);
             tok = tree_token(A, row);
             if (!(ok = tr_wait(&q_full, (uint32_t)seg & 1u))) break;
-            // this row's score unit, |scale| log2(e) 2^e (not 0: masked scores stay -inf)
-            float sl2 = __fmul_rn(fabsf(A.scale), 1.4426950408889634f);
-            if constexpr (!std::is_same<T, __half>::value) {
-                const int e2 = tree_shift(s_qe[seg & 1][(both ? TR_ROWS * g : 0) + r]);
-                sl2 = __fmul_rn(sl2, __uint_as_float((uint32_t)(127 + e2) << 23));
-            }
-            sl2 = fmaxf(sl2, 1e-37f);
+            const float sl2 = unit_of(seg, (both ? TR_ROWS * g : 0) + r);
             m = TR_NONE;
             l = 0.f;
             for (int k = 0; k < nj; k++) {
@@ -770,19 +1044,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 if (active) {
                     uint32_t sv[64];
                     tmem_ld64(t_b, sv);
-                    if (p0 + TR_KB > pre || skip) {
-                        const uint32_t v0 = skip & 1 ? 0u : tree_visible(A, w.s, tok, p0);
-                        const uint32_t v1 = skip & 2 ? 0u : tree_visible(A, w.s, tok, p0 + 32);
-#pragma unroll
-                        for (int t = 0; t < 32; t++) {
-                            if (!((v0 >> t) & 1)) sv[t] = 0xff800000u;  // -inf
-                            if (!((v1 >> t) & 1)) sv[32 + t] = 0xff800000u;
-                        }
-                    }
-                    float b4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int t = 0; t < 64; t++) b4[t & 3] = fmaxf(b4[t & 3], __uint_as_float(sv[t]));
-                    const float bm = fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
+                    if (p0 + TR_KB > pre || skip) hide(w, tok, p0, skip, sv);
+                    const float bm = largest(sv);
                     const float mn = fmaxf(m, __fmul_rn(bm, sl2));
                     const bool need = k > 0 && mn > m + 8.f;
                     if (__any_sync(FULL, need)) {
@@ -804,69 +1067,16 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                         }
                     }
                     if (k == 0) m = mn;
-                    // p = 2^(s sl2 - m + 7): fp16 pairs over the scores, low parts behind the high ones
-                    const float ref = __fsub_rn(TR_LIFT, m);
-                    float l4[4] = {0.f, 0.f, 0.f, 0.f};
-                    uint32_t hi[32], lo[32];
-#pragma unroll
-                    for (int t = 0; t < 32; t++) {
-                        const float pa = exp2_approx(__fmaf_rn(__uint_as_float(sv[2 * t]), sl2, ref));
-                        const float pb = exp2_approx(__fmaf_rn(__uint_as_float(sv[2 * t + 1]), sl2, ref));
-                        l4[t & 3] = __fadd_rn(l4[t & 3], __fadd_rn(pa, pb));
-                        const __half2 h2 = __floats2half2_rn(pa, pb);
-                        hi[t] = *reinterpret_cast<const uint32_t *>(&h2);
-                        if (C::LO) {
-                            const float2 hf = __half22float2(h2);
-                            const __half2 q2 = __floats2half2_rn(__fsub_rn(pa, hf.x), __fsub_rn(pb, hf.y));
-                            lo[t] = *reinterpret_cast<const uint32_t *>(&q2);
-                        }
-                    }
-                    l = __fadd_rn(l, __fadd_rn(__fadd_rn(l4[0], l4[1]), __fadd_rn(l4[2], l4[3])));
-                    tmem_st32(t_b, hi);
-                    if (C::LO) tmem_st32(t_b + 32, lo);
+                    l = __fadd_rn(l, exponentials(sv, sl2, m, t_b));
                 }
-                if (p0 + TR_KB > pre || skip) {
-                    // Values that some row must not see: 0 * NaN would reach it.  Behind the last key and in
-                    // skipped pages all are zeroed; at new rows the non-finite ones, which the rows that see
-                    // them get back at the end (s_odd).  (With two tiles both groups do it, each before its own
-                    // product: they write the same values, and the flag before them.)
-                    const int st = c % ST;
-                    if (!(ok = tr_wait(&v_full[c % (2 * ST)], (uint32_t)(c / (2 * ST)) & 1u))) break;
-                    for (int i = threadIdx.x & 127; i < (int)C::KV_BYTES / 16; i += 128) {
-                        const int t = (i >> 3) & 63;
-                        uint4 *cell = reinterpret_cast<uint4 *>(sV + st * C::KV_BYTES) + i;
-                        if (p0 + t >= w.s.len || ((skip >> (t >> 5)) & 1)) {
-                            *cell = make_uint4(0, 0, 0, 0);
-                        } else if (p0 + t >= pre) {
-                            uint4 v = *cell;
-                            uint32_t *e = reinterpret_cast<uint32_t *>(&v);
-                            bool odd = false;
-#pragma unroll
-                            for (int i4 = 0; i4 < 4; i4++) {
-                                if ((e[i4] & 0x7C00u) == 0x7C00u) {
-                                    e[i4] &= 0xffff0000u;
-                                    odd = true;
-                                }
-                                if ((e[i4] & 0x7C000000u) == 0x7C000000u) {
-                                    e[i4] &= 0xffffu;
-                                    odd = true;
-                                }
-                            }
-                            if (odd) {
-                                s_odd[seg & 1] = seg + 1;
-                                __threadfence_block();
-                                *cell = v;
-                            }
-                        }
-                    }
-                    fence_proxy_async_smem();
-                }
+                if ((p0 + TR_KB > pre || skip) && !(ok = mend_values(w, c, p0, skip, seg))) break;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[g][j & 1]);
             }
             if (!ok) break;
             more = nw.next(A);
+        }
         }
         if (!ok) s_abort = 1;
     }
@@ -894,7 +1104,7 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
     const int b = blockIdx.z;
     TreeSeq s;
     s.load(A, b);
-    const int row0 = pair * TR_PAIR + 32 * slab;
+    const int row0 = pair * A.grows + 32 * slab;
     if (row0 >= s.n * A.group) return;
     // units before this sequence, and in all
     int before = 0, total = 0;
@@ -911,8 +1121,8 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
         before += __shfl_xor_sync(0xffffffffu, before, o);
     }
     const int quota = tree_quota(A, total);
-    const int wt = pair < s.pairs - 1 ? 2 : s.weight;
-    const int gs = before + blockIdx.y * s.head_units(A) + pair * 2 * s.blocks;  // the group's first unit
+    const int wt = pair < s.pairs - 1 ? s.full : s.weight;
+    const int gs = before + blockIdx.y * s.head_units(A) + pair * s.full * s.blocks;  // the group's first unit
     const int c0 = gs / quota, c1 = (gs + wt * (s.blocks - 1)) / quota;          // CTAs of its first and last block
     if (c0 == c1) return;  // written by its CTA
     const int r = 32 * slab + lane;
@@ -970,10 +1180,10 @@ struct TreePlan {
     int64_t ws;
 };
 static TreePlan tree_plan(const fb_ctx *ctx, int batch, int max_new, int n_heads, int n_kv, int head_dim,
-                          int max_seq_len) {
+                          int max_seq_len, int grows) {
     TreePlan p{};
     const int64_t rows = (int64_t)max_new * (n_heads / n_kv);
-    const int64_t pairs = (rows + TR_PAIR - 1) / TR_PAIR, blocks = (max_seq_len + TR_KB - 1) / TR_KB;
+    const int64_t pairs = (rows + grows - 1) / grows, blocks = (max_seq_len + TR_KB - 1) / TR_KB;
     const int64_t groups = pairs * n_kv * batch;
     FB_REQUIRE(2 * groups * blocks < ((int64_t)1 << 31) - 4096 && pairs <= 65535, "attn_tree: batch too large");
     FB_REQUIRE((rows + TR_PAIR) * (n_heads / n_kv) < ((int64_t)1 << 32), "attn_tree: too many rows");
@@ -981,7 +1191,7 @@ static TreePlan tree_plan(const fb_ctx *ctx, int batch, int max_new, int n_heads
     const int64_t units = 2 * groups * (p.split ? blocks : 1);
     p.ctas = (int)(units < ctx->num_sms ? units : ctx->num_sms);
     p.pairs = (int)pairs;
-    p.rows_cap = (int)(rows >= TR_PAIR ? TR_PAIR : (rows + 31) / 32 * 32);
+    p.rows_cap = (int)(rows >= grows ? grows : (rows + 31) / 32 * 32);
     p.ws = p.split ? (int64_t)2 * p.ctas * (head_dim + 2) * p.rows_cap * 4 : 0;
     return p;
 }
@@ -1021,9 +1231,13 @@ int fb_attn_tree_workspace(fb_ctx *ctx, int batch, int max_new, int n_heads, int
     return guarded([&] {
         check_tree_shape(batch, max_new, n_heads, n_kv_heads, head_dim, page_size, max_seq_len);
         FB_REQUIRE(ctx && bytes, "null argument");
-        *bytes = batch && max_new && max_seq_len
-                     ? tree_plan(ctx, batch, max_new, n_heads, n_kv_heads, head_dim, max_seq_len).ws
-                     : 0;
+        *bytes = 0;
+        if (batch && max_new && max_seq_len)  // (of any dtype)
+            for (int grows : {TR_ROWS, TR_PAIR}) {
+                const int64_t ws =
+                    tree_plan(ctx, batch, max_new, n_heads, n_kv_heads, head_dim, max_seq_len, grows).ws;
+                *bytes = ws > *bytes ? ws : *bytes;
+            }
     });
 }
 
@@ -1077,7 +1291,8 @@ int fb_attn_tree(fb_ctx *ctx, int dtype, const void *q_dev, int64_t q_token_stri
         A.max_seq = max_seq_len;
         A.scale = scale;
         A.err = ctx->err_word;
-        const TreePlan plan = tree_plan(ctx, batch, max_new, n_heads, n_kv_heads, head_dim, max_seq_len);
+        const int grows = dtype == FB_F32 ? TR_ROWS : TR_PAIR;
+        const TreePlan plan = tree_plan(ctx, batch, max_new, n_heads, n_kv_heads, head_dim, max_seq_len, grows);
         FB_REQUIRE(plan.ws == 0 || (workspace_dev && workspace_bytes >= plan.ws && ((uintptr_t)workspace_dev & 15) == 0),
                    "attn_tree: the workspace must be 16-byte aligned and hold fb_attn_tree_workspace bytes (" +
                        std::to_string(plan.ws) + ")");
@@ -1085,6 +1300,7 @@ int fb_attn_tree(fb_ctx *ctx, int dtype, const void *q_dev, int64_t q_token_stri
         A.inv_group = (((uint64_t)1 << 32) + A.group - 1) / A.group;
         A.split = plan.split;
         A.ctas = plan.ctas;
+        A.grows = grows;
         A.rows_cap = plan.rows_cap;
         A.part = static_cast<float *>(workspace_dev);
         const int V = (int)(16 / esz);

@@ -307,3 +307,13 @@ def test_same_bits_over_many_runs(fbctx, torch_cuda, kind, page, qheads):
         c.go(0.09)
         assert torch.equal(c.out, want), f"run {i}"
     assert fbctx.error_word() == 0
+
+
+def test_sums_of_long_contexts(fbctx, torch_cuda):
+    """Some seventy blocks of keys to an SM: what a matrix instruction drops of a running sum must not add up over them."""
+    torch = torch_cuda
+    rng = np.random.default_rng(17)
+    B = Batch(rng, [2, 1], [40000, 40001], 8, 128, 64)
+    qd, q = rounded(torch, rng.normal(0, 1, (3, 16, 128)), "f32")
+    got = Call(torch, fbctx, B, qd, None, "f32", 16).result(0.09)
+    check(got, attention(q, B, None, 0.09), q, B, 0.09, "f32")
