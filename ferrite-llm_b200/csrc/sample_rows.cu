@@ -53,6 +53,7 @@ constexpr int SR_ROUNDS = 4;    // narrowings before the bisection
 constexpr int SR_GROUPS = 48;   // groups a thread, at most
 constexpr int SR_AHEAD = 4;     // vectors a thread has in flight
 constexpr int SR_FLAGGED = 1024;
+constexpr float SR_REF = 4194304.f;  // 2^22: below it f32 has integers and halves
 constexpr double SR_UNIT = 8796093022208.0;  // 2^43
 
 using u64 = unsigned long long;
@@ -133,7 +134,7 @@ __device__ __forceinline__ u64 sr_pair(float x, int i) { return ((u64)sr_key(x) 
 
 // A row's settings.
 struct RowRule {
-    double scale, min_p, top_p, t;  // scale = 64 log2(e) / T; min_p 0: off; top_p 2: off
+    double scale, min_p, top_p, t;  // scale = 16 log2(e) / T; min_p 0: off; top_p 2: off
     float c;                        // log2(e) / T
     int top_k;                      // 0: off
     double u;
@@ -144,44 +145,59 @@ struct RowRule {
         const int k = A.top_k ? A.top_k[r] : 0;
         greedy = tt <= 0.f;
         t = (tt != tt || greedy) ? 1.0 : (double)tt;
-        scale = 92.33248261689366 / t;  // 64 log2(e) / T
-        c = (float)fmin(fmax(scale * 0.015625, 1e-30), 1e30);  // (bounded: 0 c stays 0, -FLT_MAX c far below any weight)
+        scale = 23.083120654223414 / t;  // 16 log2(e) / T
+        c = (float)fmin(fmax(scale * 0.0625, 1e-30), 1e30);  // (bounded: 0 c stays 0, -FLT_MAX c far below any weight)
         min_p = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
         top_p = tp < 1.f ? fmax((double)tp, 0.0) : 2.0;
         top_k = k > 0 && k < A.vocab ? k : 0;
         u = uu > 0.f ? fmin((double)uu, 1.0) : 0.0;
     }
-    // exp((x - mx) / T) = 2^(z / 64), z = scale (x - mx): the table holds 2^(j / 64), and the rest |r| <= 1/2 of a
-    // step is the Taylor polynomial of e^(r ln2 / 64) (argument below 0.0055: degree 4 leaves 4e-14).  Of an
-    // infinite maximum only the infinite logits weigh, 1 each; NaN weighs 0.
+    // exp((x - mx) / T) = 2^(z / 16), z = scale (x - mx): the table holds 2^(j / 16), and the rest |r| <= 1/2 of a
+    // step is the Taylor polynomial of e^(r ln2 / 16) (argument below 0.022: degree 6 leaves 5e-16).  Sixteen doubles
+    // are one line of shared memory, which 32 lanes look up without a conflict; the polynomial's shorter form with 64
+    // of them took longer.  Of an infinite maximum only the infinite logits weigh, 1 each; NaN weighs 0.
     __device__ __forceinline__ double weight(float x, float mx, const double *table) const {
         if (mx == INFINITY) return x == mx ? 1.0 : 0.0;
         const double d = (double)x - (double)mx;
         const double z = __dmul_rn(d, scale);
-        if (!(z > -68800.0)) return 0.0;  // below 2^-1075, NaN
+        if (!(z > -17200.0)) return 0.0;  // below 2^-1075, NaN
         const double p = step(d, table, 0);
-        const int e = __double2loint(__fma_rn(d, scale, 6755399441055744.0)) >> 6, e0 = e / 2;
+        const int e = __double2loint(__fma_rn(d, scale, 6755399441055744.0)) >> 4, e0 = e / 2;
         return __dmul_rn(__dmul_rn(p, exp64_pow2(e0)), exp64_pow2(e - e0));  // (e reaches -1075)
     }
-    // 2^(z / 64 - floor) in [1, 2), or with `whole` the whole weight (z / 64 >= -900)
+    // 2^(z / 16 - floor) in [1, 2), or with `whole` the whole weight (z / 16 >= -900)
     __device__ __forceinline__ double step(double d, const double *table, int whole) const {
         const double q = __fma_rn(d, scale, 6755399441055744.0);  // 1.5 * 2^52: the nearest integer in the low bits
         const double r = __fma_rn(d, scale, -__dsub_rn(q, 6755399441055744.0));
-        constexpr double L = 0.010830424696249145;  // ln2 / 64
-        double p = __fma_rn(r, L * L * L * L / 24.0, L * L * L / 6.0);
+        constexpr double L = 0.04332169878499658;  // ln2 / 16
+        double p = __fma_rn(r, L * L * L * L * L * L / 720.0, L * L * L * L * L / 120.0);
+        p = __fma_rn(p, r, L * L * L * L / 24.0);
+        p = __fma_rn(p, r, L * L * L / 6.0);
         p = __fma_rn(p, r, L * L / 2.0);
         p = __fma_rn(p, r, L);
         p = __dmul_rn(p, r);
         const int n = __double2loint(q);
-        const double t = table[n & 63];
+        const double t = table[n & 15];
         p = __fma_rn(t, p, t);
-        return whole ? __hiloint2double(__double2hiint(p) + ((n >> 6) << 20), __double2loint(p)) : p;
+        return whole ? __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p)) : p;
     }
     // One unit and the whole units of the weight, as a double (exact: at most 2^43 + 1), for a finite maximum and x >=
     // the lowest logit that weighs at all; below vmin (weights under 2^-59) that is one unit.
     __device__ __forceinline__ double units_of(float x, float mx, float vmin, const double *table) const {
         const double w = step((double)fmaxf(x, vmin) - (double)mx, table, 1);
         return __dsub_rn(__fma_rd(w, SR_UNIT, 4503599627370496.0), 4503599627370495.0);  // + 2^52 - (2^52 - 1)
+    }
+    // The mass that top-p asks for: top_p mass rounded up, exactly (top_p is an f32, M 2^-e with M below 2^24 and e from
+    // 24 on), so that equal weights share a border as they should.
+    __device__ __forceinline__ u64 need(u64 mass) const {
+        if (!(top_p > 0.0)) return 0;
+        const long long bits = __double_as_longlong(top_p);
+        const u64 M = (u64)((bits & 0xfffffffffffffll) | 0x10000000000000ll) >> 29;
+        const int e = 1023 + 23 - (int)(bits >> 52);
+        const u64 hi = __umul64hi(mass, M), lo = mass * M;
+        if (e < 64) return (hi << (64 - e) | lo >> e) + ((lo << (64 - e)) != 0);
+        if (e == 64) return hi + (lo != 0);
+        return 1;  // (hi is below 2^22; what top_p 2^-41 asks for is one token)
     }
 };
 
@@ -224,7 +240,7 @@ struct SrShared {
     u64 slot[2][SR_CLUSTER];                   // pushed by every rank
     u64 red[32];
     u64 cut, kept_mass, target;
-    double table[64];
+    double table[16];
     float max_of[SR_CLUSTER], low_of[SR_CLUSTER], mass_of[SR_CLUSTER];
     uint32_t edge[2];
     alignas(8) uint32_t cnt[2][SR_BINS], mass[2][SR_BINS];
@@ -236,7 +252,7 @@ struct SrShared {
     uint32_t kmin;
 };
 
-static_assert(SR_BINS == 2 * SR_THREADS && SR_CLUSTER * SR_WARPS <= SR_THREADS, "a thread two bins, a thread a run");
+static_assert(SR_AHEAD == 4 && SR_BINS == 2 * SR_THREADS && SR_CLUSTER * SR_WARPS <= SR_THREADS, "a sum of four, a thread two bins, a thread a run");
 
 template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_rows(const SampleRowsArgs A) {
     constexpr int E = SR_E<T>;
@@ -295,11 +311,13 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
         }
     };
 
-    // ---- the first pass: the groups' maxima, and for top-p without min-p the approximate mass (each thread's
-    // relative to its own running maximum)
+    // ---- the first pass: the groups' maxima, and for top-p without min-p the approximate mass.  Each thread's is
+    // relative to 2^ref of its own running maximum, ref an integer (within SR_REF): x c - ref is one rounding, and a change of ref
+    // exact.  What it is off by: 2^-22 a term (ex2), 2^-23 |x c| of it (17 on average at most), 2^-24 for each of at
+    // most 170 additions one behind the other; 1.3e-5 in all.
     const bool by_topk = rule.top_k > 0 && rule.top_k <= SR_TOPK && rule.min_p == 0.0 && !rule.greedy;
     const bool has_p = rule.top_p < 1.0, cuts = rule.top_k > 0 || has_p;
-    if (tid < 64) S.table[tid] = exp2((double)tid * 0.015625);
+    if (tid < 16) S.table[tid] = exp2((double)tid * 0.0625);
     if (tid == 0) S.n_list = S.n_flagged = 0;
     for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[0][i] = S.mass[0][i] = 0;
     auto ex2 = [](float y) {
@@ -307,8 +325,10 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
         return e;
     };
+    auto ref = [&](float top) { return fminf(fmaxf(ceilf(__fmul_rn(top, rule.c)), -SR_REF), SR_REF); };
+    auto two_to = [](float n) { return __int_as_float(max(127 + (int)n, 0) << 23); };  // n <= 0, 0 from -127 on
     const bool online = has_p && rule.min_p == 0.0 && !rule.greedy;
-    float tmax = -INFINITY, tsum = 0.f;
+    float tmax = -INFINITY, tsum = 0.f, tref = -SR_REF;
     {
         // batches of SR_AHEAD vectors, the next one in flight while this one is looked at
         auto load = [&](int s, uint4 (&q)[SR_AHEAD]) {
@@ -335,20 +355,21 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             }
             gm = fmaxf(gm, m);
             if (online && m > -INFINITY) {
-                const float top = fmaxf(tmax, m);
-                const float off = -__fmul_rn(top, rule.c);
-                float sum = tsum > 0.f ? __fmul_rn(tsum, ex2(__fmul_rn(__fsub_rn(tmax, top), rule.c))) : 0.f;
+                const float top_ref = ref(fmaxf(tmax, m));
+                float sum[SR_AHEAD];
 #pragma unroll
                 for (int k = 0; k < SR_AHEAD; k++) {
                     float v[E];
                     // NaN and -inf as the lowest f32 or bf16, which weighs nothing at any T (fp16's would)
                     constexpr bool half = std::is_same<T, __half>::value;
                     sr_unpack<T>(half ? q[k] : sr_max<T>(q[k], sr_lowest<T>()), v);
+                    sum[k] = 0.f;
 #pragma unroll
                     for (int e = 0; e < E; e++)
-                        sum += ex2(__fmaf_rn(half ? fmaxf(v[e], -3.4028235e38f) : v[e], rule.c, off));
+                        sum[k] += ex2(__fmaf_rn(half ? fmaxf(v[e], -3.4028235e38f) : v[e], rule.c, -top_ref));
                 }
-                tsum = sum;
+                tsum = __fmaf_rn(tsum, two_to(tref - top_ref), (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                tref = top_ref;
             }
             tmax = fmaxf(tmax, m);
             ahead -= SR_AHEAD;
@@ -393,9 +414,8 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     const float bmax = sr_reduce(tmax, reinterpret_cast<float *>(S.red), maxf);
     const float blow = sr_reduce(tmax > -INFINITY ? tmax : INFINITY, reinterpret_cast<float *>(S.red), minf);
     float bsum = 0.f;
-    if (online)  // (relative to this CTA's maximum)
-        bsum = sr_reduce(tsum > 0.f ? __fmul_rn(tsum, ex2(__fmul_rn(__fsub_rn(tmax, bmax), rule.c))) : 0.f,
-                         reinterpret_cast<float *>(S.red), addf);
+    if (online)  // (relative to this CTA's ref)
+        bsum = sr_reduce(__fmul_rn(tsum, two_to(tref - ref(bmax))), reinterpret_cast<float *>(S.red), addf);
     if (cs > 1) csync();  // every rank has started
     push(&SrShared::max_of, bmax);
     push(&SrShared::low_of, blow);
@@ -478,9 +498,16 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     };
     bool few = false;
     float m1 = 0.f;  // approximate mass of the survivors
-    if (online)
-        for (int i = 0; i < cs; i++)
-            if (S.mass_of[i] > 0.f) m1 += __fmul_rn(S.mass_of[i], rough(S.max_of[i]));
+    // (a maximum next to the lowest value, which the first pass took NaN and -inf for, or so many times T that f32 has
+    // no place behind the point: the first pass's masses say nothing)
+    const bool summed = online && mx > -1e38f && fabsf(__fmul_rn(mx, rule.c)) < SR_REF;
+    // a rank's approximate mass, relative to the maximum's weight
+    const float lift = summed ? ex2(__fmaf_rn(-mx, rule.c, ref(mx))) : 1.f;
+    auto mass_at = [&](int i) {
+        return summed ? __fmul_rn(__fmul_rn(S.mass_of[i], two_to(ref(S.max_of[i]) - ref(mx))), lift) : S.mass_of[i];
+    };
+    if (summed)
+        for (int i = 0; i < cs; i++) m1 += mass_at(i);
     if (rule.min_p > 0.0) {
         few = true;
         if (!look_into([&](float m) { return m >= xmin; },
@@ -529,7 +556,6 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     }
 
     auto value_of = [](u64 pr) { return sr_unkey((uint32_t)(pr >> 32)); };
-    auto need_of = [&](double mass) { return (u64)ceil(rule.top_p * mass); };
     // Few entries: the block ranks them, a group of lanes adding up for one entry what counts() lets count.
     auto ranked = [&](int n, auto counts, auto use) {
         int g = 1;  // lanes an entry
@@ -636,22 +662,30 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             u64 lo = ~0ull, hi = ~0ull;
             const bool open = has_p && rule.min_p == 0.0;  // the list does not hold all survivors
             if (open) {
-                lo = need_of((double)m1 * (1.0 - 1e-4) * SR_UNIT);
-                hi = need_of((double)m1 * (1.0 + 1e-4) * SR_UNIT);
+                lo = summed ? rule.need((u64)((double)m1 * (1.0 - 2e-5) * SR_UNIT)) : 0;
+                hi = summed ? rule.need((u64)((double)m1 * (1.0 + 2e-5) * SR_UNIT)) : ~0ull;
             } else if (has_p) {
                 u64 m = 0;
                 for (int i = tid; i < n; i += SR_THREADS) m += S.wt[i];
-                lo = hi = need_of((double)sr_reduce(m, S.red, addu));
+                lo = hi = rule.need(sr_reduce(m, S.red, addu));
             }
             if (!find_cut(n, 0, 0, lo, hi)) {
                 u64 m = 0;  // the exact mass of the whole row
-#pragma unroll 4
-                for (int i = tid; i < A.vocab; i += SR_THREADS) {
-                    const float v = sr_load(x, i);
-                    const u64 w = unit_of(v);
-                    if (v >= xmin) m += w;
+                for (int i0 = tid * E; i0 < A.vocab; i0 += SR_AHEAD * SR_THREADS * E) {
+                    uint4 q[SR_AHEAD];
+#pragma unroll
+                    for (int k = 0; k < SR_AHEAD; k++) q[k] = fetch(i0 + k * SR_THREADS * E);
+                    double d = 0.0;  // (exact: at most 32 logits of 2^43 + 1)
+#pragma unroll
+                    for (int k = 0; k < SR_AHEAD; k++) {
+                        float v[E];
+                        sr_unpack<T>(q[k], v);
+#pragma unroll
+                        for (int e = 0; e < E; e++) d = __dadd_rn(d, v[e] >= xmin ? unit_d(v[e]) : 0.0);
+                    }
+                    m += (u64)d;
                 }
-                lo = need_of((double)sr_reduce(m, S.red, addu));
+                lo = rule.need(sr_reduce(m, S.red, addu));
                 find_cut(n, 0, 0, lo, lo);
             }
             const u64 cut = S.cut, total = S.kept_mass;
@@ -693,7 +727,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     unsigned c_above = 0, in_range = 0;
     if (cuts) {
         // lowest survivor, and the approximate mass, as far as the first pass has not found them
-        if (!online) {
+        if (!summed) {
             float mass = 0.f;
             stream([&](float (&v)[E], int) {
 #pragma unroll
@@ -712,16 +746,12 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[0][i] = 0;
             __syncthreads();
         }
-        // a rank's approximate mass; its bins count it in units of 2^-30
-        auto mass_at = [&](int i) {
-            const float m = S.mass_of[i];
-            return online && m > 0.f ? __fmul_rn(m, rough(S.max_of[i])) : m;
-        };
-        if (!online) {
+        if (!summed) {
             m1 = 0.f;
             for (int i = 0; i < cs; i++) m1 += S.mass_of[i];
         }
-        const float step = __fmul_rn(mass_at(rank), 0x1p-30f), per = step > 0.f ? __fdiv_rn(1.f, step) : 0.f;
+        // a rank's bins count its mass in units of 2^-31 of it (2^19 roundings of half a unit are 1.2e-4)
+        const float step = __fmul_rn(mass_at(rank), 0x1p-31f), per = step > 0.f ? __fdiv_rn(1.f, step) : 0.f;
         // The first round's bins reach to weights of 2^-43; with top-p no further than the weights that, all vocab of
         // them, would not make up what the cut leaves out.  The last bin holds the rest.
         float lo = 0.f, hi = __fdiv_rn(30.f, rule.c * 0.6931472f);
@@ -774,7 +804,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
                 n[1] += c2.y;
                 if (has_p) {
                     const uint2 m2 = *reinterpret_cast<const uint2 *>(&o->mass[buf][2 * tid]);
-                    const float unit = __fmul_rn(mass_at(i), 0x1p-30f);
+                    const float unit = __fmul_rn(mass_at(i), 0x1p-31f);
                     m[0] += __fmul_rn((float)m2.x, unit);
                     m[1] += __fmul_rn((float)m2.y, unit);
                 }
@@ -895,7 +925,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             mass += lead->slot[1][i];
             for (int j = 0; j < SR_WARPS; j++) above += lead->seg[i * SR_WARPS + j];
         }
-        const u64 need = has_p ? need_of((double)mass) : ~0ull;
+        const u64 need = has_p ? rule.need(mass) : ~0ull;
         u64 lo_pair = 0, hi_pair = ~0ull;
         while (hi_pair - lo_pair > 1) {
             const u64 mid = lo_pair + (hi_pair - lo_pair) / 2;
@@ -944,14 +974,21 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
         u64 above = tid < cs * SR_WARPS ? S.seg[tid] : 0, mass = 0;
         above = sr_reduce(above, S.red, addu);
         for (int i = 0; i < cs; i++) mass += S.slot[1][i];
-        const u64 need = has_p ? need_of((double)mass) : ~0ull;
+        const u64 need = has_p ? rule.need(mass) : ~0ull;
         find_cut(n, above, c_above, need, need);
         cut = S.cut;
         for (int i = tid; i < n; i += SR_THREADS)
-            if (S.list[i] >= cut) atomicAdd(&S.seg[(int)~(uint32_t)S.list[i] / run], unit_of(value_of(S.list[i])));
+            if (S.list[i] >= cut) {
+                // (two 32-bit atomics and the carry: a 64-bit one in shared memory is a loop)
+                const u64 w = unit_of(value_of(S.list[i]));
+                unsigned *half = reinterpret_cast<unsigned *>(&S.seg[(int)~(uint32_t)S.list[i] / run]);
+                const unsigned low32 = (unsigned)w, sum = atomicAdd(half, low32) + low32;
+                atomicAdd(half + 1, (unsigned)(w >> 32) + (sum < low32));
+            }
         __syncthreads();
     }
     const u64 mine = tid < cs * SR_WARPS ? S.seg[tid] : 0;
+    if (tid == 0) S.where = 0;
     u64 total;
     const u64 before = sr_scan(mine, S.red, &total);
     u64 target = (u64)(rule.u * (double)total);

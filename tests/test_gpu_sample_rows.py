@@ -157,3 +157,53 @@ def test_without_probabilities_and_in_a_graph(fbctx, torch_cuda):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(a, b) and (a >= 0).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [(6, 5000), (500, 3001)])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_top_p_close_to_a_border(fbctx, torch_cuda, kind, rows, vocab):
+    """top_p within 10^-6 of what the leading logits hold, on either side: an approximate mass cannot tell the cut."""
+    torch = torch_cuda
+    rng = np.random.default_rng(vocab)
+    x = 2 * rng.normal(0, 1, (rows, vocab))
+    x[:, ::7] = 2 * x[:, ::7] + rng.random((rows, 1))
+    t = rng.uniform(0.5, 1.5, rows).astype(np.float32)
+    _, held = rounded(torch, x, kind)
+    p = np.empty(rows, np.float32)
+    for r in range(rows):
+        w = np.sort(np.exp((held[r] - held[r].max()) / float(t[r])))[::-1]
+        at = int(rng.integers(2, 30))
+        while w[at] == w[at + 1]:
+            at += 1
+        p[r] = np.float32(np.cumsum(w)[at] / w.sum() * (1 + (1e-6 if r % 2 else -1e-6)))
+    for k in (50, None):
+        check(*run(torch, fbctx, x, kind, t=t, k=k, p=p, u=np.full(rows, 0.9999)))
+
+
+@pytest.mark.parametrize("size,t", [(4000.0, 0.1), (30000.0, 1.0), (3e8, 1e6), (1e30, 1e-8)])
+def test_large_logits(fbctx, torch_cuda, size, t):
+    """Logits far from zero in units of the temperature: what f32 loses of x / T must not move the cut."""
+    rng = np.random.default_rng(7)
+    x = size + 20 * t * rng.random((12, 3000))
+    for s in (dict(k=40, p=0.9), dict(p=0.7), dict(p=0.99, k=200)):
+        check(*run(torch_cuda, fbctx, x, "f32", t=t, u=rng.random(12), **s))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("t", [1.0, 0.25, 1e-6])
+def test_masks_of_the_lowest_value_and_infinities(fbctx, torch_cuda, kind, t):
+    """Masked by the type's lowest value (whole threads' logits, or all but NaN and -inf), several infinite logits."""
+    torch = torch_cuda
+    lowest = torch.finfo(torch_type(torch, kind)).min
+    rng = np.random.default_rng(8)
+    x = 3 * rng.normal(0, 1, (6, 20011))
+    x[0, 300:] = lowest
+    x[1, :19000] = lowest
+    x[2, :] = lowest
+    x[3, :] = lowest
+    x[3, ::3] = -np.inf
+    x[3, 1::3] = np.nan
+    x[4, [5, 600, 601, 9000, 20010]] = np.inf
+    x[5, rng.random(20011) < 0.9] = lowest
+    for s in (dict(k=40, p=0.9), dict(p=0.7), dict(p=0.35, k=400), dict(p=0.5, m=0.01)):
+        check(*run(torch, fbctx, x, kind, t=t, u=rng.random(6), **s))
