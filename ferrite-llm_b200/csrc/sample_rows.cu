@@ -57,6 +57,7 @@ constexpr float SR_REF = 4194304.f;  // 2^22: below it f32 has integers and halv
 constexpr double SR_UNIT = 8796093022208.0;  // 2^43
 
 using u64 = unsigned long long;
+constexpr u64 SR_BIAS = 0x4330000000000000ull - 1;  // the bits of 2^52, less each weight's extra unit
 
 // A row's logits: rank r of the cluster has the run of `chunk` logits from r
 // chunk on, its warp w the run of chunk / 8 from w chunk / 8 on, in `steps`
@@ -186,6 +187,12 @@ struct RowRule {
     __device__ __forceinline__ double units_of(float x, float mx, float vmin, const double *table) const {
         const double w = step((double)fmaxf(x, vmin) - (double)mx, table, 1);
         return __dsub_rn(__fma_rd(w, SR_UNIT, 4503599627370496.0), 4503599627370495.0);  // + 2^52 - (2^52 - 1)
+    }
+    // The same as an integer that is SR_BIAS too large: what adds up many of them adds integers and takes the surplus
+    // off once.  mx is finite here, and x above it counts as it.
+    __device__ __forceinline__ u64 biased_units(float x, float mx, float vmin, const double *table) const {
+        const double w = step((double)fminf(fmaxf(x, vmin), mx) - (double)mx, table, 1);
+        return (u64)__double_as_longlong(__fma_rd(w, SR_UNIT, 4503599627370496.0));
     }
     // The mass that top-p asks for: top_p mass rounded up, exactly (top_p is an f32, M 2^-e with M below 2^24 and e from
     // 24 on), so that equal weights share a border as they should.
@@ -471,7 +478,8 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
         }
         __syncthreads();
     }
-    const float xmin = rule.min_p > 0.0 ? sr_unkey(S.kmin) : -3.4028235e38f;  // survivors: x >= xmin
+    // survivors: x >= xmin (only the infinite logits weigh next to an infinite maximum)
+    const float xmin = mx == INFINITY ? INFINITY : rule.min_p > 0.0 ? sr_unkey(S.kmin) : -3.4028235e38f;
     const float vmin = rule.t < 1e30 ? (float)((double)mx - 41.0 * rule.t) : -3.4028235e38f;  // weight 2^-59
     const float vzero = rule.t < 1e30 ? (float)((double)mx - 745.0 * rule.t) : -3.4028235e38f;  // weighs nothing below
     // units of a logit as a double: a thread adds up to 2^9 of them exactly (2^52)
@@ -482,9 +490,8 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     };
     auto unit_of = [&](float v) { return (u64)unit_d(v); };
     // binary32 weight, relative error below 1e-5 wherever it is not negligible
-    auto rough = [&](float v) {
-        const float e = ex2(__fmul_rn(__fsub_rn(v, mx), rule.c));
-        return v == mx ? 1.f : mx == INFINITY ? 0.f : e;
+    auto rough = [&](float v) {  // (of an infinite maximum: NaN's smaller one is 0, so 1 for an infinite logit)
+        return ex2(fminf(__fmul_rn(__fsub_rn(v, mx), rule.c), 0.f));
     };
 
     // ---- few candidates: min-p's survivors, or what lies above the groups' top_k-th largest maximum
@@ -714,10 +721,9 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     // ---- many candidates: the cut's range by bins of the distance to the maximum
     u64 cut = 0;  // the last kept (logit, index) pair
     // survivors from xa on stay, those in xb .. xa are the range that the cut lies in
-    float xa = cuts ? INFINITY : xmin, xb = xmin;
-    bool to_top = cuts;  // the range still reaches the maximum
-    auto side = [&](float v) { return !to_top && v >= xa ? 1 : v >= xb ? 0 : -1; };
-    auto dist = [&](float v) { return __fsub_rn(mx, v); };  // (NaN for an infinite maximum: bin 0)
+    bool to_top = cuts;  // the range still reaches the maximum: xa is NaN, which nothing reaches
+    float xa = cuts ? __int_as_float(0x7fffffff) : xmin, xb = xmin;
+    auto side = [&](float v) { return v >= xa ? 1 : v >= xb ? 0 : -1; };
     // kept mass of every warp's run, to rank 0
     auto push_run = [&](u64 m) {
 #pragma unroll
@@ -763,25 +769,32 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
         for (int round = 0; round < SR_ROUNDS; round++) {
             const int buf = round & 1;
             const float width = hi - lo;
-            const float inv = width > 0.f && width < INFINITY ? __fdiv_rn((float)(SR_BINS - 1), width) : 0.f;
-            auto bin = [&](float v) {
-                return (int)fminf(fmaxf(__fmul_rn(__fsub_rn(dist(v), lo), inv), 0.f), (float)(SR_BINS - 1));
+            const float inv = width > 0.f && width < INFINITY ? __fdiv_rn(1.f, width) : 0.f;
+            const float from = __fsub_rn(mx, lo);
+            auto bin = [&](float v) {  // (a number of 23 bits behind 2^23; bin 0 of an infinite maximum: NaN saturates to 0)
+                const float t = __saturatef(__fmul_rn(__fsub_rn(from, v), inv));
+                return (int)(__float_as_uint(__fmaf_rd(t, (float)(SR_BINS - 1), 8388608.f)) - 0x4b000000u);
             };
             unsigned n_last = 0;  // (the last bin is a crowded one: counted in registers)
             float m_last = 0.f;
             stream([&](float (&v)[E], int) {
+                int b[E];
+                unsigned u[E];
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const int b = bin(v[e]);
                     const float p = has_p ? rough(v[e]) : 0.f;
-                    const bool in = side(v[e]) == 0, last = in && b == SR_BINS - 1;
-                    n_last += last;
-                    m_last += last ? p : 0.f;
-                    if (in && !last) {
-                        atomicAdd(&S.cnt[buf][b], 1u);
-                        if (has_p) atomicAdd(&S.mass[buf][b], __float2uint_rn(__fmul_rn(p, per)));
-                    }
+                    const int at = bin(v[e]);
+                    b[e] = side(v[e]) == 0 ? at : SR_BINS;
+                    m_last += b[e] == SR_BINS - 1 ? p : 0.f;
+                    n_last += b[e] == SR_BINS - 1;
+                    u[e] = __float2uint_rn(__fmul_rn(p, per));
                 }
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (b[e] < SR_BINS - 1) {
+                        atomicAdd(&S.cnt[buf][b[e]], 1u);
+                        if (has_p) atomicAdd(&S.mass[buf][b[e]], u[e]);
+                    }
             });
             n_last = sr_reduce(n_last, reinterpret_cast<unsigned *>(S.red), [](unsigned a, unsigned b) { return a + b; });
             m_last = sr_reduce(m_last, reinterpret_cast<float *>(S.red), addf);
@@ -892,26 +905,24 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     }
     u64 kept = 0, m_all = 0;
     {
-        double kept_d = 0.0, all_d = 0.0;
-        int n = 0;
+        // from which logit on they weigh and count (NaN: none does)
+        const float none_of = __int_as_float(0x7fffffff);
+        const float from_kept = xa == xa ? fmaxf(xa, vzero) : none_of, from_all = has_p ? fmaxf(xmin, vzero) : none_of;
+        const float top = fminf(mx, 3.4028235e38f);
         stream([&](float (&v)[E], int i) {
-            if (++n > 256 / E) {  // (256 logits of at most 2^43 + 1 are exact in a double)
-                kept += (u64)kept_d;
-                m_all += (u64)all_d;
-                kept_d = all_d = 0.0;
-                n = 1;
-            }
+            unsigned hits = 0;  // (no branch between the logits: their chains of double operations run together)
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                const int s = side(v[e]);
-                const double w = has_p || s > 0 ? unit_d(v[e]) : 0.0;
-                if (v[e] >= xmin) all_d = __dadd_rn(all_d, w);
-                if (s > 0) kept_d = __dadd_rn(kept_d, w);
-                if (s == 0 && listed) lead->list[at0 + atomicAdd(&S.n_list, 1u)] = sr_pair(v[e], i + e);
+                const u64 w = rule.biased_units(v[e], top, vmin, S.table) - SR_BIAS;
+                m_all += v[e] >= from_all ? w : 0;
+                kept += v[e] >= from_kept ? w : 0;
+                hits |= side(v[e]) == 0 ? 1u << e : 0u;
             }
+            if (listed && hits)
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (hits >> e & 1u) lead->list[at0 + atomicAdd(&S.n_list, 1u)] = sr_pair(v[e], i + e);
         });
-        kept += (u64)kept_d;
-        m_all += (u64)all_d;
     }
     push_run(kept);
     m_all = sr_reduce(m_all, S.red, addu);
