@@ -82,6 +82,7 @@ constexpr int TR_ROWS = 128;      // rows a tile (MMA M)
 constexpr int TR_PAIR = 256;      // rows a group at most: two tiles
 constexpr int TR_KB = 64;         // keys a block
 constexpr int TR_WHOLE = 4;
+constexpr int TR_SWITCH = 8;
 constexpr int TR_THREADS = 384;
 constexpr float TR_NONE = -1e30f;  // running maximum of a row that has seen nothing
 constexpr float TR_LIFT = 7.f;     // probabilities are kept 2^7 above the reference maximum
@@ -140,47 +141,61 @@ struct TreeSeq {
         return ok;
     }
     __device__ __forceinline__ int per(const TreeArgs &A) const { return A.split ? blocks : 1; }
-    __device__ __forceinline__ int head_units(const TreeArgs &A) const {
-        return pairs > 0 ? (full * (pairs - 1) + weight) * per(A) : 0;
+    __device__ __forceinline__ int head_units(const TreeArgs &A, int lead) const {
+        return pairs > 0 ? (full * (pairs - 1) + weight) * per(A) + pairs * lead : 0;
     }
-    __device__ __forceinline__ int units(const TreeArgs &A) const { return head_units(A) * A.n_kv; }
+    __device__ __forceinline__ int units(const TreeArgs &A, int lead) const { return head_units(A, lead) * A.n_kv; }
+    __device__ __forceinline__ int groups(const TreeArgs &A) const { return pairs * A.n_kv; }
 };
 
-// Units of the sequences from `from` on, this lane's part.
-__device__ __forceinline__ int tree_total(const TreeArgs &A, int lane, int from, bool report) {
-    int total = 0;
-    for (int b = from + lane; b < A.batch; b += 32) {
-        TreeSeq s;
-        if (!s.load(A, b) && report) atomicOr(A.err, ERRBIT_BAD_POS);
-        total += s.units(A);
+// Units of all sequences without leads, and row groups: the warp's sums.
+struct TreeTotal {
+    int units, groups;
+    __device__ __forceinline__ void add(const TreeArgs &A, const TreeSeq &s) {
+        units += s.units(A, 0);
+        groups += s.groups(A);
     }
-    return total;
-}
-// A CTA's share; the join kernel derives the same one.  With split and blocks of
-// two units at least two, so that none lies inside such a block.
-__device__ __forceinline__ int tree_quota(const TreeArgs &A, int total) {
-    return max(A.split && A.grows > TR_ROWS ? 2 : 1, (total + A.ctas - 1) / A.ctas);
-}
+    __device__ __forceinline__ void reduce() {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            units += __shfl_xor_sync(0xffffffffu, units, o);
+            groups += __shfl_xor_sync(0xffffffffu, groups, o);
+        }
+    }
+    // Units that a row group has in front of its blocks: what it costs a CTA to begin another one (its queries wait for
+    // the last scores, its rows are written out), so that the shares with a border inside hold fewer blocks.  Where no
+    // CTA has more than a unit there is no border.  (60 new rows of 32 heads at 4096 keys, f32: 26.6 us; 29.1 with 3,
+    // 32.7 with none; 16 sequences of 25 rows, f16: 43.2, 44.4, 47.3.)
+    __device__ __forceinline__ int lead(const TreeArgs &A) const { return A.split && units > A.ctas ? TR_SWITCH : 0; }
+    // A CTA's share; the join kernel derives the same one.  With split and blocks of two units at least two, so that
+    // none lies inside such a block.
+    __device__ __forceinline__ int all(const TreeArgs &A) const { return units + groups * lead(A); }
+    __device__ __forceinline__ int quota(const TreeArgs &A) const {
+        return max(A.split && A.grows > TR_ROWS ? 2 : 1, (all(A) + A.ctas - 1) / A.ctas);
+    }
+};
 
 // The segments of a CTA's share: consecutive blocks of one row group.  A block
 // (without split: a group) belongs to the share that holds its first unit.
 struct TreeWalk {
     TreeSeq s;
-    int b, h, pair, blk0, blk1, left;
+    int b, h, pair, blk0, blk1, left, lead;
     // warp-collective; this CTA's share.  False: it holds no block's first unit.
     __device__ __forceinline__ bool start(const TreeArgs &A, int cta, int lane, bool report) {
         int base = 0, mine = 0;
-        if (lane < A.batch) {  // (the first 32 sequences stay in the lanes' registers)
-            if (!s.load(A, lane) && report) atomicOr(A.err, ERRBIT_BAD_POS);
-            mine = s.units(A);
-        } else {
-            s = TreeSeq{};
+        TreeTotal t{};
+        s = TreeSeq{};
+        for (int i = lane; i < A.batch; i += 32) {
+            TreeSeq o;
+            if (!o.load(A, i) && report) atomicOr(A.err, ERRBIT_BAD_POS);
+            t.add(A, o);
+            if (i < 32) s = o;  // (the first 32 sequences stay in the lanes' registers)
         }
         const TreeSeq first = s;
-        int total = mine + tree_total(A, lane, 32, report);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        const int quota = tree_quota(A, total);
+        t.reduce();
+        lead = t.lead(A);
+        const int total = t.all(A), quota = t.quota(A);
+        mine = s.units(A, lead);
         const int64_t u0l = (int64_t)quota * cta;
         if (u0l >= total) return false;
         const int u0 = (int)u0l;
@@ -191,7 +206,7 @@ struct TreeWalk {
                 mine = 0;
                 if (b0 + lane < A.batch) {
                     s.load(A, b0 + lane);
-                    mine = s.units(A);
+                    mine = s.units(A, lead);
                 }
             }
             int incl = mine;
@@ -220,21 +235,21 @@ struct TreeWalk {
         } else {
             s.load(A, b);
         }
-        const int per = s.per(A), hu = s.head_units(A);
+        const int each = s.full * s.per(A) + lead, hu = s.head_units(A, lead);
         int r = u0 - base;
         h = r / hu;
         r -= h * hu;
-        pair = min(r / (s.full * per), s.pairs - 1);
-        r -= pair * s.full * per;
+        pair = min(r / each, s.pairs - 1);
+        r -= pair * each;
         span(A, r);
         return blk0 < blk1 || next(A);
     }
     __device__ __forceinline__ int weight() const { return pair < s.pairs - 1 ? s.full : s.weight; }
     __device__ __forceinline__ void span(const TreeArgs &A, int r) {
-        const int w = weight(), take = min(left, w * s.per(A) - r);
+        const int w = weight(), take = min(left, w * s.per(A) + lead - r);
         if (A.split) {
-            blk0 = (r + w - 1) / w;
-            blk1 = (r + take + w - 1) / w;
+            blk0 = (max(r - lead, 0) + w - 1) / w;
+            blk1 = (max(r + take - lead, 0) + w - 1) / w;
         } else {
             blk0 = r == 0 ? 0 : s.blocks;
             blk1 = s.blocks;
@@ -251,7 +266,7 @@ struct TreeWalk {
                     do {
                         if (++b >= A.batch) return false;
                         s.load(A, b);
-                    } while (s.units(A) == 0);
+                    } while (s.groups(A) == 0);
                 }
             }
             span(A, 0);
@@ -1109,22 +1124,20 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
     const int row0 = pair * A.grows + 32 * slab;
     if (row0 >= s.n * A.group) return;
     // units before this sequence, and in all
-    int before = 0, total = 0;
+    TreeTotal t{}, before{};
     for (int i = lane; i < A.batch; i += 32) {
         TreeSeq o;
         o.load(A, i);
-        const int u = o.units(A);
-        total += u;
-        if (i < b) before += u;
+        t.add(A, o);
+        if (i < b) before.add(A, o);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    const int quota = tree_quota(A, total);
+    t.reduce();
+    before.reduce();
+    const int quota = t.quota(A), lead = t.lead(A);
     const int wt = pair < s.pairs - 1 ? s.full : s.weight;
-    const int gs = before + blockIdx.y * s.head_units(A) + pair * s.full * s.blocks;  // the group's first unit
+    // the group's first block's first unit
+    const int gs = before.units + before.groups * lead + blockIdx.y * s.head_units(A, lead) +
+                   pair * (s.full * s.blocks + lead) + lead;
     const int c0 = gs / quota, c1 = (gs + wt * (s.blocks - 1)) / quota;          // CTAs of its first and last block
     if (c0 == c1) return;  // written by its CTA
     const int rr = row0 + 8 * warp + (lane & 7), r = rr - pair * A.grows;
@@ -1194,7 +1207,7 @@ static TreePlan tree_plan(const fb_ctx *ctx, int batch, int max_new, int n_heads
     const int64_t rows = (int64_t)max_new * (n_heads / n_kv);
     const int64_t pairs = (rows + grows - 1) / grows, blocks = (max_seq_len + TR_KB - 1) / TR_KB;
     const int64_t groups = pairs * n_kv * batch;
-    FB_REQUIRE(2 * groups * blocks < ((int64_t)1 << 31) - 4096 && pairs <= 65535, "attn_tree: batch too large");
+    FB_REQUIRE(groups * (2 * blocks + TR_SWITCH) < ((int64_t)1 << 31) - 4096 && pairs <= 65535, "attn_tree: batch too large");
     FB_REQUIRE((rows + TR_PAIR) * (n_heads / n_kv) < ((int64_t)1 << 32), "attn_tree: too many rows");
     p.split = blocks > TR_WHOLE;
     const int64_t units = 2 * groups * (p.split ? blocks : 1);
