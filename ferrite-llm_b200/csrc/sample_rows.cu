@@ -194,17 +194,28 @@ struct RowRule {
         const double w = step((double)fminf(fmaxf(x, vmin), mx) - (double)mx, table, 1);
         return (u64)__double_as_longlong(__fma_rd(w, SR_UNIT, 4503599627370496.0));
     }
-    // The mass that top-p asks for: top_p mass rounded up, exactly (top_p is an f32, M 2^-e with M below 2^24 and e from
-    // 24 on), so that equal weights share a border as they should.
-    __device__ __forceinline__ u64 need(u64 mass) const {
-        if (!(top_p > 0.0)) return 0;
-        const long long bits = __double_as_longlong(top_p);
+    // f mass, exactly, of an f32 f in 0 .. 1 (M 2^-e, M below 2^24, e from 23 on) and a mass below 2^62: rounded down,
+    // rest whether anything was dropped.
+    static __device__ __forceinline__ u64 share(double f, u64 mass, bool &rest) {
+        rest = false;
+        if (!(f > 0.0)) return 0;
+        const long long bits = __double_as_longlong(f);
         const u64 M = (u64)((bits & 0xfffffffffffffll) | 0x10000000000000ll) >> 29;
         const int e = 1023 + 23 - (int)(bits >> 52);
         const u64 hi = __umul64hi(mass, M), lo = mass * M;
-        if (e < 64) return (hi << (64 - e) | lo >> e) + ((lo << (64 - e)) != 0);
-        if (e == 64) return hi + (lo != 0);
-        return 1;  // (hi is below 2^22; what top_p 2^-41 asks for is one token)
+        rest = e >= 64 || lo << (64 - e) != 0;  // (from 64 on: taken so, below one token's mass either way)
+        return e < 64 ? hi << (64 - e) | lo >> e : e < 128 ? hi >> (e - 64) : 0;
+    }
+    // The mass that top-p asks for, rounded up, and the place of u in a mass: exact, so that equal weights share a
+    // border as they should.
+    __device__ __forceinline__ u64 need(u64 mass) const {
+        bool rest;
+        const u64 n = share(top_p, mass, rest);
+        return n + rest;
+    }
+    __device__ __forceinline__ u64 place(u64 mass) const {
+        bool rest;
+        return min(share(u, mass, rest), mass - 1);
     }
 };
 
@@ -248,7 +259,8 @@ struct SrShared {
     u64 red[32];
     u64 cut, kept_mass, target;
     double table[16];
-    float max_of[SR_CLUSTER], low_of[SR_CLUSTER], mass_of[SR_CLUSTER];
+    float max_of[SR_CLUSTER], low_of[SR_CLUSTER];
+    double mass_of[SR_CLUSTER];
     uint32_t edge[2];
     alignas(8) uint32_t cnt[2][SR_BINS], mass[2][SR_BINS];
     uint32_t flagged[SR_FLAGGED];              // groups to look into
@@ -319,9 +331,10 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     };
 
     // ---- the first pass: the groups' maxima, and for top-p without min-p the approximate mass.  Each thread's is
-    // relative to 2^ref of its own running maximum, ref an integer (within SR_REF): x c - ref is one rounding, and a change of ref
-    // exact.  What it is off by: 2^-22 a term (ex2), 2^-23 |x c| of it (17 on average at most), 2^-24 for each of at
-    // most 170 additions one behind the other; 1.3e-5 in all.
+    // relative to 2^ref of its own running maximum, ref an integer (within SR_REF): x c - ref is one rounding, and a
+    // change of ref exact.  What it is off by: 2^-22 a term (ex2), 2^-24 |x c - ref| of it and half as much for c (together 1e-6, as the
+    // weights of a row are below 17 of these on average), 10 2^-24 for a batch's sum; from there on it is a double.
+    // 2.3e-6 with the last factors.
     const bool by_topk = rule.top_k > 0 && rule.top_k <= SR_TOPK && rule.min_p == 0.0 && !rule.greedy;
     const bool has_p = rule.top_p < 1.0, cuts = rule.top_k > 0 || has_p;
     if (tid < 16) S.table[tid] = exp2((double)tid * 0.0625);
@@ -333,9 +346,10 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
         return e;
     };
     auto ref = [&](float top) { return fminf(fmaxf(ceilf(__fmul_rn(top, rule.c)), -SR_REF), SR_REF); };
-    auto two_to = [](float n) { return __int_as_float(max(127 + (int)n, 0) << 23); };  // n <= 0, 0 from -127 on
+    auto two_to = [](float n) { return __hiloint2double(max(1023 + (int)n, 0) << 20, 0); };  // n <= 0, 0 from -1023 on
     const bool online = has_p && rule.min_p == 0.0 && !rule.greedy;
-    float tmax = -INFINITY, tsum = 0.f, tref = -SR_REF;
+    float tmax = -INFINITY, tref = -SR_REF;
+    double tsum = 0.0;
     {
         // batches of SR_AHEAD vectors, the next one in flight while this one is looked at
         auto load = [&](int s, uint4 (&q)[SR_AHEAD]) {
@@ -375,7 +389,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
                     for (int e = 0; e < E; e++)
                         sum[k] += ex2(__fmaf_rn(half ? fmaxf(v[e], -3.4028235e38f) : v[e], rule.c, -top_ref));
                 }
-                tsum = __fmaf_rn(tsum, two_to(tref - top_ref), (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                tsum = __fma_rn(tsum, two_to(tref - top_ref), (double)((sum[0] + sum[1]) + (sum[2] + sum[3])));
                 tref = top_ref;
             }
             tmax = fmaxf(tmax, m);
@@ -415,14 +429,15 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
         }
         return true;
     };
-    auto push = [&](float (SrShared::*field)[SR_CLUSTER], float v) {  // own value into every rank's [rank]
+    auto push = [&](auto field, auto v) {  // own value into every rank's [rank]
         if (tid < cs) (cl.map_shared_rank(&S, tid)->*field)[rank] = v;
     };
     const float bmax = sr_reduce(tmax, reinterpret_cast<float *>(S.red), maxf);
     const float blow = sr_reduce(tmax > -INFINITY ? tmax : INFINITY, reinterpret_cast<float *>(S.red), minf);
-    float bsum = 0.f;
+    double bsum = 0.0;
     if (online)  // (relative to this CTA's ref)
-        bsum = sr_reduce(__fmul_rn(tsum, two_to(tref - ref(bmax))), reinterpret_cast<float *>(S.red), addf);
+        bsum = sr_reduce(__dmul_rn(tsum, two_to(tref - ref(bmax))), reinterpret_cast<double *>(S.red),
+                         [](double a, double b) { return a + b; });
     if (cs > 1) csync();  // every rank has started
     push(&SrShared::max_of, bmax);
     push(&SrShared::low_of, blow);
@@ -482,13 +497,10 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     const float xmin = mx == INFINITY ? INFINITY : rule.min_p > 0.0 ? sr_unkey(S.kmin) : -3.4028235e38f;
     const float vmin = rule.t < 1e30 ? (float)((double)mx - 41.0 * rule.t) : -3.4028235e38f;  // weight 2^-59
     const float vzero = rule.t < 1e30 ? (float)((double)mx - 745.0 * rule.t) : -3.4028235e38f;  // weighs nothing below
-    // units of a logit as a double: a thread adds up to 2^9 of them exactly (2^52)
-    auto unit_d = [&](float v) {
-        if (mx == INFINITY) return v == mx ? SR_UNIT : 0.0;
-        const double n = rule.units_of(v, mx, vmin, S.table);
-        return v >= vzero ? n : 0.0;  // (NaN and -inf too)
+    auto unit_of = [&](float v) -> u64 {
+        if (mx == INFINITY) return v == mx ? (u64)SR_UNIT + 1 : 0;
+        return v >= vzero ? (u64)rule.units_of(v, mx, vmin, S.table) : 0;  // (not NaN, not -inf)
     };
-    auto unit_of = [&](float v) { return (u64)unit_d(v); };
     // binary32 weight, relative error below 1e-5 wherever it is not negligible
     auto rough = [&](float v) {  // (of an infinite maximum: NaN's smaller one is 0, so 1 for an infinite logit)
         return ex2(fminf(__fmul_rn(__fsub_rn(v, mx), rule.c), 0.f));
@@ -504,14 +516,14 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
         if (tid == 0) atomicAdd(&lead->n_list, (unsigned)SR_LIST + 1);
     };
     bool few = false;
-    float m1 = 0.f;  // approximate mass of the survivors
+    double m1 = 0.0;  // approximate mass of the survivors
     // (a maximum next to the lowest value, which the first pass took NaN and -inf for, or so many times T that f32 has
     // no place behind the point: the first pass's masses say nothing)
     const bool summed = online && mx > -1e38f && fabsf(__fmul_rn(mx, rule.c)) < SR_REF;
     // a rank's approximate mass, relative to the maximum's weight
     const float lift = summed ? ex2(__fmaf_rn(-mx, rule.c, ref(mx))) : 1.f;
     auto mass_at = [&](int i) {
-        return summed ? __fmul_rn(__fmul_rn(S.mass_of[i], two_to(ref(S.max_of[i]) - ref(mx))), lift) : S.mass_of[i];
+        return summed ? S.mass_of[i] * two_to(ref(S.max_of[i]) - ref(mx)) * (double)lift : S.mass_of[i];
     };
     if (summed)
         for (int i = 0; i < cs; i++) m1 += mass_at(i);
@@ -669,8 +681,8 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             u64 lo = ~0ull, hi = ~0ull;
             const bool open = has_p && rule.min_p == 0.0;  // the list does not hold all survivors
             if (open) {
-                lo = summed ? rule.need((u64)((double)m1 * (1.0 - 2e-5) * SR_UNIT)) : 0;
-                hi = summed ? rule.need((u64)((double)m1 * (1.0 + 2e-5) * SR_UNIT)) : ~0ull;
+                lo = summed ? rule.need((u64)(m1 * (1.0 - 4e-6) * SR_UNIT)) : 0;
+                hi = summed ? rule.need((u64)(m1 * (1.0 + 4e-6) * SR_UNIT)) : ~0ull;
             } else if (has_p) {
                 u64 m = 0;
                 for (int i = tid; i < n; i += SR_THREADS) m += S.wt[i];
@@ -678,26 +690,27 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             }
             if (!find_cut(n, 0, 0, lo, hi)) {
                 u64 m = 0;  // the exact mass of the whole row
+                const float from = fmaxf(xmin, vzero), top = fminf(mx, 3.4028235e38f);
                 for (int i0 = tid * E; i0 < A.vocab; i0 += SR_AHEAD * SR_THREADS * E) {
                     uint4 q[SR_AHEAD];
 #pragma unroll
                     for (int k = 0; k < SR_AHEAD; k++) q[k] = fetch(i0 + k * SR_THREADS * E);
-                    double d = 0.0;  // (exact: at most 32 logits of 2^43 + 1)
 #pragma unroll
                     for (int k = 0; k < SR_AHEAD; k++) {
                         float v[E];
                         sr_unpack<T>(q[k], v);
 #pragma unroll
-                        for (int e = 0; e < E; e++) d = __dadd_rn(d, v[e] >= xmin ? unit_d(v[e]) : 0.0);
+                        for (int e = 0; e < E; e++) {
+                            const u64 w = rule.biased_units(v[e], top, vmin, S.table) - SR_BIAS;
+                            m += v[e] >= from ? w : 0;
+                        }
                     }
-                    m += (u64)d;
                 }
                 lo = rule.need(sr_reduce(m, S.red, addu));
                 find_cut(n, 0, 0, lo, lo);
             }
             const u64 cut = S.cut, total = S.kept_mass;
-            u64 target = (u64)(rule.u * (double)total);
-            if (target >= total) target = total - 1;
+            const u64 target = rule.place(total);
             // mass before each kept entry in index order (the low halves hold ~index)
             auto draw = [&](u64 mine, int, u64 mass, u64 w) {
                 if (mass <= target && target < mass + w) {
@@ -744,7 +757,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             });
             mass = sr_reduce(mass, reinterpret_cast<float *>(S.red), addf);
             csync();  // the earlier values have been read
-            push(&SrShared::mass_of, mass);
+            push(&SrShared::mass_of, (double)mass);
             for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[0][i] = 0;
             csync();
         } else if (by_topk) {
@@ -753,16 +766,16 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             __syncthreads();
         }
         if (!summed) {
-            m1 = 0.f;
+            m1 = 0.0;
             for (int i = 0; i < cs; i++) m1 += S.mass_of[i];
         }
         // a rank's bins count its mass in units of 2^-31 of it (2^19 roundings of half a unit are 1.2e-4)
-        const float step = __fmul_rn(mass_at(rank), 0x1p-31f), per = step > 0.f ? __fdiv_rn(1.f, step) : 0.f;
+        const float step = (float)mass_at(rank) * 0x1p-31f, per = step > 0.f ? __fdiv_rn(1.f, step) : 0.f;
         // The first round's bins reach to weights of 2^-43; with top-p no further than the weights that, all vocab of
         // them, would not make up what the cut leaves out.  The last bin holds the rest.
         float lo = 0.f, hi = __fdiv_rn(30.f, rule.c * 0.6931472f);
         if (has_p) {
-            const float left = __fdiv_rn((float)A.vocab, __fmul_rn(fmaxf((float)(1.0 - rule.top_p), 1e-7f), m1));
+            const float left = __fdiv_rn((float)A.vocab, __fmul_rn(fmaxf((float)(1.0 - rule.top_p), 1e-7f), (float)m1));
             hi = fminf(hi, __fdiv_rn(fmaxf(__log2f(left), 0.f) + 0.5f, rule.c));
         }
         float m_above = 0.f;
@@ -817,7 +830,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
                 n[1] += c2.y;
                 if (has_p) {
                     const uint2 m2 = *reinterpret_cast<const uint2 *>(&o->mass[buf][2 * tid]);
-                    const float unit = __fmul_rn(mass_at(i), 0x1p-31f);
+                    const float unit = (float)mass_at(i) * 0x1p-31f;
                     m[0] += __fmul_rn((float)m2.x, unit);
                     m[1] += __fmul_rn((float)m2.y, unit);
                 }
@@ -833,7 +846,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[buf ^ 1][i] = S.mass[buf ^ 1][i] = 0;
             __syncthreads();
             // the cut is in the first bin that may complete top_k or top_p, or behind it up to the first that must
-            const float need = (float)rule.top_p * m1, slack = 2e-4f * m1;
+            const float need = (float)(rule.top_p * m1), slack = 2e-4f * (float)m1;
             unsigned nb_of[2];
             float mb_of[2];
 #pragma unroll
@@ -1002,8 +1015,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     if (tid == 0) S.where = 0;
     u64 total;
     const u64 before = sr_scan(mine, S.red, &total);
-    u64 target = (u64)(rule.u * (double)total);
-    if (target >= total) target = total - 1;
+    u64 target = rule.place(total);
     if (before <= target && target < before + mine) {
         S.where = tid;
         S.target = target - before;

@@ -207,3 +207,14 @@ def test_masks_of_the_lowest_value_and_infinities(fbctx, torch_cuda, kind, t):
     x[5, rng.random(20011) < 0.9] = lowest
     for s in (dict(k=40, p=0.9), dict(p=0.7), dict(p=0.35, k=400), dict(p=0.5, m=0.01)):
         check(*run(torch, fbctx, x, kind, t=t, u=rng.random(6), **s))
+
+
+def test_equal_weights_share_a_border(fbctx, torch_cuda):
+    """top_p times a number of equal logits that is whole keeps that many: few, many, infinite ones."""
+    torch = torch_cuda
+    for vocab, equal, value in ((64, 10, 5.0), (5000, 40, 1e3), (5000, 3000, 2.0), (200000, 1000, 7.0), (9000, 600, np.inf),
+                                (9000, 4, np.inf)):
+        x = np.full((3, vocab), -np.inf)
+        x[:, np.random.default_rng(vocab).permutation(vocab)[:equal]] = value
+        for s in (dict(p=0.5), dict(p=0.25, k=40), dict(p=0.75, m=0.5)):
+            check(*run(torch, fbctx, x, "f32", u=[0.0, 0.5, 0.99999994], **s))
