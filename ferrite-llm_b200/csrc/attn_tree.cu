@@ -1106,16 +1106,17 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 }
 
 // Joins the partials of the row groups that several CTAs hold.  grid (row groups a
-// kv head x rows_cap / 32 x HD / 16, n_kv, batch): a warp has eight rows by four
-// columns of four dimensions, so that it reads the parts by 128 bytes and writes
-// whole 32-byte sectors of the rows (with a lane a row and single values the writes
-// alone took 10 us of 16 sequences of 25 tokens, 32 heads); the parts are read in
-// batches of JOIN, all loads of one in flight together.
-constexpr int JOIN = 8;
-template <typename T, int HD>
+// kv head x rows_cap / 32 x HD / (16 COLS), n_kv, batch): a warp has eight rows by
+// four COLS columns of four dimensions, so that it reads the parts by 128 bytes and
+// writes whole 32-byte sectors of the rows (with a lane a row and single values the
+// writes alone took 10 us of 16 sequences of 25 tokens, 32 heads); the loads of
+// eight (part, column) pairs are in flight together.  Finding a group's parts costs
+// a block more than reading them, so where there are blocks enough a lane takes
+// four columns: 40.2 us for those sequences instead of 43.4.
+template <typename T, int HD, int COLS>
 __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ TreeArgs A) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int CG = HD / 16;  // column groups
+    constexpr int CG = HD / (16 * COLS), JOIN = 8 / COLS;  // column groups; parts whose loads are in flight together
     const int cgroup = blockIdx.x % CG, rest = blockIdx.x / CG;
     const int slabs = A.rows_cap / 32, slab = rest % slabs, pair = rest / slabs;
     const int b = blockIdx.z;
@@ -1145,18 +1146,22 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
     // the CTA with the group's first block keeps it as its partial 1, the others as their 0
     auto part = [&](int c) { return A.part + (2 * (int64_t)c + (c == c0)) * slot; };
     pdl_wait();
-    const int col = cgroup * 4 + (lane >> 3);
+    const int col = cgroup * 4 * COLS + (lane >> 3);  // and every 4th from there
     float M = TR_NONE, L = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 o[COLS];
+#pragma unroll
+    for (int k = 0; k < COLS; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c = c0; c <= c1; c += JOIN) {
         float2 ml[JOIN];
-        float4 v[JOIN];
+        float4 v[JOIN][COLS];
 #pragma unroll
         for (int i = 0; i < JOIN; i++)
             if (c + i <= c1) {
                 const float *p = part(c + i);
                 ml[i] = reinterpret_cast<const float2 *>(p + (int64_t)HD * A.rows_cap)[r];
-                v[i] = reinterpret_cast<const float4 *>(p)[(int64_t)col * A.rows_cap + r];
+#pragma unroll
+                for (int k = 0; k < COLS; k++)
+                    v[i][k] = reinterpret_cast<const float4 *>(p)[(int64_t)(col + 4 * k) * A.rows_cap + r];
             }
         float mn = M;
 #pragma unroll
@@ -1165,16 +1170,21 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
         const float al = exp2f(__fsub_rn(M, mn));  // (1 where nothing has been seen yet: there is nothing to scale)
         M = mn;
         L = __fmul_rn(L, al);
-        o = make_float4(__fmul_rn(o.x, al), __fmul_rn(o.y, al), __fmul_rn(o.z, al), __fmul_rn(o.w, al));
+#pragma unroll
+        for (int k = 0; k < COLS; k++)
+            o[k] = make_float4(__fmul_rn(o[k].x, al), __fmul_rn(o[k].y, al), __fmul_rn(o[k].z, al), __fmul_rn(o[k].w, al));
 #pragma unroll
         for (int i = 0; i < JOIN; i++)
             if (c + i <= c1) {
                 const float wgt = exp2f(__fsub_rn(ml[i].x, M));
                 L = __fmaf_rn(wgt, ml[i].y, L);
-                o.x = __fmaf_rn(wgt, v[i].x, o.x);
-                o.y = __fmaf_rn(wgt, v[i].y, o.y);
-                o.z = __fmaf_rn(wgt, v[i].z, o.z);
-                o.w = __fmaf_rn(wgt, v[i].w, o.w);
+#pragma unroll
+                for (int k = 0; k < COLS; k++) {
+                    o[k].x = __fmaf_rn(wgt, v[i][k].x, o[k].x);
+                    o[k].y = __fmaf_rn(wgt, v[i][k].y, o[k].y);
+                    o[k].z = __fmaf_rn(wgt, v[i][k].z, o[k].z);
+                    o[k].w = __fmaf_rn(wgt, v[i][k].w, o[k].w);
+                }
             }
     }
     if (rr >= s.n * A.group) return;
@@ -1182,17 +1192,20 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
     const int tok = tree_token(A, rr);
     T *out = static_cast<T *>(A.out) + (int64_t)(s.off + tok) * A.ot +
              (int64_t)(blockIdx.y * A.group + rr - tok * A.group) * HD + 4 * col;
-    alignas(16) T y[4];
-    tr_put(y, __fmul_rn(o.x, inv));
-    tr_put(y + 1, __fmul_rn(o.y, inv));
-    tr_put(y + 2, __fmul_rn(o.z, inv));
-    tr_put(y + 3, __fmul_rn(o.w, inv));
-    if (A.ovec) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<const uint4 *>(y);
-        else *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(y);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) out[i] = y[i];
+    for (int k = 0; k < COLS; k++) {
+        alignas(16) T y[4];
+        tr_put(y, __fmul_rn(o[k].x, inv));
+        tr_put(y + 1, __fmul_rn(o[k].y, inv));
+        tr_put(y + 2, __fmul_rn(o[k].z, inv));
+        tr_put(y + 3, __fmul_rn(o[k].w, inv));
+        if (A.ovec) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(out + 16 * k) = *reinterpret_cast<const uint4 *>(y);
+            else *reinterpret_cast<uint2 *>(out + 16 * k) = *reinterpret_cast<const uint2 *>(y);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) out[16 * k + i] = y[i];
+        }
     }
 }
 
@@ -1227,9 +1240,13 @@ static void launch_tree(fb_ctx *ctx, const TreeArgs &A, const TreePlan &plan, co
                A);
     if (!plan.split) return;
     // the join's blocks start while the attention drains and wait for it
-    launch_with(ctx->stream, ctx->pdl, k_attn_tree_join<T, HD>,
-               dim3((unsigned)(plan.pairs * (plan.rows_cap / 32) * (HD / 16)), (unsigned)A.n_kv, (unsigned)A.batch), 128,
-               0, 1, A);
+    const int64_t slabs = (int64_t)plan.pairs * (plan.rows_cap / 32);
+    auto join = [&](auto kernel, int cols) {
+        launch_with(ctx->stream, ctx->pdl, kernel,
+                    dim3((unsigned)(slabs * (HD / (16 * cols))), (unsigned)A.n_kv, (unsigned)A.batch), 128, 0, 1, A);
+    };
+    if (slabs * (HD / 64) * A.n_kv * A.batch >= 4 * ctx->num_sms) join(k_attn_tree_join<T, HD, 4>, 4);
+    else join(k_attn_tree_join<T, HD, 1>, 1);
 }
 
 static void check_tree_shape(int batch, int max_new, int n_heads, int n_kv, int head_dim, int page_size,
