@@ -47,6 +47,14 @@
 // start from zero and the second group adds it to its registers, a rounded FMA an
 // element (6.6e-7 there).  Where the tensor core does accumulate, the sums are
 // rescaled only when a row's maximum grows by more than 8 (log 2 units).
+//
+// Measured (back to back in a graph, the join included; 6559 GB/s the copy rate,
+// 1627 TFLOP/s the library's bf16 rate): 16 sequences of 25 new rows over up to
+// 4096 keys, 32 heads on 8, f16: 40.2 us, 4.5 TB/s of keys and values; 4 of 40
+// over 32000, 64 heads, bf16: 152 us, 646 TFLOP/s, where the exponentials and the
+// 64-key products (N = 64 runs at two thirds of N = 128's rate) take turns; 60 rows
+// over 4096, f32: 26.6 us, half of it the queries' way in and the join; 7 over 190:
+// 12.5 us, three blocks and the same ends.
 #include <math.h>
 
 #include <type_traits>

@@ -11,7 +11,11 @@
 // what sincospif sees, so a far position costs no precision.
 //
 // Bound: HBM (every value is read and written once); one token's call is
-// bound by the launch and two dependent loads.
+// bound by the launch and two dependent loads.  Measured (back to back in a
+// graph, 6559 GB/s the copy rate): 2048 tokens x 32 heads of 128, f16, 33.6 MB
+// in 8.2 us, 4.1 TB/s; 777 x 64 heads with half a head turned, bf16, 25.5 MB in
+// 7.7 us; one token 2.2 us.  The append: three prompts of up to 2731
+// bf16 rows of 8 heads, 56 MB in 15.3 us, 3.7 TB/s; 400 drafted rows in 6.9 us.
 #include <math.h>
 
 #include <memory>

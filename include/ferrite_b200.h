@@ -293,10 +293,12 @@ int fb_kv_append(fb_ctx *ctx, const fb_rotary *r, int dtype, const void *k_dev, 
  * nothing gets zeros; what a row does not see never reaches it, NaN and
  * infinities included.  q [n_rows][n_heads][head_dim] and out of the same
  * shape and dtype have token strides, heads contiguous.  Scores and sums
- * in f32; q and the probabilities enter the tensor cores as fp16 high and low
- * parts.  mask_words >= ceil(max_new / 32).  The workspace is the caller's
- * (fb_attn_tree_workspace bytes for the same sizes, 16-byte aligned, contents
- * ignored and clobbered): calls that may overlap need one each. */
+ * in f32; with dtype FB_F32 q and the probabilities enter the tensor cores as
+ * fp16 high and low parts, otherwise as one fp16 value each (bf16 q scaled
+ * into its range).  mask_words >= ceil(max_new / 32).  The workspace is the
+ * caller's (fb_attn_tree_workspace bytes for the same sizes, any dtype,
+ * 16-byte aligned, contents ignored and clobbered): calls that may overlap
+ * need one each. */
 int fb_attn_tree_workspace(fb_ctx *ctx, int batch, int max_new, int n_heads, int n_kv_heads, int head_dim,
                            int page_size, int max_seq_len, int64_t *bytes);
 int fb_attn_tree(fb_ctx *ctx, int dtype, const void *q_dev, int64_t q_token_stride, const void *k_pages_dev,
