@@ -329,9 +329,10 @@ template <typename T, int HD> struct TreeCfg {
     static constexpr uint32_t KV_BYTES = TR_KB * HD * 2;            // one block of K or V
     static constexpr int TILES = LO ? 1 : 2;  // row tiles a group
     static constexpr size_t SMEM = 1024 + TILES * (size_t)TILE_BYTES + 2 * ST * (size_t)KV_BYTES;
-    static_assert(SMEM + 2048 <= 227 * 1024, "tree attention stages must fit");
+    static_assert(SMEM + (LO ? 5120 : 2048) <= 227 * 1024, "tree attention stages must fit");
 };
-constexpr uint32_t TR_TMEM_COLS = 512;  // scores (group, buffer) at 128 g + 64 buffer, O of group (f32: buffer) g at 256 + HD g
+// Tensor memory columns: scores (group, buffer) at 128 g + 64 buffer, O of group (f32: buffer) g at 256 + HD g.
+constexpr uint32_t TR_TMEM_COLS = 512;  
 constexpr uint32_t TR_O_COL = 256;
 
 // Bounded wait (~1 s) for waits that are short in the steady state: polls without the suspension of
@@ -538,7 +539,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
                 for (int i = 0; i < 2 * (TR_KB / 16); i++) {  // 16 keys: 8 columns of fp16 pairs; low parts first
                     const int ks = i % (TR_KB / 16);
-                    umma_f16_tmem(d, p + (i < TR_KB / 16 ? 32 : 0) + 8 * ks, vd + ks * (2048 >> 4), IDESC_O, i > 0 ? 1u : 0u);
+                    umma_f16_tmem(d, p + (i < TR_KB / 16 ? 32 : 0) + 8 * ks, vd + ks * (2048 >> 4), IDESC_O,
+                                  i > 0 ? 1u : 0u);
                 }
                 umma_commit(&o_done[0][c & 1]);
                 umma_commit(&v_empty[st]);
@@ -603,9 +605,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ks++) {  // 16 dims: 16 rows of the dim-major pages
                         const uint32_t qo = ((uint32_t)(ks >> 2) * (TR_ROWS * 128) + (uint32_t)(ks & 3) * 32) >> 4;
-                        const uint64_t db = kd + ks * (16 * PAGE * 2 >> 4);
-                        umma_f16_desc(d, dq + qo, db, IDESC_S, ks > 0 ? 1u : 0u);
-                        if (C::LO) umma_f16_desc(d, dq + (C::Q_BYTES >> 4) + qo, db, IDESC_S, 1u);
+                        umma_f16_desc(d, dq + qo, kd + ks * (16 * PAGE * 2 >> 4), IDESC_S, ks > 0 ? 1u : 0u);
                     }
                     umma_commit(&s_full[g][j & 1]);
                     release(&k_empty[st]);
@@ -623,11 +623,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     if (!tr_wait(&p_full[g][j & 1], (uint32_t)(j >> 1) & 1u)) return false;
                     tc_fence_after();
 #pragma unroll
-                    for (int ks = 0; ks < TR_KB / 16; ks++) {  // 16 keys: 8 columns of fp16 pairs
-                        const uint64_t db = vd + ks * (2048 >> 4);
-                        umma_f16_tmem(t_o, p + 8 * ks, db, IDESC_O, (k > 0 || ks > 0) ? 1u : 0u);
-                        if (C::LO) umma_f16_tmem(t_o, p + 32 + 8 * ks, db, IDESC_O, 1u);
-                    }
+                    for (int ks = 0; ks < TR_KB / 16; ks++)  // 16 keys: 8 columns of fp16 pairs
+                        umma_f16_tmem(t_o, p + 8 * ks, vd + ks * (2048 >> 4), IDESC_O, (k > 0 || ks > 0) ? 1u : 0u);
                     umma_commit(&o_done[g][j & 1]);
                     release(&v_empty[st]);
                     forward(vf, vph);
@@ -655,10 +652,10 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
         uint32_t npair = 0;  // uses of pair_bar[qd]
         bool ok = true;
         int cb = 0, jb = 0, seg = 0;  // blocks and this group's jobs of the segments before
-        // The group's queries as fp16 parts scaled by 2^-e: HD / 8 lanes a row, the first 8 (or 4) warps share the rows.  f32: two
-        // batches of loads through registers (128 KB for two tiles: L2's rate, shared by all CTAs, bounds them).  16-bit:
-        // copied as they are into their places, all copies in flight together, and (bf16) turned in place by the
-        // thread that copied them, in rolled loops: code that runs once a segment arrives more slowly than it executes.
+        // The group's queries as fp16 parts scaled by 2^-e: HD / 8 lanes a row, the first 8 (or 4) warps share the
+        // rows.  f32: batches of eight loads through registers.  16-bit: copied as they are into their places, all
+        // copies in flight together, and (bf16) turned in place by the thread that copied them, in rolled loops: code
+        // that runs once a segment arrives more slowly than it executes.
         auto load_q = [&](const TreeWalk &t, int sg, int warps) {
             constexpr int LPR = HD / 8, RPI = 32 / LPR;
             const int rows = t.rows(A), each = (t.both() ? TR_PAIR : TR_ROWS) / warps, d = (lane % LPR) * 8;
@@ -730,7 +727,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                         uint4 *dst = reinterpret_cast<uint4 *>(place(rr));
                         if constexpr (half) {
                             const uint4 q = *dst;
-                            *dst = make_uint4(q.x ^ 0x80008000u, q.y ^ 0x80008000u, q.z ^ 0x80008000u, q.w ^ 0x80008000u);
+                            constexpr uint32_t S = 0x80008000u;
+                            *dst = make_uint4(q.x ^ S, q.y ^ S, q.z ^ S, q.w ^ S);
                         } else {
                             float x[8];
                             uint4 lo;
@@ -1180,7 +1178,8 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
         L = __fmul_rn(L, al);
 #pragma unroll
         for (int k = 0; k < COLS; k++)
-            o[k] = make_float4(__fmul_rn(o[k].x, al), __fmul_rn(o[k].y, al), __fmul_rn(o[k].z, al), __fmul_rn(o[k].w, al));
+            o[k] = make_float4(__fmul_rn(o[k].x, al), __fmul_rn(o[k].y, al), __fmul_rn(o[k].z, al),
+                               __fmul_rn(o[k].w, al));
 #pragma unroll
         for (int i = 0; i < JOIN; i++)
             if (c + i <= c1) {
@@ -1208,8 +1207,8 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
         tr_put(y + 2, __fmul_rn(o[k].z, inv));
         tr_put(y + 3, __fmul_rn(o[k].w, inv));
         if (A.ovec) {
-            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(out + 16 * k) = *reinterpret_cast<const uint4 *>(y);
-            else *reinterpret_cast<uint2 *>(out + 16 * k) = *reinterpret_cast<const uint2 *>(y);
+            using W = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+            *reinterpret_cast<W *>(out + 16 * k) = *reinterpret_cast<const W *>(y);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) out[16 * k + i] = y[i];
@@ -1228,7 +1227,8 @@ static TreePlan tree_plan(const fb_ctx *ctx, int batch, int max_new, int n_heads
     const int64_t rows = (int64_t)max_new * (n_heads / n_kv);
     const int64_t pairs = (rows + grows - 1) / grows, blocks = (max_seq_len + TR_KB - 1) / TR_KB;
     const int64_t groups = pairs * n_kv * batch;
-    FB_REQUIRE(groups * (2 * blocks + TR_SWITCH) < ((int64_t)1 << 31) - 4096 && pairs <= 65535, "attn_tree: batch too large");
+    FB_REQUIRE(groups * (2 * blocks + TR_SWITCH) < ((int64_t)1 << 31) - 4096 && pairs <= 65535,
+               "attn_tree: batch too large");
     FB_REQUIRE((rows + TR_PAIR) * (n_heads / n_kv) < ((int64_t)1 << 32), "attn_tree: too many rows");
     p.split = blocks > TR_WHOLE;
     const int64_t units = 2 * groups * (p.split ? blocks : 1);
@@ -1244,8 +1244,8 @@ static void launch_tree(fb_ctx *ctx, const TreeArgs &A, const TreePlan &plan, co
                         const CUtensorMap &vmap) {
     constexpr size_t smem = TreeCfg<T, HD>::SMEM;
     FB_CUDA(cudaFuncSetAttribute(k_attn_tree<T, HD, PAGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    launch_with(ctx->stream, ctx->pdl, k_attn_tree<T, HD, PAGE>, dim3((unsigned)plan.ctas), TR_THREADS, smem, 1, kmap, vmap,
-               A);
+    launch_with(ctx->stream, ctx->pdl, k_attn_tree<T, HD, PAGE>, dim3((unsigned)plan.ctas), TR_THREADS, smem, 1, kmap,
+               vmap, A);
     if (!plan.split) return;
     // the join's blocks start while the attention drains and wait for it
     const int64_t slabs = (int64_t)plan.pairs * (plan.rows_cap / 32);
@@ -1308,6 +1308,7 @@ int fb_attn_tree(fb_ctx *ctx, int dtype, const void *q_dev, int64_t q_token_stri
         FB_REQUIRE(ctx && q_dev && k_pages_dev && v_pages_dev && block_table_dev && row_offsets_dev && seq_lens_dev &&
                        out_dev,
                    "null argument");
+        FB_REQUIRE(q_dev != out_dev, "attn_tree: q and out must not overlap");
         const size_t esz = dtype == FB_F32 ? 4 : 2;
         FB_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) & (esz - 1)) == 0 &&
                        (((uintptr_t)row_offsets_dev | (uintptr_t)seq_lens_dev | (uintptr_t)block_table_dev |

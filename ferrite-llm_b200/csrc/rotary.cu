@@ -521,7 +521,7 @@ int fb_rotary_create(const fb_rotary_config *cfg, fb_rotary **out) {
         FB_REQUIRE(isfinite(c.theta) && c.theta > 1.0, "rotary: theta must be above 1");
         FB_REQUIRE(isfinite(c.amplitude) && c.amplitude >= 0.0, "rotary: amplitude must not be negative");
         if (c.scaling != FB_ROTARY_PLAIN)
-            FB_REQUIRE(isfinite(c.factor) && c.factor > 0.0, "rotary: factor must be positive");
+            FB_REQUIRE(isfinite(c.factor) && c.factor >= 1e-6, "rotary: factor must be positive, 1e-6 at least");
         if (c.scaling == FB_ROTARY_BANDS || c.scaling == FB_ROTARY_YARN) {
             FB_REQUIRE(c.orig_ctx >= 1, "rotary: orig_ctx must be positive");
             FB_REQUIRE(isfinite(c.high) && c.low > 0.0 && c.high > c.low, "rotary: need 0 < low < high");
@@ -578,7 +578,10 @@ int fb_rotary_apply(fb_ctx *ctx, const fb_rotary *r, int dtype, const void *x_de
         FB_REQUIRE(r->cfg.rot_dim <= head_dim, "rotary_apply: rot_dim exceeds head_dim");
         FB_REQUIRE(x_token_stride >= 0 && x_head_stride >= 0 && y_token_stride >= 0 && y_head_stride >= 0,
                    "rotary_apply: strides must not be negative");
-        FB_REQUIRE((n_heads == 1 || y_head_stride >= head_dim) && (n_tok <= 1 || y_token_stride >= head_dim),
+        // one stride steps over all that the other spans
+        FB_REQUIRE((n_heads == 1 || y_head_stride >= head_dim) && (n_tok <= 1 || y_token_stride >= head_dim) &&
+                       (n_heads == 1 || n_tok <= 1 || (y_token_stride - head_dim) / (n_heads - 1) >= y_head_stride ||
+                        (y_head_stride - head_dim) / (n_tok - 1) >= y_token_stride),
                    "rotary_apply: rows of y overlap");
         FB_REQUIRE(x_dev != y_dev || (x_token_stride == y_token_stride && x_head_stride == y_head_stride),
                    "rotary_apply: in place needs equal strides");

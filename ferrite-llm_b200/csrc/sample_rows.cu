@@ -114,7 +114,8 @@ __device__ __forceinline__ uint32_t sr_max32(uint32_t a, uint32_t b, __nv_bfloat
     return *reinterpret_cast<const uint32_t *>(&m);
 }
 template <typename T> __device__ __forceinline__ uint4 sr_max(const uint4 &a, const uint4 &b) {
-    return make_uint4(sr_max32(a.x, b.x, T{}), sr_max32(a.y, b.y, T{}), sr_max32(a.z, b.z, T{}), sr_max32(a.w, b.w, T{}));
+    return make_uint4(sr_max32(a.x, b.x, T{}), sr_max32(a.y, b.y, T{}), sr_max32(a.z, b.z, T{}),
+                      sr_max32(a.w, b.w, T{}));
 }
 // The lowest finite f32 or bf16 in every place.
 template <typename T> __device__ __forceinline__ uint4 sr_lowest() {
@@ -275,7 +276,8 @@ struct SrShared {
     uint32_t kmin;
 };
 
-static_assert(SR_AHEAD == 4 && SR_BINS == 2 * SR_THREADS && SR_CLUSTER * SR_WARPS <= SR_THREADS, "a sum of four, a thread two bins, a thread a run");
+static_assert(SR_AHEAD == 4 && SR_BINS == 2 * SR_THREADS && SR_CLUSTER * SR_WARPS <= SR_THREADS,
+              "a sum of four, a thread two bins, a thread a run");
 
 template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_rows(const SampleRowsArgs A) {
     constexpr int E = SR_E<T>;
@@ -336,9 +338,9 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
 
     // ---- the first pass: the groups' maxima, and for top-p without min-p the approximate mass.  Each thread's is
     // relative to 2^ref of its own running maximum, ref an integer (within SR_REF): x c - ref is one rounding, and a
-    // change of ref exact.  What it is off by: 2^-22 a term (ex2), 2^-24 |x c - ref| of it and half as much for c (together 1e-6, as the
-    // weights of a row are below 17 of these on average), 10 2^-24 for a batch's sum; from there on it is a double.
-    // 2.3e-6 with the last factors.
+    // change of ref exact.  What it is off by: 2^-22 a term (ex2), 2^-24 |x c - ref| of it and half as much for c
+    // (together 1e-6: |x c - ref| is below 17 on average over a row's mass), 10 2^-24 for a batch's sum; from there on
+    // it is a double.  2.3e-6 with the last factors.
     const bool by_topk = rule.top_k > 0 && rule.top_k <= SR_TOPK && rule.min_p == 0.0 && !rule.greedy;
     const bool has_p = rule.top_p < 1.0, cuts = rule.top_k > 0 || has_p;
     if (tid < 16) S.table[tid] = exp2((double)tid * 0.0625);
@@ -788,7 +790,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             const float width = hi - lo;
             const float inv = width > 0.f && width < INFINITY ? __fdiv_rn(1.f, width) : 0.f;
             const float from = __fsub_rn(mx, lo);
-            auto bin = [&](float v) {  // (a number of 23 bits behind 2^23; bin 0 of an infinite maximum: NaN saturates to 0)
+            auto bin = [&](float v) {  // (the low bits of 2^23 + bin; an infinite maximum's NaN saturates to 0)
                 const float t = __saturatef(__fmul_rn(__fsub_rn(from, v), inv));
                 return (int)(__float_as_uint(__fmaf_rd(t, (float)(SR_BINS - 1), 8388608.f)) - 0x4b000000u);
             };
@@ -813,7 +815,8 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
                         if (has_p) atomicAdd(&S.mass[buf][b[e]], u[e]);
                     }
             });
-            n_last = sr_reduce(n_last, reinterpret_cast<unsigned *>(S.red), [](unsigned a, unsigned b) { return a + b; });
+            n_last = sr_reduce(n_last, reinterpret_cast<unsigned *>(S.red),
+                               [](unsigned a, unsigned b) { return a + b; });
             m_last = sr_reduce(m_last, reinterpret_cast<float *>(S.red), addf);
             if (tid == 0) {
                 S.cnt[buf][SR_BINS - 1] = n_last;

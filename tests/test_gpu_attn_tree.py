@@ -309,6 +309,16 @@ def test_same_bits_over_many_runs(fbctx, torch_cuda, kind, page, qheads):
     assert fbctx.error_word() == 0
 
 
+def test_in_place_is_refused(fbctx, torch_cuda):
+    torch = torch_cuda
+    rng = np.random.default_rng(18)
+    B = Batch(rng, [2], [70], 2, 64, 64)
+    qd, _ = rounded(torch, rng.normal(0, 1, (2, 4, 64)), "f32")
+    c = Call(torch, fbctx, B, qd, None, "f32", 4, out=qd)
+    with pytest.raises(fb.FerriteError, match="overlap"):
+        c.go(0.1)
+
+
 def test_sums_of_long_contexts(fbctx, torch_cuda):
     """Some seventy blocks of keys to an SM: what a matrix instruction drops of a running sum must not add up over them."""
     torch = torch_cuda

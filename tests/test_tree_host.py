@@ -127,6 +127,19 @@ def test_sample_rows_refuses(over, msg):
         fb.sample_rows(NoContext, **sample_args(**over))
 
 
+@pytest.mark.parametrize("tok,head,fits", [(512, 128, True), (128, 256, True), (511, 128, False), (128, 255, False),
+                                           (256, 128, False), (1 << 40, 128, True), (200, 150, False)])
+def test_rotary_rows_that_overlap(tok, head, fits):
+    """Two tokens of four heads, 128 wide: nested strides reach the next check, others are refused."""
+    with pytest.raises(fb.FerriteError, match="null argument" if fits else "overlap"):
+        fb.rotary_apply(NoContext, fb.Rotary(64, 1e4), **rotary_args(y_token_stride=tok, y_head_stride=head))
+
+
+def test_rotary_refuses_a_vanishing_factor():
+    with pytest.raises(fb.FerriteError, match="factor"):
+        fb.Rotary(64, 1e4, scaling=1, factor=1e-300)
+
+
 def test_nothing_to_do_needs_no_device():
     fb.rotary_apply(NoContext, fb.Rotary(64, 1e4), **rotary_args(n_tok=0))
     fb.kv_append(NoContext, None, **append_args(n_rows=0))
