@@ -315,7 +315,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1)
             if (lane == 0) mbar_arrive(&p_full[sb]);
         }
         // ---- O / l once the last P V has landed (l = the two halves' sums)
-        if (okw) okw = mbar_wait_bounded(&o_done, (uint32_t)(nkb - 1) & 1u);
+        // (by p_free, of which this warp has met every phase but the last: of o_done the phase of block nkb - 2 may be
+        // open too, and a wait for nkb - 1's parity would pass on nkb - 3's)
+        if (okw) okw = mbar_wait_bounded(&p_free[(nkb - 1) & 1], (uint32_t)((nkb - 1) >> 1) & 1u);
         if (okw) {
             s_l[ch][r] = l;
             mbar_arrive(&l_bar[qd]);
