@@ -327,3 +327,15 @@ def test_sums_of_long_contexts(fbctx, torch_cuda):
     qd, q = rounded(torch, rng.normal(0, 1, (3, 16, 128)), "f32")
     got = Call(torch, fbctx, B, qd, None, "f32", 16).result(0.09)
     check(got, attention(q, B, None, 0.09), q, B, 0.09, "f32")
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_scales_of_either_sign_and_none(fbctx, torch_cuda, kind):
+    torch = torch_cuda
+    rng = np.random.default_rng(19)
+    B = Batch(rng, [9, 2], [500, 64], 2, 128, 64)
+    qd, q = rounded(torch, rng.normal(0, 1, (11, 8, 128)), kind)
+    mask = tree_mask(rng, B.new, 1)
+    for scale in (-0.09, 0.0):
+        got = Call(torch, fbctx, B, qd, mask, kind, 8).result(scale)
+        check(got, attention(q, B, mask, scale), q, B, abs(scale), kind)
