@@ -218,3 +218,14 @@ def test_equal_weights_share_a_border(fbctx, torch_cuda):
         x[:, np.random.default_rng(vocab).permutation(vocab)[:equal]] = value
         for s in (dict(p=0.5), dict(p=0.25, k=40), dict(p=0.75, m=0.5)):
             check(*run(torch, fbctx, x, "f32", u=[0.0, 0.5, 0.99999994], **s))
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 151936), (30, 20000), (500, 3001), (3, 700)])
+def test_top_k_among_many_survivors_of_min_p(fbctx, torch_cuda, rows, vocab):
+    rng = np.random.default_rng(vocab)
+    x = rng.normal(0, 1, (rows, vocab))
+    x[:, ::5] = -np.inf
+    x[rows // 2, 1:] = 0.25  # equal ones
+    for s in (dict(k=1, m=0.02), dict(k=50, m=0.01, t=2.0), dict(k=256, m=1e-4), dict(k=257, m=0.001), dict(k=40, m=0.3, t=3.0),
+              dict(k=20, m=0.01, p=0.5)):
+        check(*run(torch_cuda, fbctx, x, "bf16", u=rng.random(rows), **s))
