@@ -15,7 +15,7 @@
 // graph, 6559 GB/s the copy rate): 2048 tokens x 32 heads of 128, f16, 33.6 MB
 // in 8.2 us, 4.1 TB/s; 777 x 64 heads with half a head turned, bf16, 25.5 MB in
 // 7.7 us; one token 2.2 us.  The append: three prompts of up to 2731
-// bf16 rows of 8 heads, 56 MB in 15.3 us, 3.7 TB/s; 400 drafted rows in 6.9 us.
+// bf16 rows of 8 heads, 56 MB in 14.3 us, 3.9 TB/s; 400 drafted rows in 6.4 us.
 #include <math.h>
 
 #include <memory>
@@ -310,7 +310,7 @@ template <typename T> struct Raw8 {
 // exchanged by the dimension's chunk (both the scattered 2-byte stores and the
 // rows' 16-byte loads then touch every bank once).  The pages are dim-major: 8
 // lanes write the 128 bytes of a dimension's 64 tokens.
-constexpr int KVA_HEADS = 4;
+constexpr int KVA_HEADS = 2;  // (three prompts: 14.3 us; 15.3 with 4, 16.0 with 1)
 template <typename T, int HD, int PAGE, int MODE>
 __global__ void __launch_bounds__(KVA_THREADS)
     k_kv_append(const __grid_constant__ RotaryParams P, const __grid_constant__ AppendArgs A) {
@@ -337,6 +337,15 @@ __global__ void __launch_bounds__(KVA_THREADS)
             tile[d * PAGE + (((t >> 3) ^ (c & (CH - 1))) << 3) + (t & 7)] = __float2half_rn(v[i]);
         }
     };
+    // V rows, as they come (first: K waits for its angles anyway)
+    for (int e = threadIdx.x; e < cnt * nh * (HD / 8); e += KVA_THREADS) {
+        const int c = e % (HD / 8), q = e / (HD / 8), h = q % nh, t = q / nh;
+        Raw8<T> raw;
+        raw.load(vr + t * A.vt + h * HD + 8 * c);
+        float v[8];
+        raw.get(v);
+        *reinterpret_cast<uint4 *>(vp + (int64_t)h * HD * PAGE + t * HD + 8 * c) = pack8(v);
+    }
     for (int wt = warp; wt < ug * tg; wt += KVA_THREADS / 32) {
         const int u = (wt % ug) * 4 + (lane & 3), t = (wt / ug) * 8 + (lane >> 2);
         if (u >= nu || t >= cnt) continue;
@@ -384,15 +393,6 @@ __global__ void __launch_bounds__(KVA_THREADS)
                 if (MODE == 1 && pair) put(h + k, c2, t0 + t, y);
             }
         }
-    }
-    // V rows, as they come
-    for (int e = threadIdx.x; e < cnt * nh * (HD / 8); e += KVA_THREADS) {
-        const int c = e % (HD / 8), q = e / (HD / 8), h = q % nh, t = q / nh;
-        Raw8<T> raw;
-        raw.load(vr + t * A.vt + h * HD + 8 * c);
-        float v[8];
-        raw.get(v);
-        *reinterpret_cast<uint4 *>(vp + (int64_t)h * HD * PAGE + t * HD + 8 * c) = pack8(v);
     }
     __syncthreads();
     for (int e = threadIdx.x; e < nh * HD * CH; e += KVA_THREADS) {
