@@ -765,17 +765,19 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     if (cuts) {
         // lowest survivor, and the approximate mass, as far as the first pass has not found them
         if (!summed) {
-            float mass = 0.f;
+            double mass = 0.0;
             stream([&](float (&v)[E], int) {
+                float sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
                     const float p = rough(v[e]);
-                    mass += v[e] >= xmin ? p : 0.f;
+                    sum += v[e] >= xmin ? p : 0.f;
                 }
+                mass += (double)sum;
             });
-            mass = sr_reduce(mass, reinterpret_cast<float *>(S.red), addf);
+            mass = sr_reduce(mass, reinterpret_cast<double *>(S.red), [](double a, double b) { return a + b; });
             csync();  // the earlier values have been read
-            push(&SrShared::mass_of, (double)mass);
+            push(&SrShared::mass_of, mass);
             for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[0][i] = 0;
             csync();
         } else if (then_topk) {
@@ -787,7 +789,8 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             m1 = 0.0;
             for (int i = 0; i < cs; i++) m1 += S.mass_of[i];
         }
-        // a rank's bins count its mass in units of 2^-31 of it (2^19 roundings of half a unit are 1.2e-4)
+        // a rank's bins count its mass in units of 2^-31 of it (2^19 roundings of half a unit are 1.2e-4, the last bin's
+        // 512 f32 additions 3e-5: below the slack)
         const float step = (float)mass_at(rank) * 0x1p-31f, per = step > 0.f ? __fdiv_rn(1.f, step) : 0.f;
         // The first round's bins reach to weights of 2^-43; with top-p no further than the weights that, all vocab of
         // them, would not make up what the cut leaves out.  The last bin holds the rest.
@@ -811,15 +814,17 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             stream([&](float (&v)[E], int) {
                 int b[E];
                 unsigned u[E];
+                float m_here = 0.f;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
                     const float p = has_p ? rough(v[e]) : 0.f;
                     const int at = bin(v[e]);
                     b[e] = side(v[e]) == 0 ? at : SR_BINS;
-                    m_last += b[e] == SR_BINS - 1 ? p : 0.f;
+                    m_here += b[e] == SR_BINS - 1 ? p : 0.f;
                     n_last += b[e] == SR_BINS - 1;
                     u[e] = __float2uint_rn(__fmul_rn(p, per));
                 }
+                m_last += m_here;
 #pragma unroll
                 for (int e = 0; e < E; e++)
                     if (b[e] < SR_BINS - 1) {
