@@ -38,8 +38,11 @@
 // enters as fp16 high + low parts where it is f32 (f16 and bf16 queries fit the
 // high part); the probabilities are kept 2^7 above the running maximum's unit (at
 // most 2^15).  For f32 results they are fp16 high + low parts too, 22 bits down
-// to 2^-21 of the largest; for f16 and bf16 results the high part alone, whose
-// half step of 2^-12 averages out over the keys below the result's own rounding.
+// to 2^-21 of the largest; for f16 and bf16 results the high part alone, off by
+// 2^-11 of it at most: below half a step of a bf16 result, and for f16 results,
+// whose own rounding is as large, the sum is that of the rounded probabilities,
+// so that a row that one key dominates is not off by that key's (1.4 times the
+// output rounding's error in the 2-norm; both parts would take twice the products).
 // Products and sums are f32.  The tensor core truncates its sums, by 2^-25 of
 // them on average at each instruction, always towards zero: over 100 blocks that
 // is 10^-5 (7.4e-6 measured in the 2-norm at 30000 keys), nothing beside a 16-bit
@@ -827,9 +830,14 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             for (int t = 0; t < 32; t++) {
                 const float pa = exp2_approx(__fmaf_rn(__uint_as_float(sv[2 * t]), u, ref));
                 const float pb = exp2_approx(__fmaf_rn(__uint_as_float(sv[2 * t + 1]), u, ref));
-                l4[t & 3] = __fadd_rn(l4[t & 3], __fadd_rn(pa, pb));
                 const __half2 h2 = __floats2half2_rn(pa, pb);
                 hi[t] = *reinterpret_cast<const uint32_t *>(&h2);
+                if (std::is_same<T, __half>::value) {  // (the sum of what the products see)
+                    const float2 hf = __half22float2(h2);
+                    l4[t & 3] = __fadd_rn(l4[t & 3], __fadd_rn(hf.x, hf.y));
+                } else {
+                    l4[t & 3] = __fadd_rn(l4[t & 3], __fadd_rn(pa, pb));
+                }
                 if (C::LO) {
                     const float2 hf = __half22float2(h2);
                     const __half2 q2 = __floats2half2_rn(__fsub_rn(pa, hf.x), __fsub_rn(pb, hf.y));
