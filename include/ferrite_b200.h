@@ -319,8 +319,10 @@ int fb_attn_tree(fb_ctx *ctx, int dtype, const void *q_dev, int64_t q_token_stri
  * top_p, all of them for min_p).  u is taken into [0, 1]; NaN settings count
  * as off and NaN u as 0.  NaN logits are never selected, -inf ones only by T
  * <= 0; +inf ones share the whole mass.  A row without any candidate gets token
- * -1 and probability 0.  Masses are summed in 64-bit integers (weights in
- * units of 2^-43), so results do not depend on the order of the work.
+ * -1 and probability 0.  Masses are summed in 64-bit integers, so results do
+ * not depend on the order of the work: a weight is its whole units of 2^-43
+ * and one more (none where exp is 0), so that every kept token can be drawn,
+ * and a border that lies within that of two tokens may fall to either.
  * probs_dev (may be NULL): the token's probability among the kept ones.
  * row_stride in elements; vocab 1..524288. */
 int fb_sample_rows(fb_ctx *ctx, int dtype, const void *logits_dev, int64_t row_stride, int64_t rows, int vocab,
