@@ -7,7 +7,7 @@
 //
 // The (drafted token, query head of the group) pairs of a sequence and kv head
 // are the rows of one matrix product, up to 256 rows a group (two tiles of 128,
-// the MMA's M): they share every key and value that is read.  A verified tree of
+// the MMA's M; f32: one): they share every key and value that is read.  A verified tree of
 // 32 tokens with 4 heads a kv head needs 128 multiplications a byte of cache, so
 // up to one full tile the bound is HBM (4 head_dim bytes a key and kv head),
 // beyond it the tensor cores.
