@@ -1137,7 +1137,12 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
     TreeSeq s;
     s.load(A, b);
     const int row0 = pair * A.grows + 32 * slab;
-    if (row0 >= s.n * A.group) return;
+    // (a block without work waits too: what is behind this kernel on the stream waits for it alone, so it must not end
+    // before the attention has)
+    if (row0 >= s.n * A.group) {
+        pdl_wait();
+        return;
+    }
     // units before this sequence, and in all
     TreeTotal t{}, before{};
     for (int i = lane; i < A.batch; i += 32) {
@@ -1154,7 +1159,10 @@ __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ 
     const int gs = before.units + before.groups * lead + blockIdx.y * s.head_units(A, lead) +
                    pair * (s.full * s.blocks + lead) + lead;
     const int c0 = gs / quota, c1 = (gs + wt * (s.blocks - 1)) / quota;          // CTAs of its first and last block
-    if (c0 == c1) return;  // written by its CTA
+    if (c0 == c1) {  // written by its CTA
+        pdl_wait();
+        return;
+    }
     const int rr = row0 + 8 * warp + (lane & 7), r = rr - pair * A.grows;
     const int64_t slot = (int64_t)(HD + 2) * A.rows_cap;
     // the CTA with the group's first block keeps it as its partial 1, the others as their 0

@@ -69,9 +69,12 @@ struct DeviceGuard {
     DeviceGuard &operator=(const DeviceGuard &) = delete;
 };
 
-// Launches a kernel with its attributes.  pdl: it reads and writes nothing before
-// its pdl_wait(), so it may be brought up while its predecessor on the stream
-// still runs (fb_ctx_set_pdl); it calls pdl_launch() after that wait, so that what
+// Launches a kernel with its attributes.  pdl: it writes nothing before its
+// pdl_wait() and reads only what was complete before its predecessor on the stream
+// called pdl_launch(), so it may be brought up while that one still runs
+// (fb_ctx_set_pdl).  Every block calls pdl_wait(), those without work too: what
+// comes next waits for this kernel alone, which therefore must not end before its
+// predecessor.  It calls pdl_launch(), if at all, after that wait, so that what
 // comes before it is complete for its dependents too.  cluster > 1: CTAs a
 // thread-block cluster.
 template <class... P, class... A>
