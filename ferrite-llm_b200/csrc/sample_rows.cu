@@ -1087,7 +1087,8 @@ template <typename T> static void launch_sample_rows(fb_ctx *ctx, SampleRowsArgs
     A.gsteps = SR_AHEAD * ((A.steps + SR_AHEAD * SR_GROUPS - 1) / (SR_AHEAD * SR_GROUPS));
     const size_t smem = (size_t)((A.steps + A.gsteps - 1) / A.gsteps) * SR_THREADS * 4;
     auto kernel = k_sample_rows<T>;
-    FB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // (the kernel's bound, not this call's size: the attribute belongs to the process, whose other threads launch other sizes)
+    FB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SR_GROUPS * SR_THREADS * 4));
     if (cs > 8) FB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     launch_with(ctx->stream, false, kernel, dim3((unsigned)(rows * cs)), SR_THREADS, smem, (unsigned)cs, A);
 }
