@@ -481,6 +481,11 @@ __global__ void __launch_bounds__(KVA_THREADS)
     }
 }
 
+// Shared memory of the general form: f32 rows and angles.
+constexpr size_t append_any_bytes(int page, int hd, int rot) {
+    return (size_t)(page * (hd + 1) + 1) * 4 + (size_t)page * (rot / 2 + 1) * 8;
+}
+
 template <typename T, int HD, int PAGE>
 static void launch_append(fb_ctx *ctx, const RotaryParams &P, AppendArgs A, int batch) {
     const int tiles = (A.max_new + PAGE - 2) / PAGE + 1;
@@ -492,15 +497,18 @@ static void launch_append(fb_ctx *ctx, const RotaryParams &P, AppendArgs A, int 
     const bool fast = A.vec && P.rot % (P.mode == 1 ? 16 : 8) == 0;
     if (fast && A.heads_per_block > KVA_HEADS) A.heads_per_block = KVA_HEADS;
     const dim3 grid((unsigned)tiles, (unsigned)((A.n_kv + A.heads_per_block - 1) / A.heads_per_block), (unsigned)batch);
-    auto go = [&](auto kernel, size_t smem) {
-        FB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // most: the kernel's bound for its shared-memory limit, not this call's size: the limit belongs to the process, whose
+    // other threads launch other sizes
+    auto go = [&](auto kernel, size_t smem, size_t most) {
+        FB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
         kernel<<<grid, KVA_THREADS, smem, ctx->stream>>>(P, A);
         FB_CUDA(cudaGetLastError());
     };
     const size_t tile = (size_t)A.heads_per_block * HD * PAGE * 2;
-    if (!fast) go(k_kv_append_any<T, HD>, (size_t)(PAGE * (HD + 1) + 1) * 4 + (size_t)PAGE * (P.rot / 2 + 1) * 8);
-    else if (P.mode == 1) go(k_kv_append<T, HD, PAGE, 1>, tile);
-    else go(k_kv_append<T, HD, PAGE, 0>, tile);
+    constexpr size_t tiles_most = (size_t)KVA_HEADS * HD * PAGE * 2;
+    if (!fast) go(k_kv_append_any<T, HD>, append_any_bytes(PAGE, HD, P.rot), append_any_bytes(64, HD, HD));
+    else if (P.mode == 1) go(k_kv_append<T, HD, PAGE, 1>, tile, tiles_most);
+    else go(k_kv_append<T, HD, PAGE, 0>, tile, tiles_most);
 }
 
 }  // namespace fb

@@ -1,6 +1,6 @@
-"""Host threads with a context each call the row sampler with sizes of their own
-at the same time: the kernel's launch limits belong to the process, so a small
-call must not take away what a large one needs."""
+"""Host threads with a context each call the row sampler and the cache append
+with sizes of their own at the same time: a kernel's launch limits belong to the
+process, so a small call must not take away what a large one needs."""
 import threading
 
 import numpy as np
@@ -54,3 +54,29 @@ def test_row_sampling_of_two_sizes(torch_cuda):
 
     together(torch, call(230, 151936), [call(230, 300) for _ in range(3)], 2000)
     assert [int(t[-1]) for t in tokens] == want
+
+
+@pytest.mark.parametrize("rots", [(128, 64), (120, 6)])  # whole chunks, two heads a block or one; the general form
+def test_cache_append_of_two_sizes(torch_cuda, rots):
+    torch = torch_cuda
+    pages, page, heads, dim = 80, 64, 8, 128
+    checks = []
+
+    def call(rot, batch, new):
+        rows = batch * new
+        x = torch.randn(rows, 2, heads, dim, device="cuda")
+        off = torch.arange(0, rows + 1, new, dtype=torch.int32, device="cuda")
+        lens = torch.full((batch,), new, dtype=torch.int32, device="cuda")
+        bt = torch.arange(pages, dtype=torch.int32, device="cuda").reshape(batch, -1).contiguous()
+        k, v = (torch.zeros(pages, heads, dim, page, dtype=torch.float16, device="cuda") for _ in range(2))
+        r = fb.Rotary(rot, 1e5)
+        checks.append((v, x, bt, new))
+        at, row = x.data_ptr(), heads * dim
+        return lambda ctx: fb.kv_append(ctx, r, fb.F32, at, 2 * row, at + 4 * row, 2 * row, off.data_ptr(), lens.data_ptr(), 0,
+                                        bt.data_ptr(), k.data_ptr(), v.data_ptr(), batch, rows, new, heads, dim, page,
+                                        bt.shape[1], pages)
+
+    together(torch, call(rots[0], 40, 100), [call(rots[1], 1, 1) for _ in range(3)], 4000)
+    for v, x, bt, new in checks:
+        last = v.view(pages, heads, page, dim)[bt[-1, (new - 1) // page], :, (new - 1) % page]
+        assert torch.equal(last, x[-1, 1].half())
