@@ -188,16 +188,19 @@ struct RowRule {
         return whole ? __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p)) : p;
     }
     // One unit and the whole units of the weight, as a double (exact: at most 2^43 + 1), for a finite maximum and x >=
-    // the lowest logit that weighs at all; below vmin (weights under 2^-59) that is one unit.
+    // the lowest logit that weighs at all.  vmin is the lowest f32 from max - 41 T on (weights of 2^-59): what lies below
+    // it weighs one unit, and the next f32 above it may be the maximum itself.
     __device__ __forceinline__ double units_of(float x, float mx, float vmin, const double *table) const {
         const double w = step((double)fmaxf(x, vmin) - (double)mx, table, 1);
-        return __dsub_rn(__fma_rd(w, SR_UNIT, 4503599627370496.0), 4503599627370495.0);  // + 2^52 - (2^52 - 1)
+        const double u = __dsub_rn(__fma_rd(w, SR_UNIT, 4503599627370496.0), 4503599627370495.0);  // + 2^52 - (2^52 - 1)
+        return x < vmin ? 1.0 : u;
     }
     // The same as an integer that is SR_BIAS too large: what adds up many of them adds integers and takes the surplus
     // off once.  mx is finite here, and x above it counts as it.
     __device__ __forceinline__ u64 biased_units(float x, float mx, float vmin, const double *table) const {
         const double w = step((double)fminf(fmaxf(x, vmin), mx) - (double)mx, table, 1);
-        return (u64)__double_as_longlong(__fma_rd(w, SR_UNIT, 4503599627370496.0));
+        const u64 u = (u64)__double_as_longlong(__fma_rd(w, SR_UNIT, 4503599627370496.0));
+        return x < vmin ? SR_BIAS + 1 : u;
     }
     // f mass, exactly, of an f32 f in 0 .. 1 (M 2^-e, M below 2^24, e from 23 on) and a mass below 2^62: rounded down,
     // rest whether anything was dropped.
@@ -501,8 +504,11 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     }
     // survivors: x >= xmin (only the infinite logits weigh next to an infinite maximum)
     const float xmin = mx == INFINITY ? INFINITY : rule.min_p > 0.0 ? sr_unkey(S.kmin) : -3.4028235e38f;
-    const float vmin = rule.t < 1e30 ? (float)((double)mx - 41.0 * rule.t) : -3.4028235e38f;  // weight 2^-59
-    const float vzero = rule.t < 1e30 ? (float)((double)mx - 745.0 * rule.t) : -3.4028235e38f;  // weighs nothing below
+    // The lowest f32 that weighs 2^-59 at least, and the lowest that weighs anything: e^-745.1332 is 2^-1075, which
+    // binary64 rounds to 0.  (Rounded up: where f32 has no number between max - 41 T and the maximum, the next one below
+    // is too small for vmin and does not stand for it.  From -FLT_MAX on at any T.)
+    const float vmin = fmaxf(__double2float_ru((double)mx - 41.0 * rule.t), -3.4028235e38f);
+    const float vzero = fmaxf(__double2float_ru((double)mx - 745.1332191019412 * rule.t), -3.4028235e38f);
     auto unit_of = [&](float v) -> u64 {
         if (mx == INFINITY) return v == mx ? (u64)SR_UNIT + 1 : 0;
         return v >= vzero ? (u64)rule.units_of(v, mx, vmin, S.table) : 0;  // (not NaN, not -inf)
