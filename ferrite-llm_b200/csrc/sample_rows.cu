@@ -32,7 +32,8 @@
 // then.  A decision that leans on approximate masses is taken with their error
 // on both sides; where that leaves it open, the exact mass of the row is summed.
 // Rows whose cut falls among more than SR_LIST logits that no bin tells apart are
-// bisected by key.
+// bisected by key, as are those whose temperature leaves f32 no approximate mass
+// (above 10^36, or beyond 10^30 and 10^-30 with logits near its size).
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -531,7 +532,9 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     double m1 = 0.0;  // approximate mass of the survivors
     // (a maximum next to the lowest value, which the first pass took NaN and -inf for, or so many times T that f32 has
     // no place behind the point: the first pass's masses say nothing)
-    const bool summed = online && mx > -1e38f && fabsf(__fmul_rn(mx, rule.c)) < SR_REF;
+    // (T beyond what rule.c holds, or next to the logits' own size there: no approximate mass at all, the cut is bisected)
+    const bool coarse = rule.t >= 1e30 ? rule.t >= 1e36 || fabsf(mx) >= 1e20f : rule.t < 1.5e-30 && fabsf(mx) < 1e-18f;
+    const bool summed = online && !coarse && mx > -1e38f && fabsf(__fmul_rn(mx, rule.c)) < SR_REF;
     // a rank's approximate mass, relative to the maximum's weight
     const float lift = summed ? ex2(__fmaf_rn(-mx, rule.c, ref(mx))) : 1.f;
     auto mass_at = [&](int i) {
@@ -767,8 +770,8 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
         for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
         if (lane == 0) lead->seg[rank * SR_WARPS + warp] = m;
     };
-    unsigned c_above = 0, in_range = 0;
-    if (cuts) {
+    unsigned c_above = 0, in_range = cuts && coarse ? SR_LIST + 1 : 0;
+    if (cuts && !coarse) {
         // lowest survivor, and the approximate mass, as far as the first pass has not found them
         if (!summed) {
             double mass = 0.0;

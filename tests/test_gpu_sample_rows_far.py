@@ -1,5 +1,6 @@
-"""Row sampling where neighbouring f32 logits lie hundreds of temperatures apart:
-the weights of exp((x - max) / T) all the same.
+"""Row sampling where neighbouring f32 logits lie hundreds of temperatures apart,
+and at temperatures beyond every difference: the weights of exp((x - max) / T)
+all the same.
 
 A kept weight counts in whole units of 2^-43, rounded up by one at most, so the
 masses of N kept tokens are off by N 2^-43 at most: the token is one whose share
@@ -64,3 +65,30 @@ def test_neighbours_many_temperatures_apart(fbctx, torch_cuda, size, gap):
     for s in SETTINGS:
         for u in (0.0, 0.5, 0.9999):
             check(torch_cuda, fbctx, x, "f32", t, u, **s)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("t", [1e28, 2e30, 3e33, 1e36, 3.4e38])
+def test_temperatures_beyond_the_logits(fbctx, torch_cuda, kind, t):
+    """Logits over the type's whole range (masks of its lowest value among them) and over a little of it."""
+    torch = torch_cuda
+    rng = np.random.default_rng(3)
+    lowest = float(torch.finfo(torch.float32 if kind == "f32" else torch.bfloat16).min)
+    x = rng.uniform(-3.3e38, 3.3e38, (5, 2500))
+    x[1] = 3e36 * rng.normal(0, 1, 2500)
+    x[2, 10:] = lowest
+    x[3] = rng.normal(0, 1, 2500)
+    x[3, ::2] = lowest
+    x[4, ::3] = -np.inf
+    for s in SETTINGS:
+        check(torch, fbctx, x, kind, t, rng.random(5), **s)
+
+
+@pytest.mark.parametrize("t", [1e-38, 1e-33, 1e-25])
+def test_smallest_logits_and_temperatures(fbctx, torch_cuda, t):
+    rng = np.random.default_rng(4)
+    x = 5 * t * rng.normal(0, 1, (3, 2500))
+    x[1, ::2] = -3.0
+    x[2, 1::2] = -np.inf
+    for s in SETTINGS:
+        check(torch_cuda, fbctx, x, "f32", t, rng.random(3), **s)
