@@ -536,8 +536,8 @@ int fb_rotary_create(const fb_rotary_config *cfg, fb_rotary **out) {
         }
         auto r = std::make_unique<fb_rotary>();
         r->cfg = c;
-        r->amplitude = c.amplitude > 0.0 ? c.amplitude
-                       : c.scaling == FB_ROTARY_YARN && c.factor > 1.0 ? 0.1 * log(c.factor) + 1.0 : 1.0;
+        r->amplitude = c.amplitude > 0.0 ? c.amplitude : c.scaling == FB_ROTARY_YARN ? 0.1 * log(c.factor) + 1.0 : 1.0;
+        FB_REQUIRE(r->amplitude > 0.0, "rotary: YaRN's own amplitude is not positive at this factor: give one");
         const double ctx_len = (double)c.orig_ctx;
         double a = 0.0, b = 0.0;
         if (c.scaling == FB_ROTARY_YARN) {

@@ -248,7 +248,8 @@ int fb_attn_decode_noalloc(fb_ctx *ctx, const float *q_dev,
  *                     that make high and low turns over orig_ctx, rot_dim
  *                     ln(orig_ctx / 2 pi turns) / 2 ln(theta), rounded outward
  *                     and clamped to 0..rot_dim - 1; b at least a + 0.001
- * amplitude multiplies cos and sin (0: 1, and for YARN 0.1 ln(factor) + 1).
+ * amplitude multiplies cos and sin (0: 1, and for YARN 0.1 ln(factor) + 1 at
+ * any factor, which must come to more than 0).
  * mode 0 pairs dimensions (2i, 2i + 1), mode 1 (i, i + rot_dim / 2).  A
  * host-side object: no device memory, usable with every context and thread. */
 typedef struct fb_rotary fb_rotary;

@@ -145,3 +145,21 @@ def test_nothing_to_do_needs_no_device():
     fb.kv_append(NoContext, None, **append_args(n_rows=0))
     fb.attn_tree(NoContext, **tree_args(batch=0))
     fb.sample_rows(NoContext, **sample_args(rows=0))
+
+
+@pytest.mark.parametrize("factor", [0.25, 0.5, 0.999, 1.0])
+def test_yarn_amplitude_of_factors_up_to_one(factor):
+    """0.1 ln(factor) + 1 below a factor of one too."""
+    kw = dict(factor=factor, orig_ctx=4096, low=1.0, high=32.0)
+    want, amp = frequencies(64, 1e4, "yarn", **kw)
+    got, gamp = fb.Rotary(64, 1e4, scaling=fb.ROTARY_YARN, **kw).frequencies()
+    np.testing.assert_allclose(got, want, rtol=1e-13)
+    assert abs(gamp - amp) < 1e-14 and (amp < 1.0 or factor == 1.0)
+
+
+def test_yarn_refuses_an_amplitude_of_nothing():
+    """0.1 ln(factor) + 1 reaches 0 at e^-10; an amplitude given replaces it."""
+    kw = dict(scaling=fb.ROTARY_YARN, factor=4e-5, orig_ctx=4096, low=1.0, high=32.0)
+    with pytest.raises(fb.FerriteError, match="amplitude"):
+        fb.Rotary(64, 1e4, **kw)
+    assert fb.Rotary(64, 1e4, amplitude=1.5, **kw).frequencies()[1] == 1.5
