@@ -383,6 +383,8 @@ def kv_append(ctx: Context, rotary: Rotary | None, dtype: int, k_ptr: int, k_tok
               page_size: int, max_pages: int, num_pages: int):
     """The new rows of a ragged batch into the cache pages (k rotated at
     positions_ptr, 0: at the cache position; rotary None: not rotated)."""
+    if rotary is not None and not rotary.h:  # (no handle would mean no rotation)
+        raise FerriteError(-1, "kv_append: the rotary handle is closed")
     _check(lib().fb_kv_append(ctx.h, rotary.h if rotary is not None else None, dtype, k_ptr, k_token_stride, v_ptr,
                               v_token_stride, row_offsets_ptr, seq_lens_ptr, positions_ptr or None, bt_ptr,
                               k_pages_ptr, v_pages_ptr, batch, n_rows, max_new, n_kv, head_dim, page_size, max_pages,

@@ -163,3 +163,12 @@ def test_yarn_refuses_an_amplitude_of_nothing():
     with pytest.raises(fb.FerriteError, match="amplitude"):
         fb.Rotary(64, 1e4, **kw)
     assert fb.Rotary(64, 1e4, amplitude=1.5, **kw).frequencies()[1] == 1.5
+
+
+def test_a_closed_rotary_handle_is_refused():
+    r = fb.Rotary(64, 1e4)
+    r.close()
+    with pytest.raises(fb.FerriteError, match="closed"):
+        fb.kv_append(NoContext, r, **append_args(n_rows=0))
+    with pytest.raises(fb.FerriteError, match="rotary"):
+        fb.rotary_apply(NoContext, r, **rotary_args())
