@@ -1324,8 +1324,10 @@ int fb_attn_tree(fb_ctx *ctx, int dtype, const void *q_dev, int64_t q_token_stri
         FB_REQUIRE(ctx && q_dev && k_pages_dev && v_pages_dev && block_table_dev && row_offsets_dev && seq_lens_dev &&
                        out_dev,
                    "null argument");
-        FB_REQUIRE(q_dev != out_dev, "attn_tree: q and out must not overlap");
         const size_t esz = dtype == FB_F32 ? 4 : 2;
+        FB_REQUIRE(!rows_overlap(q_dev, q_token_stride, 0, out_dev, out_token_stride, 0, n_rows, 1,
+                                 (int64_t)n_heads * head_dim, esz),
+                   "attn_tree: q and out must not overlap");
         FB_REQUIRE((((uintptr_t)q_dev | (uintptr_t)out_dev) & (esz - 1)) == 0 &&
                        (((uintptr_t)row_offsets_dev | (uintptr_t)seq_lens_dev | (uintptr_t)block_table_dev |
                          (uintptr_t)mask_dev) & 3) == 0,

@@ -8,6 +8,7 @@
 
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/ferrite_b200.h"
@@ -68,6 +69,35 @@ struct DeviceGuard {
     DeviceGuard(const DeviceGuard &) = delete;
     DeviceGuard &operator=(const DeviceGuard &) = delete;
 };
+
+// Whether rows of x and y share memory: rows of `width` elements at x + i xa + j xb and at y + i ya + j yb (strides
+// of elements, i < na, j < nb), in y one stride steps over all that the other spans.  With equal strides exactly so
+// (two column ranges of one buffer's rows do not overlap); with unequal ones wherever the spans of x and y meet.
+inline bool rows_overlap(const void *x, int64_t xa, int64_t xb, const void *y, int64_t ya, int64_t yb, int64_t na,
+                         int64_t nb, int64_t width, size_t esz) {
+    using wide = __int128;
+    if (na <= 1) xa = ya = 0;  // (a stride that is not taken)
+    if (nb <= 1) xb = yb = 0;
+    const wide d = ((wide)(uintptr_t)y - (wide)(uintptr_t)x) / (wide)esz;
+    auto span = [&](int64_t a, int64_t b) { return (wide)(na - 1) * a + (wide)(nb - 1) * b + width; };
+    if (na < 1 || nb < 1 || d >= span(xa, xb) || -d >= span(ya, yb)) return false;
+    if (xa != ya || xb != yb) return true;
+    if (ya < yb) {
+        std::swap(ya, yb);
+        std::swap(na, nb);
+    }
+    // steps of the outer stride, then of the inner one, that bring the distance below what is inside
+    auto near = [](wide at, int64_t stride, int64_t n, auto &&found) {
+        if (stride == 0 || n <= 1) return found(at);
+        const wide k = -at / stride;
+        for (wide i = k - 1; i <= k + 1; i++)
+            if (i > -n && i < n && found(at + i * stride)) return true;
+        return false;
+    };
+    return near(d, ya, na, [&](wide r) {
+        return near(r, yb, nb, [&](wide e) { return e > -(wide)width && e < (wide)width; });
+    });
+}
 
 // Launches a kernel with its attributes.  pdl: it writes nothing before its
 // pdl_wait() and reads only what was complete before its predecessor on the stream

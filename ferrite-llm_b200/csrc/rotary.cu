@@ -598,6 +598,9 @@ int fb_rotary_apply(fb_ctx *ctx, const fb_rotary *r, int dtype, const void *x_de
         const size_t esz = dtype == FB_F32 ? 4 : 2;
         FB_REQUIRE((((uintptr_t)x_dev | (uintptr_t)y_dev) & (esz - 1)) == 0 && ((uintptr_t)positions_dev & 3) == 0,
                    "rotary_apply: misaligned pointer");
+        FB_REQUIRE(x_dev == y_dev || !rows_overlap(x_dev, x_token_stride, x_head_stride, y_dev, y_token_stride,
+                                                   y_head_stride, n_tok, n_heads, head_dim, esz),
+                   "rotary_apply: x and y overlap");
         DeviceGuard guard(ctx->device);
         const RotaryParams P = rotary_params(r);
         switch (dtype) {

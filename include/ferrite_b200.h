@@ -271,7 +271,8 @@ int fb_rotary_frequencies(const fb_rotary *r, double *freq_host, int capacity, d
  * back), for x [n_tok][n_heads][head_dim] with the given token and head
  * strides; dimensions from rot_dim on are copied.  Angles are reduced in
  * binary64, so far positions keep full precision.  y_dev == x_dev with equal
- * strides rotates in place; otherwise x and y must not overlap.  In y one of
+ * strides rotates in place; otherwise x and y must not overlap (refused; with
+ * unequal strides the memory that either spans must not meet).  In y one of
  * the strides steps over all rows that the other spans.  head_dim up to 1024. */
 int fb_rotary_apply(fb_ctx *ctx, const fb_rotary *r, int dtype, const void *x_dev, int64_t x_token_stride,
                     int64_t x_head_stride, void *y_dev, int64_t y_token_stride, int64_t y_head_stride,
@@ -293,7 +294,8 @@ int fb_kv_append(fb_ctx *ctx, const fb_rotary *r, int dtype, const void *k_dev, 
  * ancestors and itself.  mask_dev NULL: rows 0..i (a chain).  A row that sees
  * nothing gets zeros; what a row does not see never reaches it, NaN and
  * infinities included.  q [n_rows][n_heads][head_dim] and out of the same
- * shape and dtype have token strides, heads contiguous; they must not overlap.  Scores and sums
+ * shape and dtype have token strides, heads contiguous; they must not overlap
+ * (refused, as in fb_rotary_apply).  Scores and sums
  * in f32; with dtype FB_F32 q and the probabilities enter the tensor cores as
  * fp16 high and low parts, otherwise as one fp16 value each (bf16 q scaled
  * into its range).  mask_words >= ceil(max_new / 32).  The workspace is the

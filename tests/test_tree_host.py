@@ -172,3 +172,31 @@ def test_a_closed_rotary_handle_is_refused():
         fb.kv_append(NoContext, r, **append_args(n_rows=0))
     with pytest.raises(fb.FerriteError, match="rotary"):
         fb.rotary_apply(NoContext, r, **rotary_args())
+
+
+class AnyContext:
+    h = A  # never read by a refused call
+
+
+@pytest.mark.parametrize("over", [
+    dict(y_ptr=A + 4), dict(y_ptr=A - 4 * 127), dict(y_ptr=A + 4 * 512),  # shifted by a value, almost a head, a token
+    dict(y_ptr=A + 4 * 128 * 3, n_tok=1),
+    dict(y_ptr=A + 4 * 1000, x_token_stride=1024, y_token_stride=1024),  # 24 values into the next token
+    dict(y_ptr=A + 4 * 100, x_token_stride=256, x_head_stride=1024, y_token_stride=256, y_head_stride=1024),
+    dict(y_ptr=A + 4 * 512, x_token_stride=1024, y_token_stride=512),    # unequal strides over the same memory
+    dict(dtype=fb.F16, y_ptr=A + 2 * 127, n_tok=1, n_heads=1),
+])
+def test_rotary_apply_refuses_overlap(over):
+    with pytest.raises(fb.FerriteError, match="x and y overlap"):
+        fb.rotary_apply(AnyContext, fb.Rotary(64, 1e4), **rotary_args(**over))
+
+
+@pytest.mark.parametrize("over", [
+    dict(out_ptr=A), dict(out_ptr=A + 4 * 4095), dict(out_ptr=A - 4 * 4095), dict(out_ptr=A + 4 * 4096 * 59),
+    dict(q_token_stride=8192, out_token_stride=8192, out_ptr=A + 4 * 8192 * 30 + 4 * 4095),
+    dict(q_token_stride=8192, out_token_stride=4096, out_ptr=A + 4 * 4096),
+    dict(q_token_stride=0, out_ptr=A + 16), dict(n_rows=1, q_token_stride=1, out_token_stride=0, out_ptr=A + 4 * 100),
+])
+def test_attn_tree_refuses_overlap(over):
+    with pytest.raises(fb.FerriteError, match="q and out must not overlap"):
+        fb.attn_tree(AnyContext, **tree_args(**{"q_ptr": A, **over}))
