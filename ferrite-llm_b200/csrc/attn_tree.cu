@@ -37,16 +37,15 @@
 // Precision: q is scaled by a power of two a row (to 2^13..2^14 at most) and
 // enters as fp16 high + low parts where it is f32 (f16 and bf16 queries fit the
 // high part); the probabilities are kept 2^7 above the running maximum's unit (at
-// most 2^15).  For f32 results they are fp16 high + low parts too, 22 bits down
-// to 2^-21 of the largest; for f16 and bf16 results the high part alone, off by
-// 2^-11 of it at most: below half a step of a bf16 result, and for f16 results,
-// whose own rounding is as large, the sum is that of the rounded probabilities,
-// so that a row that one key dominates is not off by that key's (1.4 times the
-// output rounding's error in the 2-norm; both parts would take twice the products).
+// most 2^15) and are fp16 high + low parts at every type, 22 bits down to 2^-21 of
+// the largest.  (The high part alone would be off by 2^-11 of a probability: f16
+// results were 1.37 times as far from binary64 as their own rounding, bf16 ones
+// 1.008 times; with both parts 1.000.  The second product costs 2.5 us of 44 and
+// 33 of 196 below.)
 // Products and sums are f32.  The tensor core truncates its sums, by 2^-25 of
 // them on average at each instruction, always towards zero: over 100 blocks that
-// is 10^-5 (7.4e-6 measured in the 2-norm at 30000 keys), nothing beside a 16-bit
-// result's rounding, but not f32's.  So f32 results have each block's product
+// is 10^-5 (7.4e-6 measured in the 2-norm at 30000 keys), little beside a 16-bit
+// result's rounding, but not beside f32's.  So f32 results have each block's product
 // start from zero and the second group adds it to its registers, a rounded FMA an
 // element (6.6e-7 there).  Where the tensor core does accumulate, the sums are
 // rescaled only when a row's maximum grows by more than 8 (log 2 units).
@@ -325,7 +324,7 @@ __device__ __forceinline__ uint32_t tree_visible(const TreeArgs &A, const TreeSe
 }
 
 template <typename T, int HD> struct TreeCfg {
-    static constexpr bool LO = sizeof(T) == 4;          // f32: q and the probabilities have low parts
+    static constexpr bool LO = sizeof(T) == 4;          // f32: q has low parts, the blocks are summed in registers
     static constexpr int ST = HD == 128 && LO ? 4 : 5;  // K and V stages
     static constexpr uint32_t Q_BYTES = TR_ROWS * HD * 2;
     static constexpr uint32_t TILE_BYTES = (LO ? 2 : 1) * Q_BYTES;  // a tile's queries
@@ -626,8 +625,11 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     if (!tr_wait(&p_full[g][j & 1], (uint32_t)(j >> 1) & 1u)) return false;
                     tc_fence_after();
 #pragma unroll
-                    for (int ks = 0; ks < TR_KB / 16; ks++)  // 16 keys: 8 columns of fp16 pairs
-                        umma_f16_tmem(t_o, p + 8 * ks, vd + ks * (2048 >> 4), IDESC_O, (k > 0 || ks > 0) ? 1u : 0u);
+                    for (int i = 0; i < 2 * (TR_KB / 16); i++) {  // 16 keys: 8 columns of fp16 pairs; low parts first
+                        const int ks = i % (TR_KB / 16);
+                        umma_f16_tmem(t_o, p + (i < TR_KB / 16 ? 32 : 0) + 8 * ks, vd + ks * (2048 >> 4), IDESC_O,
+                                      (k > 0 || i > 0) ? 1u : 0u);
+                    }
                     umma_commit(&o_done[g][j & 1]);
                     release(&v_empty[st]);
                     forward(vf, vph);
@@ -832,20 +834,13 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 const float pb = exp2_approx(__fmaf_rn(__uint_as_float(sv[2 * t + 1]), u, ref));
                 const __half2 h2 = __floats2half2_rn(pa, pb);
                 hi[t] = *reinterpret_cast<const uint32_t *>(&h2);
-                if (std::is_same<T, __half>::value) {  // (the sum of what the products see)
-                    const float2 hf = __half22float2(h2);
-                    l4[t & 3] = __fadd_rn(l4[t & 3], __fadd_rn(hf.x, hf.y));
-                } else {
-                    l4[t & 3] = __fadd_rn(l4[t & 3], __fadd_rn(pa, pb));
-                }
-                if (C::LO) {
-                    const float2 hf = __half22float2(h2);
-                    const __half2 q2 = __floats2half2_rn(__fsub_rn(pa, hf.x), __fsub_rn(pb, hf.y));
-                    lo[t] = *reinterpret_cast<const uint32_t *>(&q2);
-                }
+                l4[t & 3] = __fadd_rn(l4[t & 3], __fadd_rn(pa, pb));
+                const float2 hf = __half22float2(h2);
+                const __half2 q2 = __floats2half2_rn(__fsub_rn(pa, hf.x), __fsub_rn(pb, hf.y));
+                lo[t] = *reinterpret_cast<const uint32_t *>(&q2);
             }
             tmem_st32(t_b, hi);
-            if (C::LO) tmem_st32(t_b + 32, lo);
+            tmem_st32(t_b + 32, lo);
             return __fadd_rn(__fadd_rn(l4[0], l4[1]), __fadd_rn(l4[2], l4[3]));
         };
         if constexpr (C::LO) {
