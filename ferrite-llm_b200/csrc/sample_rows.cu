@@ -1,6 +1,7 @@
 // One token per logits row from given random numbers (fb_sample_rows): the
 // rules of the reference sampler (crates/ferrite-core/src/sampling.rs:61-239)
-// for many rows with settings of their own, without its host round trip.
+// for many rows with settings of their own, without its host round trip and its
+// repetition penalty.
 //
 // Mathematics: w_i = exp((x_i - max) / T).  In the row sorted by descending
 // logit (equal logits in index order) min-p, top-p and top-k each keep a

@@ -310,9 +310,10 @@ int fb_attn_tree(fb_ctx *ctx, int dtype, const void *q_dev, int64_t q_token_stri
                  int64_t out_token_stride, int batch, int n_rows, int max_new, int n_heads, int n_kv_heads,
                  int head_dim, int page_size, int max_pages, int num_pages, int max_seq_len, float scale,
                  void *workspace_dev, int64_t workspace_bytes);
-/* One token per logits row from given random numbers (fb_sample's rules for
- * many rows with settings of their own, on the device): weights w = exp((x -
- * max x) / T); of the row sorted by descending logit (equal logits in index
+/* One token per logits row from given random numbers (fb_sample's filters and
+ * draw for many rows with settings of their own, on the device; its repetition
+ * penalty is not applied: the logits are taken as they are): weights w =
+ * exp((x - max x) / T); of the row sorted by descending logit (equal logits in index
  * order) min-p keeps w >= min_p, top-p of those the fewest first ones that
  * hold top_p of their mass, top-k the first top_k; the token is the first in
  * index order whose kept mass, its own included, exceeds u times the whole
