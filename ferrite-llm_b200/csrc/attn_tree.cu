@@ -94,8 +94,9 @@ constexpr int TR_KB = 64;         // keys a block
 constexpr int TR_WHOLE = 4;
 constexpr int TR_SWITCH = 8;
 constexpr int TR_THREADS = 384;
-constexpr float TR_NONE = -1e30f;  // running maximum of a row that has seen nothing
+constexpr float TR_NONE = -3e38f;  // running maximum of a row that has seen nothing
 constexpr float TR_LIFT = 7.f;     // probabilities are kept 2^7 above the reference maximum
+constexpr float TR_FAR = 1048576.f;  // 2^20: maxima beyond it are taken off the scores before the lift is added
 
 __device__ __forceinline__ float tr_f32(float v) { return v; }
 __device__ __forceinline__ float tr_f32(__half v) { return __half2float(v); }
@@ -843,6 +844,17 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             tmem_st32(t_b + 32, lo);
             return __fadd_rn(__fadd_rn(l4[0], l4[1]), __fadd_rn(l4[2], l4[3]));
         };
+        // The maximum m is rounded down, and what a score exceeds it by is computed exactly; where f32 has no fractions
+        // left at m's size that excess could reach 2^9 and more.  So far maxima are taken off first (s u - m, at most 8:
+        // 2^15), and the exponentials see scores next to 0.
+        auto far = [&](float m) { return __any_sync(FULL, fabsf(m) > TR_FAR && m != TR_NONE); };
+        auto bring_near = [&](uint32_t (&sv)[64], float u, float m) {
+#pragma unroll
+            for (int t = 0; t < 64; t++) {
+                const float x = __fmaf_rn(__uint_as_float(sv[t]), u, -m);
+                sv[t] = __float_as_uint(x > 8.f ? 8.f : x);  // (NaN stays)
+            }
+        };
         if constexpr (C::LO) {
             // ---- f32: group 0 turns scores into probabilities, group 1 sums the blocks' products in registers
             load_q(w, 0, 8);
@@ -867,12 +879,19 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                             uint32_t sv[64];
                             tmem_ld64(t_b, sv);
                             if (odd) hide(w, tok, p0, skip, sv);
-                            const float mn = fmaxf(m, __fmul_rn(largest(sv), u));
+                            const float mn = fmaxf(m, __fmul_rd(largest(sv), u));
                             const float al = exp2f(__fsub_rn(m, mn));
                             m = mn;
                             // (four blocks in flight at most: the product of block j - 2 waits for the reader of j - 4)
                             s_al[j & 3][r] = al;
-                            l = __fmaf_rn(l, al, exponentials(sv, u, m, t_b));
+                            float sum;
+                            if (__builtin_expect(far(m), 0)) {
+                                bring_near(sv, u, m);
+                                sum = exponentials(sv, 1.f, 0.f, t_b);
+                            } else {
+                                sum = exponentials(sv, u, m, t_b);
+                            }
+                            l = __fmaf_rn(l, al, sum);
                         }
                         if (odd && !(ok = mend_values(w, j, p0, skip, seg))) break;
                         tc_fence_before();
@@ -1070,7 +1089,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     tmem_ld64(t_b, sv);
                     if (p0 + TR_KB > pre || skip) hide(w, tok, p0, skip, sv);
                     const float bm = largest(sv);
-                    const float mn = fmaxf(m, __fmul_rn(bm, sl2));
+                    const float mn = fmaxf(m, __fmul_rd(bm, sl2));
                     const bool need = k > 0 && mn > m + 8.f;
                     if (__any_sync(FULL, need)) {
                         // rescale the accumulator rows once the product of this group's last block has landed
@@ -1091,7 +1110,12 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                         }
                     }
                     if (k == 0) m = mn;
-                    l = __fadd_rn(l, exponentials(sv, sl2, m, t_b));
+                    if (__builtin_expect(far(m), 0)) {
+                        bring_near(sv, sl2, m);
+                        l = __fadd_rn(l, exponentials(sv, 1.f, 0.f, t_b));
+                    } else {
+                        l = __fadd_rn(l, exponentials(sv, sl2, m, t_b));
+                    }
                 }
                 if ((p0 + TR_KB > pre || skip) && !(ok = mend_values(w, c, p0, skip, seg))) break;
                 tc_fence_before();
