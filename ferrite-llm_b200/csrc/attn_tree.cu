@@ -37,11 +37,12 @@
 // Precision: q is scaled by a power of two a row (to 2^13..2^14 at most) and
 // enters as fp16 high + low parts where it is f32 (f16 and bf16 queries fit the
 // high part); the probabilities are kept 2^7 above the running maximum's unit (at
-// most 2^15) and are fp16 high + low parts at every type, 22 bits down to 2^-21 of
-// the largest.  (The high part alone would be off by 2^-11 of a probability: f16
-// results were 1.37 times as far from binary64 as their own rounding, bf16 ones
-// 1.008 times; with both parts 1.000.  The second product costs 2.5 us of 44 and
-// 33 of 196 below.)
+// most 2^15).  For f32 and f16 results they are fp16 high + low parts, 22 bits down
+// to 2^-21 of the largest: f16 results are off by their own rounding alone (1.37
+// times that with the high part alone; the second product costs 2.5 us of 44 below).
+// For bf16 results the high part is enough: it is off by 2^-11 of a probability
+// where a result's own rounding is 2^-8 of it (together 1.008 times that rounding
+// in the 2-norm; the low part would cost a fifth of the long contexts' time below).
 // Products and sums are f32.  The tensor core truncates its sums, by 2^-25 of
 // them on average at each instruction, always towards zero: over 100 blocks that
 // is 10^-5 (7.4e-6 measured in the 2-norm at 30000 keys), little beside a 16-bit
@@ -326,6 +327,7 @@ __device__ __forceinline__ uint32_t tree_visible(const TreeArgs &A, const TreeSe
 
 template <typename T, int HD> struct TreeCfg {
     static constexpr bool LO = sizeof(T) == 4;          // f32: q has low parts, the blocks are summed in registers
+    static constexpr bool PLO = !std::is_same<T, __nv_bfloat16>::value;  // the probabilities have low parts
     static constexpr int ST = HD == 128 && LO ? 4 : 5;  // K and V stages
     static constexpr uint32_t Q_BYTES = TR_ROWS * HD * 2;
     static constexpr uint32_t TILE_BYTES = (LO ? 2 : 1) * Q_BYTES;  // a tile's queries
@@ -626,10 +628,10 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                     if (!tr_wait(&p_full[g][j & 1], (uint32_t)(j >> 1) & 1u)) return false;
                     tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < 2 * (TR_KB / 16); i++) {  // 16 keys: 8 columns of fp16 pairs; low parts first
+                    for (int i = 0; i < (C::PLO ? 2 : 1) * (TR_KB / 16); i++) {  // 16 keys: 8 columns of fp16 pairs
                         const int ks = i % (TR_KB / 16);
-                        umma_f16_tmem(t_o, p + (i < TR_KB / 16 ? 32 : 0) + 8 * ks, vd + ks * (2048 >> 4), IDESC_O,
-                                      (k > 0 || i > 0) ? 1u : 0u);
+                        const uint32_t part = C::PLO && i < TR_KB / 16 ? 32 : 0;  // the low parts first
+                        umma_f16_tmem(t_o, p + part + 8 * ks, vd + ks * (2048 >> 4), IDESC_O, (k > 0 || i > 0) ? 1u : 0u);
                     }
                     umma_commit(&o_done[g][j & 1]);
                     release(&v_empty[st]);
@@ -824,7 +826,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
             for (int t = 0; t < 64; t++) b4[t & 3] = fmaxf(b4[t & 3], __uint_as_float(sv[t]));
             return fmaxf(fmaxf(b4[0], b4[1]), fmaxf(b4[2], b4[3]));
         };
-        // p = 2^(s u - m + 7) as fp16 pairs over the scores, low parts behind the high ones; their sum
+        // p = 2^(s u - m + 7) as fp16 pairs over the scores, low parts (not bf16) behind the high ones; their sum
         auto exponentials = [&](const uint32_t (&sv)[64], float u, float m, uint32_t t_b) {
             const float ref = __fsub_rn(TR_LIFT, m);
             float l4[4] = {0.f, 0.f, 0.f, 0.f};
@@ -836,12 +838,14 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
                 const __half2 h2 = __floats2half2_rn(pa, pb);
                 hi[t] = *reinterpret_cast<const uint32_t *>(&h2);
                 l4[t & 3] = __fadd_rn(l4[t & 3], __fadd_rn(pa, pb));
-                const float2 hf = __half22float2(h2);
-                const __half2 q2 = __floats2half2_rn(__fsub_rn(pa, hf.x), __fsub_rn(pb, hf.y));
-                lo[t] = *reinterpret_cast<const uint32_t *>(&q2);
+                if (C::PLO) {
+                    const float2 hf = __half22float2(h2);
+                    const __half2 q2 = __floats2half2_rn(__fsub_rn(pa, hf.x), __fsub_rn(pb, hf.y));
+                    lo[t] = *reinterpret_cast<const uint32_t *>(&q2);
+                }
             }
             tmem_st32(t_b, hi);
-            tmem_st32(t_b + 32, lo);
+            if (C::PLO) tmem_st32(t_b + 32, lo);
             return __fadd_rn(__fadd_rn(l4[0], l4[1]), __fadd_rn(l4[2], l4[3]));
         };
         // The maximum m is rounded down, and what a score exceeds it by is computed exactly; where f32 has no fractions

@@ -296,8 +296,10 @@ int fb_kv_append(fb_ctx *ctx, const fb_rotary *r, int dtype, const void *k_dev, 
  * infinities included.  q [n_rows][n_heads][head_dim] and out of the same
  * shape and dtype have token strides, heads contiguous; they must not overlap
  * (refused, as in fb_rotary_apply).  Scores and sums in f32; the probabilities
- * enter the tensor cores as fp16 high and low parts (22 bits), and so does q
- * with dtype FB_F32; f16 q as it is, bf16 q scaled into fp16's range.
+ * enter the tensor cores as fp16 high and low parts (22 bits; with FB_BF16 one
+ * fp16 value, 11 bits), and so does q with FB_F32; f16 q as it is, bf16 q scaled
+ * into fp16's range.  Results are off by their own rounding alone (1e-6 in the
+ * 2-norm with FB_F32, 1.01 times the rounding with FB_BF16).
  * mask_words >= ceil(max_new / 32).  The workspace is the
  * caller's (fb_attn_tree_workspace bytes for the same sizes, any dtype,
  * 16-byte aligned, contents ignored and clobbered): calls that may overlap
