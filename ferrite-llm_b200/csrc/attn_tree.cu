@@ -39,7 +39,7 @@
 // high part); the probabilities are kept 2^7 above the running maximum's unit (at
 // most 2^15).  For f32 and f16 results they are fp16 high + low parts, 22 bits down
 // to 2^-21 of the largest: f16 results are off by their own rounding alone (1.37
-// times that with the high part alone; the second product costs 2.5 us of 44 below).
+// times that with the high part alone; the second product costs 2.5 us of 45 below).
 // For bf16 results the high part is enough: it is off by 2^-11 of a probability
 // where a result's own rounding is 2^-8 of it (together 1.008 times that rounding
 // in the 2-norm; the low part would cost a fifth of the long contexts' time below).
@@ -53,11 +53,11 @@
 //
 // Measured (back to back in a graph, the join included; 6559 GB/s the copy rate,
 // 1627 TFLOP/s the library's bf16 rate): 16 sequences of 25 new rows over up to
-// 4096 keys, 32 heads on 8, f16: 40.2 us, 4.5 TB/s of keys and values; 4 of 40
-// over 32000, 64 heads, bf16: 152 us, 646 TFLOP/s, where the exponentials and the
+// 4096 keys, 32 heads on 8, f16: 45.2 us, 4.0 TB/s of keys and values; 4 of 40
+// over 32000, 64 heads, bf16: 154 us, 640 TFLOP/s, where the exponentials and the
 // 64-key products (N = 64 runs at two thirds of N = 128's rate) take turns; 60 rows
-// over 4096, f32: 26.6 us, half of it the queries' way in and the join; 7 over 190:
-// 12.5 us, three blocks and the same ends.
+// over 4096, f32: 27.4 us, half of it the queries' way in and the join; 7 over 190:
+// 12.4 us, three blocks and the same ends.
 #include <math.h>
 
 #include <type_traits>
@@ -176,8 +176,8 @@ struct TreeTotal {
     }
     // Units that a row group has in front of its blocks: what it costs a CTA to begin another one (its queries wait for
     // the last scores, its rows are written out), so that the shares with a border inside hold fewer blocks.  Where no
-    // CTA has more than a unit there is no border.  (60 new rows of 32 heads at 4096 keys, f32: 26.6 us; 29.1 with 3,
-    // 32.7 with none; 16 sequences of 25 rows, f16: 43.2, 44.4, 47.3.)
+    // CTA has more than a unit there is no border.  (When it was chosen: 60 new rows of 32 heads at 4096 keys, f32: 26.6
+    // us; 29.1 with 3, 32.7 with none; 16 sequences of 25 rows, f16: 43.2, 44.4, 47.3.)
     __device__ __forceinline__ int lead(const TreeArgs &A) const { return A.split && units > A.ctas ? TR_SWITCH : 0; }
     // A CTA's share; the join kernel derives the same one.  With split and blocks of two units at least two, so that
     // none lies inside such a block.
@@ -1149,7 +1149,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1)
 // writes alone took 10 us of 16 sequences of 25 tokens, 32 heads); the loads of
 // eight (part, column) pairs are in flight together.  Finding a group's parts costs
 // a block more than reading them, so where there are blocks enough a lane takes
-// four columns: 40.2 us for those sequences instead of 43.4.
+// four columns, which saves 3 us of those sequences' call (8.5 us cold, 12.5 before).
 template <typename T, int HD, int COLS>
 __global__ void __launch_bounds__(128) k_attn_tree_join(const __grid_constant__ TreeArgs A) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

@@ -10,12 +10,16 @@
 // whole turns drop out exactly, and the remaining eighth of a turn at most is
 // what sincospif sees, so a far position costs no precision.
 //
-// Bound: HBM (every value is read and written once); one token's call is
-// bound by the launch and two dependent loads.  Measured (back to back in a
-// graph, 6559 GB/s the copy rate): 2048 tokens x 32 heads of 128, f16, 33.6 MB
-// in 8.2 us, 4.1 TB/s; 777 x 64 heads with half a head turned, bf16, 25.5 MB in
-// 7.7 us; one token 2.2 us.  The append: three prompts of up to 2731
-// bf16 rows of 8 heads, 56 MB in 14.3 us, 3.9 TB/s; 400 drafted rows in 6.4 us.
+// Bound: every value is read and written once, but memory is not what these
+// kernels wait for (13 to 18 % of DRAM's rate from cold caches, 50 to 62 % of the
+// issue slots).  A block of the rotation begins with binary64 angles and a barrier,
+// and 2048 tokens are 1.7 waves of blocks; one token's call is a launch and two
+// dependent loads; the append's transposing tiles are steps one after another.
+// Measured (back to back in a graph, inputs warm in L2; in brackets from cold
+// caches; 6559 GB/s the copy rate): 2048 tokens x 32 heads of 128, f16, 33.6 MB:
+// 8.3 us (12.3); 777 x 64 heads with half a head turned, bf16, 25.5 MB: 8.0 us
+// (12.4); one token 2.2 us (5.5).  The append: three prompts of up to 2731 bf16 rows
+// of 8 heads, 56 MB: 14.5 us (18.7); 400 drafted rows 6.5 us (10.5).
 #include <math.h>
 
 #include <memory>

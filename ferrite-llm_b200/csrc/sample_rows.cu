@@ -8,18 +8,20 @@
 // prefix, so the kept set is the shortest of the three and ends at one (logit,
 // index) pair, the cut.  Masses are 64-bit integers in units of 2^-43 (vocab <=
 // 2^19 keeps them below 2^62), summed in any order with one result; a weight
-// counts for its whole units and one more (none below e^-745), so no kept token
+// counts for its whole units and one more (none where exp is 0), so no kept token
 // is unreachable.
 //
-// Bound: HBM for many rows (a row streams through registers once; what comes
-// later reads a few of its vectors, or passes that find it in L2); a few rows
-// are bound by the steps of the cluster that shares a row.  The first pass keeps
+// Bound: many rows by the first pass, which streams a row through registers once
+// (an exponential a logit where top-p asks: 53 % of the issue slots and 38 % of the
+// special-function unit at 31 % of DRAM's rate; what comes later reads a few of a
+// row's vectors, or passes that find it in L2); a few rows by the steps of the
+// cluster that shares a row.  The first pass keeps
 // the maximum of every group of 16-byte vectors in shared memory.  Measured
 // (back to back in a graph): 400 rows of 151936 bf16 logits, top-k 50 and top-p,
-// in 44 us (53 us from HBM, 2.3 TB/s: a row is one CTA and three of them share
-// an SM, whose exponentials take half of the first pass); 65 rows of 128256 f32
-// logits, top-p alone, in 73 us, a third each for counting into bins and for the
-// exact masses; one row of 151936 in 8.7 us.  No sort of the row:
+// in 45 us (48 us from cold caches, 2.5 TB/s: a row is one CTA and three of them
+// share an SM); 65 rows of 128256 f32 logits, top-p alone, in 74 us, some 16 us each
+// for counting into bins and for the exact masses; one row of 151936 in 8.6 us.  No
+// sort of the row:
 //  * min-p: the threshold logit is found exactly (the f32 whose binary64 weight
 //    is the first to reach min_p); the survivors are the candidates;
 //  * top_k <= SR_TOPK: at least top_k of the groups' maxima lie above the
