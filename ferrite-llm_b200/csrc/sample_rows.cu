@@ -34,10 +34,12 @@
 // bitonic sort), adds up their exact weights and draws; the cluster's other CTAs are gone by
 // then.  A decision that leans on approximate masses is taken with their error
 // on both sides; where that leaves it open, the exact mass of the row is summed.
-// A cut by top-k alone that lies beyond the bins is narrowed by key, 9 bits a pass.
-// Rows whose cut falls among more than SR_LIST logits that no bin tells apart are
-// bisected by (key, index), as are those whose temperature leaves f32 no approximate mass
-// (above 10^36, or beyond 10^30 and 10^-30 with logits near its size).
+// Where no bins come down to SR_LIST logits (top-k alone far below the maximum in
+// temperatures, top-p so near 1 that the masses' error spans more, many equal
+// logits, temperatures that leave f32 no approximate mass: above 10^36, or beyond
+// 10^30 and 10^-30 with logits near its size) bins of (key, index) pairs with exact
+// masses close in on the cut, 9 bits a pass.  (65 rows of 151936: top-k 1000 at T
+// 0.1 120 us, top-p 0.999 at T 0.7 184 us.)
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -58,7 +60,7 @@ constexpr int SR_RANKED = 256;  // up to here every candidate is compared with a
 constexpr int SR_TOPK = 256;    // top_k up to here goes by the groups' maxima
 constexpr int SR_BINS = 512;
 constexpr int SR_CLUSTER = 16;
-constexpr int SR_ROUNDS = 4;    // narrowings by distance
+constexpr int SR_ROUNDS = 3;    // narrowings by distance (two are enough unless the masses' error spans more than the list)
 constexpr int SR_GROUPS = 48;   // groups a thread, at most
 constexpr int SR_AHEAD = 4;     // vectors a thread has in flight
 constexpr int SR_FLAGGED = 1024;
@@ -536,7 +538,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     double m1 = 0.0;  // approximate mass of the survivors
     // (a maximum next to the lowest value, which the first pass took NaN and -inf for, or so many times T that f32 has
     // no place behind the point: the first pass's masses say nothing)
-    // (T beyond what rule.c holds, or next to the logits' own size there: no approximate mass at all, the cut is bisected)
+    // (T beyond what rule.c holds, or next to the logits' own size there: no approximate mass at all)
     const bool coarse =
         has_p && (rule.t >= 1e30 ? rule.t >= 1e36 || fabsf(mx) >= 1e20f : rule.t < 1.5e-30 && fabsf(mx) < 1e-18f);
     const bool summed = online && !coarse && mx > -1e38f && fabsf(__fmul_rn(mx, rule.c)) < SR_REF;
@@ -814,9 +816,8 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             hi = fminf(hi, __fdiv_rn(fmaxf(__log2f(left), 0.f) + 0.5f, rule.c));
         }
         float m_above = 0.f;
-        int rounds = 0;
-        while (rounds < SR_ROUNDS) {
-            const int buf = rounds++ & 1;
+        for (int round = 0; round < SR_ROUNDS; round++) {
+            const int buf = round & 1;
             const float width = hi - lo;
             const float inv = width > 0.f && width < INFINITY ? __fdiv_rn(1.f, width) : 0.f;
             const float from = __fsub_rn(mx, lo);
@@ -940,59 +941,126 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
             to_top = to_top && ka > sr_key(mx);
             if (!to_top) xa = sr_unkey(ka);
             xb = sr_unkey(kb);
-            if (in_range <= SR_LIST || (!has_p && lb >= SR_BINS - 1)) break;
+            // (the last bin reaches down to the lowest value of the type, a mask perhaps, and 512 distances tell nothing
+            // apart there; and no finer bins divide what the masses' slack leaves open)
+            if (in_range <= SR_LIST || lb >= SR_BINS - 1) break;
             // the next round divides these bins
             const float w1 = width * (1.f / (SR_BINS - 1));
-            hi = lb >= SR_BINS - 1 ? fmaxf(__fsub_rn(mx, xb), hi) : lo + w1 * (lb + 1);
+            hi = lo + w1 * (lb + 1);
             lo = lo + w1 * fb;
         }
-        // top-k alone, the cut in the last bin: that one reaches down to the lowest value of the type (a mask), and no 512
-        // distances tell anything apart there.  So 512 bins of 2^shift keys each, counts alone: 9 bits a round.  (One
-        // row of 151936, k 1000, T 0.1: 45 us; 423 by bisection.)
-        while (!has_p && in_range > SR_LIST) {
-            const uint32_t ktop = to_top ? sr_key(mx) : sr_key(xa) - 1, kb = sr_key(xb);
-            if (ktop == kb) break;  // equal logits
-            const int buf = rounds++ & 1, shift = max(23 - __clz(ktop - kb), 0);
+    }
+    // ---- still more than the list holds: exact counts and masses of 512 bins of equal numbers of (key, index) pairs, 9
+    // bits a pass, of whole keys as long as there is more than one; down to a list, or among equal logits to the cut
+    bool found = false;
+    if (in_range > SR_LIST) {
+        constexpr int IB = 19;  // bits of an index
+        static_assert(SR_MAX_VOCAB == 1 << IB, "a pair is a key and an index");
+        auto place = [&](float v, int i) { return (u64)sr_key(v) << IB | (u64)(SR_MAX_VOCAB - 1 - i); };
+        u64 m_above = 0, need = ~0ull;
+        if (has_p) {
+            u64 m = 0;
             stream([&](float (&v)[E], int) {
 #pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (side(v[e]) == 0) atomicAdd(&S.cnt[buf][(ktop - sr_key(v[e])) >> shift], 1u);
+                for (int e = 0; e < E; e++) {
+                    const u64 w = v[e] >= xmin ? unit_of(v[e]) : 0;
+                    m += w;
+                    m_above += side(v[e]) > 0 ? w : 0;
+                }
             });
+            m = sr_reduce(m, S.red, addu);
+            m_above = sr_reduce(m_above, S.red, addu);
+            csync();  // (earlier uses of the slots are over)
+            if (tid < cs) {
+                SrShared *o = cl.map_shared_rank(&S, tid);
+                o->slot[0][rank] = m;
+                o->slot[1][rank] = m_above;
+            }
+            csync();
+            m = m_above = 0;
+            for (int i = 0; i < cs; i++) {
+                m += S.slot[0][i];
+                m_above += S.slot[1][i];
+            }
+            need = rule.need(m);
+        }
+        u64 top = (u64)(to_top ? sr_key(mx) : sr_key(xa) - 1) << IB | (SR_MAX_VOCAB - 1), low = (u64)sr_key(xb) << IB;
+        for (;;) {
+            const u64 span = top - low;
+            const int bits = 64 - __clzll((long long)span), shift = max(bits - 9, span >> IB ? IB : 0);
+            csync();  // the bins of the last pass have been read
+            for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[0][i] = S.mass[0][i] = S.mass[1][i] = 0;
+            __syncthreads();
+            stream([&](float (&v)[E], int i) {
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const u64 at = place(v[e], i + e);
+                    if (side(v[e]) != 0 || at > top || at < low) continue;
+                    const int b = (int)((top - at) >> shift);
+                    atomicAdd(&S.cnt[0][b], 1u);
+                    if (has_p) {  // (two 32-bit atomics and the carry: a 64-bit one in shared memory is a loop)
+                        const u64 w = unit_of(v[e]);
+                        const unsigned w32 = (unsigned)w, sum = atomicAdd(&S.mass[0][b], w32) + w32;
+                        atomicAdd(&S.mass[1][b], (unsigned)(w >> 32) + (sum < w32));
+                    }
+                }
+            });
+            if (tid == 0) S.first_bin = SR_BINS;
             csync();
             unsigned n[2] = {0, 0}, n_low[2] = {0, 0}, n_all;
+            u64 m[2] = {0, 0}, all;
             for (int i = 0; i < cs; i++) {
-                const uint2 c2 = *reinterpret_cast<const uint2 *>(&cl.map_shared_rank(&S, i)->cnt[buf][2 * tid]);
-                if (i == rank) {
-                    n_low[0] = n[0];
-                    n_low[1] = n[1];
+                const SrShared *o = cl.map_shared_rank(&S, i);
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    if (i == rank) n_low[k] = n[k];
+                    n[k] += o->cnt[0][2 * tid + k];
+                    m[k] += (u64)o->mass[1][2 * tid + k] << 32 | o->mass[0][2 * tid + k];
                 }
-                n[0] += c2.x;
-                n[1] += c2.y;
             }
             unsigned nb = c_above + sr_scan(n[0] + n[1], reinterpret_cast<unsigned *>(S.red), &n_all);
-            for (int i = tid; i < SR_BINS; i += SR_THREADS) S.cnt[buf ^ 1][i] = 0;
+            __syncthreads();
+            u64 mb = m_above + sr_scan(m[0] + m[1], S.red, &all);
+            const unsigned nb0 = nb;
+            const u64 mb0 = mb;
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                if (nb < (unsigned)rule.top_k && nb + n[k] >= (unsigned)rule.top_k) {  // (one bin: the range holds the cut)
-                    S.first_bin = 2 * tid + k;
-                    S.last_bin = (int)nb;
-                    S.range_count = n[k];
-                    S.range_low = n_low[k];
-                }
                 nb += n[k];
+                mb += m[k];
+                if (n[k] && ((rule.top_k && nb >= (unsigned)rule.top_k) || (has_p && mb >= need)))
+                    atomicMin(&S.first_bin, 2 * tid + k);
             }
             __syncthreads();
-            const uint32_t at = (uint32_t)S.first_bin, above = ktop - (at << shift) + 1, from = ktop - ((at + 1) << shift) + 1;
-            c_above = (unsigned)S.last_bin;
-            in_range = S.range_count;
-            to_top = to_top && at == 0;
-            if (!to_top) xa = sr_unkey(above);
-            if ((u64)(at + 1) << shift <= ktop - kb) xb = sr_unkey(from);
+            const int fb = S.first_bin;  // (the range holds the cut)
+            if (fb >> 1 == tid) {
+                const int k = fb & 1;
+                S.range_count = k ? n[1] : n[0];
+                S.range_low = k ? n_low[1] : n_low[0];
+                S.red[31] = nb0 + (k ? n[0] : 0);
+                S.target = mb0 + (k ? m[0] : 0);
+            }
             __syncthreads();
+            in_range = S.range_count;
+            c_above = (unsigned)S.red[31];
+            m_above = S.target;
+            const u64 end = (u64)(fb + 1) << shift;
+            if (end <= span) low = top - end + 1;
+            top -= (u64)fb << shift;
+            if (shift >= IB) {
+                to_top = to_top && (uint32_t)(top >> IB) == sr_key(mx);
+                if (!to_top) xa = sr_unkey((uint32_t)(top >> IB) + 1);
+                xb = sr_unkey((uint32_t)(low >> IB));
+                if (in_range <= SR_LIST) break;
+            }
+            if (shift == 0) {
+                cut = (top >> IB) << 32 | (uint32_t)~(uint32_t)(SR_MAX_VOCAB - 1 - (int)(top & (SR_MAX_VOCAB - 1)));
+                found = true;
+                break;
+            }
         }
     }
     // ---- exact masses: above the range (kept), and of all survivors where top-p needs it; the range to rank 0
-    const bool listed = in_range > 0 && in_range <= SR_LIST;
+    const bool listed = in_range > 0 && !found;
     const unsigned at0 = listed ? S.range_low : 0;  // the entries of the ranks before this one come first
     if (listed) {  // (in other cases a rank may still be reading rank 0's count)
         __syncthreads();
@@ -1024,46 +1092,7 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
     m_all = sr_reduce(m_all, S.red, addu);
     if (tid == 0) lead->slot[1][rank] = m_all;
     csync();
-    const bool bisect = in_range > SR_LIST;
-    if (bisect) {
-        // over (key, index) pairs: the largest pair whose upper set completes top_k or top_p
-        u64 above = 0, mass = 0;
-        for (int i = 0; i < cs; i++) {
-            mass += lead->slot[1][i];
-            for (int j = 0; j < SR_WARPS; j++) above += lead->seg[i * SR_WARPS + j];
-        }
-        const u64 need = has_p ? rule.need(mass) : ~0ull;
-        u64 lo_pair = 0, hi_pair = ~0ull;
-        while (hi_pair - lo_pair > 1) {
-            const u64 mid = lo_pair + (hi_pair - lo_pair) / 2;
-            u64 m = 0, n = 0;
-            stream([&](float (&v)[E], int i) {
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (side(v[e]) == 0 && sr_pair(v[e], i + e) >= mid) {
-                        n++;
-                        if (has_p) m += unit_of(v[e]);
-                    }
-            });
-            m = sr_reduce(m, S.red, addu);
-            n = sr_reduce(n, S.red, addu);
-            csync();  // the slots of the last turn have been read
-            if (tid < cs) {
-                SrShared *o = cl.map_shared_rank(&S, tid);
-                o->slot[0][rank] = m;
-                o->slot[1][rank] = n;
-            }
-            csync();
-            m = above;
-            n = c_above;
-            for (int i = 0; i < cs; i++) {
-                m += S.slot[0][i];
-                n += S.slot[1][i];
-            }
-            if ((rule.top_k && n >= (u64)rule.top_k) || (has_p && m >= need && m > 0)) lo_pair = mid;
-            else hi_pair = mid;
-        }
-        cut = lo_pair;
+    if (found) {
         stream([&](float (&v)[E], int i) {
 #pragma unroll
             for (int e = 0; e < E; e++)
