@@ -491,21 +491,31 @@ template <typename T> __global__ void __launch_bounds__(SR_THREADS, 3) k_sample_
         if (tid < 32) {
             const float g = (float)((double)mx + rule.t * log(rule.min_p));
             uint32_t k0 = sr_key(isfinite(g) ? g : g > 0.f ? 3.4028235e38f : -3.4028235e38f);
-            for (int it = 0; it < 64; it++) {  // (the guess is an ulp or two off at most)
+            const uint32_t kmax = sr_key(mx);
+            uint32_t found = 0;
+            for (int it = 0; it < 4 && !found; it++) {  // (the guess is an ulp or two off)
                 const uint32_t k = k0 + lane - 16;
                 const float v = sr_unkey(k);
                 const uint32_t ok = __ballot_sync(0xffffffffu, v <= mx && rule.weight(v, mx, S.table) >= rule.min_p) |
                                     __ballot_sync(0xffffffffu, v > mx);
-                if (ok && !(ok & 1)) {
-                    if (lane == 0) S.kmin = k0 + __ffs(ok) - 1 - 16;
-                    break;
-                }
-                if (mx == INFINITY || it == 63) {
-                    if (lane == 0) S.kmin = sr_key(mx);
-                    break;
-                }
+                if (ok && !(ok & 1)) found = k0 + __ffs(ok) - 1 - 16;
                 k0 += ok ? -31 : 31;
             }
+            if (!found && mx < INFINITY) {
+                // The guess comes out of two large numbers next to 0, where f32 has many more between; or no difference
+                // that f32 holds near the maximum counts at this T.  32 lanes close in.
+                uint32_t l = sr_key(-INFINITY), h = kmax;  // never l, always h
+                while (h - l > 1) {
+                    const uint32_t k = l + (uint32_t)(((u64)(h - l) * (lane + 1)) >> 5);
+                    const bool in = k >= h || (k > l && rule.weight(sr_unkey(k), mx, S.table) >= rule.min_p);
+                    const int w = __ffs(__ballot_sync(0xffffffffu, in)) - 1;
+                    const uint32_t nh = __shfl_sync(0xffffffffu, k, w), nl = __shfl_sync(0xffffffffu, k, max(w - 1, 0));
+                    h = min(nh, h);
+                    l = w > 0 ? nl : l;
+                }
+                found = h;
+            }
+            if (lane == 0) S.kmin = found ? found : kmax;
         }
         __syncthreads();
     }
