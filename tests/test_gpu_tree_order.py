@@ -8,7 +8,7 @@ import pytest
 
 import ferrite_b200 as fb
 from oracle import oracle as O
-from tree_reference import Batch, attention, fb_type, rounded, torch_type
+from tree_reference import Batch, attention, fb_type, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -69,4 +69,65 @@ def test_readers_and_writers_behind_the_attention(torch_cuda, kind, lens):
     if kind == "f32":
         assert (runs[0][4] != 7.0).any(dim=1).all()
     weight.close()
+    ctx.close()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_appends_behind_the_attention(torch_cuda, kind):
+    """Append, attend, overwrite the same cache places, attend again, captured and replayed: each attention sees the rows
+    appended before it and none of the later ones."""
+    torch = torch_cuda
+    rng = np.random.default_rng(3)
+    lens, n = [40 + i for i in range(16)], 20
+    B = Batch(rng, [n] * 16, lens, KV, DIM, PAGE)
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    row, kvrow = QH * DIM, KV * DIM
+    qd, _ = rounded(torch, rng.normal(0, 1, (B.total, QH, DIM)), kind)
+    rows = [rounded(torch, rng.normal(0, 1, (B.total, 2, KV, DIM)), kind)[0] for _ in range(4)]
+    k, v, off, ln, bt = t(B.k), t(B.v), t(B.offsets), t(np.array(lens, np.int32)), t(np.maximum(B.table, 0))
+    outs = [torch.empty_like(qd) for _ in rows]
+    stream = torch.cuda.Stream()
+    ctx = fb.Context(0, stream.cuda_stream)
+    capacity = B.max_pages * PAGE
+    longer = t(np.zeros((16, CAPACITY // PAGE), np.int32))
+    longer[:, :B.max_pages] = bt
+    ws = torch.empty(fb.attn_tree_workspace(ctx, 16, n, QH, KV, DIM, PAGE, CAPACITY), dtype=torch.uint8, device="cuda")
+
+    def step(i):
+        at = rows[i].data_ptr()
+        fb.kv_append(ctx, None, fb_type(fb, kind), at, 2 * kvrow, at + kvrow * rows[i].element_size(), 2 * kvrow, off.data_ptr(),
+                     ln.data_ptr(), 0, longer.data_ptr(), k.data_ptr(), v.data_ptr(), 16, B.total, n, KV, DIM, PAGE,
+                     CAPACITY // PAGE, B.num_pages)
+        fb.attn_tree(ctx, fb_type(fb, kind), qd.data_ptr(), row, k.data_ptr(), v.data_ptr(), longer.data_ptr(), off.data_ptr(),
+                     ln.data_ptr(), 0, 1, outs[i].data_ptr(), row, 16, B.total, n, QH, KV, DIM, PAGE, CAPACITY // PAGE,
+                     B.num_pages, CAPACITY, 0.09, ws.data_ptr(), ws.numel())
+
+    assert capacity < CAPACITY
+    want = []
+    torch.cuda.synchronize()
+    for i in range(4):
+        step(i)
+        stream.synchronize()
+        want.append(outs[i].clone())
+    assert not any(torch.equal(a, b) for a, b in zip(want, want[1:]))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        for i in range(4):
+            step(i)
+    for _ in range(3):
+        for o in outs:
+            o.fill_(7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        stream.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    for o in outs:
+        o.fill_(7.0)
+    torch.cuda.synchronize()
+    for i in range(4):
+        step(i)
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want)) and ctx.error_word() == 0
     ctx.close()
