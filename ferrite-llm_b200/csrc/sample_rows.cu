@@ -12,15 +12,15 @@
 // is unreachable.
 //
 // Bound: many rows by the first pass, which streams a row through registers once
-// (an exponential a logit where top-p asks: 53 % of the issue slots and 38 % of the
+// (an exponential a logit where top-p asks: 53 % of the issue slots and 37 % of the
 // special-function unit at 31 % of DRAM's rate; what comes later reads a few of a
 // row's vectors, or passes that find it in L2); a few rows by the steps of the
 // cluster that shares a row.  The first pass keeps
 // the maximum of every group of 16-byte vectors in shared memory.  Measured
 // (back to back in a graph): 400 rows of 151936 bf16 logits, top-k 50 and top-p,
 // in 45 us (48 us from cold caches, 2.5 TB/s: a row is one CTA and three of them
-// share an SM); 65 rows of 128256 f32 logits, top-p alone, in 74 us, some 16 us each
-// for counting into bins and for the exact masses; one row of 151936 in 8.6 us.  No
+// share an SM); 65 rows of 128256 f32 logits, top-p alone, in 75 us, some 16 us each
+// for counting into bins and for the exact masses; one row of 151936 in 8.7 us.  No
 // sort of the row:
 //  * min-p: the threshold logit is found exactly (the f32 whose binary64 weight
 //    is the first to reach min_p); the survivors are the candidates;
